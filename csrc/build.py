@@ -62,6 +62,10 @@ NATIVE_MODULE = {
 }
 
 
+# packed fp32 instructions (v_pk_add / mul / fma_f32) stay out of the device code
+NO_PACKED_FP32 = ["-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
+
+
 def build_hip(force=False, jobs=8):
     d = HIP_MODULE["src_dir"]
     hdrs = _headers(d)
@@ -75,7 +79,7 @@ def build_hip(force=False, jobs=8):
         objs.append(obj)
         if force or _stale(obj, [src] + hdrs):
             jobs_list.append([HIPCC, "-O3", f"--offload-arch={ARCH}", "-fPIC", "-std=c++17",
-                              "-munsafe-fp-atomics", "-c", src, "-o", obj] + inc)
+                              "-munsafe-fp-atomics", *NO_PACKED_FP32, "-c", src, "-o", obj] + inc)
     bind_src = os.path.join(d, "bind.cpp")
     bind_obj = os.path.join(BUILD, "hip_bind.cpp.o")
     objs.append(bind_obj)

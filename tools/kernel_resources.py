@@ -28,8 +28,8 @@ KEYS = ("vgpr_count", "agpr_count", "sgpr_count", "vgpr_spill_count", "sgpr_spil
 
 def device_asm(src: str, out_dir: str) -> str:
     out = os.path.join(out_dir, os.path.basename(src) + ".s")
-    cmd = [HIPCC, "-O3", "--offload-arch=gfx950", "-std=c++17", "-munsafe-fp-atomics", "--offload-device-only",
-           "-S", src, "-o", out, "-I" + HIP_DIR]
+    cmd = [HIPCC, "-O3", "--offload-arch=gfx950", "-std=c++17", "-munsafe-fp-atomics", "-Xclang", "-target-feature",
+           "-Xclang", "-packed-fp32-ops", "--offload-device-only", "-S", src, "-o", out, "-I" + HIP_DIR]
     r = subprocess.run(cmd, capture_output=True, text=True)
     if r.returncode != 0:
         raise RuntimeError(f"{' '.join(cmd)}\n{r.stderr[-2000:]}")
