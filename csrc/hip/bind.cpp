@@ -29,6 +29,11 @@ void ytk_split_find(uintptr_t, int, int, uintptr_t, uintptr_t, int, uintptr_t, i
                     float, float, float, float, double, double, uintptr_t, uintptr_t, uintptr_t,
                     uintptr_t, uintptr_t);
 void ytk_split_combine(uintptr_t, int, int, uintptr_t, int, int, uintptr_t, uintptr_t);
+// head.hip
+long long ytk_head_loss_ws(const long long*);
+void ytk_head_loss(const uintptr_t*, const long long*, double, uintptr_t);
+long long ytk_head_topk_ws(const long long*);
+void ytk_head_topk(const uintptr_t*, const long long*, double, uintptr_t);
 // gbst.hip
 int ytk_gbst_wide_max();
 void ytk_gbst_epilogue(uintptr_t, int, uintptr_t, uintptr_t, uintptr_t, uintptr_t, double, uintptr_t, int, int, int,
@@ -352,5 +357,21 @@ PYBIND11_MODULE(_ytk_hip, m) {
   m.def("seg_median", &ytk_seg_median);
   m.def("seg_prune", &ytk_seg_prune);
   m.def("owner_unpack", &ytk_owner_unpack);
+  m.def("head_loss_ws", [](const std::vector<long long>& lp) {
+    if (lp.size() != 19) throw std::invalid_argument("head_loss_ws: bad argument sizes");
+    return ytk_head_loss_ws(lp.data());
+  });
+  m.def("head_topk_ws", [](const std::vector<long long>& lp) {
+    if (lp.size() != 19) throw std::invalid_argument("head_topk_ws: bad argument sizes");
+    return ytk_head_topk_ws(lp.data());
+  });
+  m.def("head_loss", [](const std::vector<uintptr_t>& ptrs, const std::vector<long long>& lp, double temp, uintptr_t stream) {
+    if (ptrs.size() != 13 || lp.size() != 19) throw std::invalid_argument("head_loss: bad argument sizes");
+    ytk_head_loss(ptrs.data(), lp.data(), temp, stream);
+  });
+  m.def("head_topk", [](const std::vector<uintptr_t>& ptrs, const std::vector<long long>& lp, double temp, uintptr_t stream) {
+    if (ptrs.size() != 7 || lp.size() != 19) throw std::invalid_argument("head_topk: bad argument sizes");
+    ytk_head_topk(ptrs.data(), lp.data(), temp, stream);
+  });
   m.attr("arch") = "gfx950";
 }

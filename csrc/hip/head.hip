@@ -1,0 +1,1117 @@
+// Softmax class head over many classes (gfx950): z = (x w^T + b) / T for rows x [n, d] and classes w [V, d],
+// without ever holding n x V scores.
+//
+//   loss:    per-row targets q_j on classes v_j (one label, or a teacher's k best), lse = log sum_v e^z,
+//            loss = g T^2 sum_j q_j (log q_j + lse - z_j);  D = g T (s p - q), s = sum_j q_j, p = e^(z - lse);
+//            dx = D w, dw = D^T x, db = sum_i D
+//   top k:   the k largest z of each row and lse
+//
+// Rows are taken in pieces so that at most `piece_bytes` of exponentials live at a time. Per piece:
+//   1. scores_kernel   z by MFMA; per row and group of 64 classes the maximum m and sum s of e^(z - m); with
+//                      gradients also E = e^(z - m) (bf16 inputs: as fp16 scaled by 2^15, 11 bits, so that
+//                      the one rounding that matters is D's own to bf16; fp32 inputs: fp32)
+//   2. target_kernel   z of the target classes as plain fp32 dot products
+//   3. row_kernel      lse from the groups, loss, and the row's coefficients
+//   4. dscore_kernel   E -> D in place (fp32: three bf16 planes), bias gradient partials
+//   5. grad kernels    dx = D w, dw = D^T x
+// The scores are computed once: 6 n d V operations for a step, against 8 n d V where the scores are computed
+// again for the gradient.
+#include "head_gemm.h"
+
+#include <algorithm>
+#include <cstring>
+
+namespace ytk {
+
+constexpr int kGroup = 64;                         // classes per (m, s) pair
+constexpr float kLog2e = 1.4426950408889634f;
+
+// ------------------------------------------------------------------ scalar types
+template <typename T>
+struct Elem;
+template <>
+struct Elem<float> {
+  static __device__ __forceinline__ float get(const float* p, long long i) { return p[i]; }
+  static __device__ __forceinline__ void put(float* p, long long i, float v) { p[i] = v; }
+};
+template <>
+struct Elem<__bf16> {
+  static __device__ __forceinline__ float get(const __bf16* p, long long i) { return (float)p[i]; }
+  static __device__ __forceinline__ void put(__bf16* p, long long i, float v) { p[i] = (__bf16)v; }
+};
+
+// fp32 -> hi + mid + lo in bf16 (round to nearest each: |rest| <= 2^-27 of the value). Values that would round up to
+// infinity are cut instead; infinities and NaN stay in hi alone.
+__device__ __forceinline__ void split3(float v, __bf16& h, __bf16& m, __bf16& l) {
+  h = (__bf16)v;
+  if (!__builtin_isfinite((float)h)) {
+    if (__builtin_isfinite(v)) {
+      h = __builtin_bit_cast(__bf16, (unsigned short)(__builtin_bit_cast(unsigned, v) >> 16));
+    } else {
+      m = l = (__bf16)0.0f;
+      return;
+    }
+  }
+  const float r = v - (float)h;
+  m = (__bf16)r;
+  l = (__bf16)(r - (float)m);
+}
+
+// ------------------------------------------------------------------ operand layout
+// rows x cols of any strides -> kPlanes bf16 planes [rows][pitch/2], columns padded with zeros. Rows whose
+// `coef` is zero are written as zeros (ignored rows must not carry an infinity or NaN into 0 * x).
+template <typename T, int kPlanes>
+__global__ __launch_bounds__(256) void pack_kernel(const T* __restrict__ src, long long rs, long long cs, long long rows,
+                                                   int cols, __bf16* __restrict__ dst, long long ld, long long plane,
+                                                   const float* __restrict__ coef) {
+  __shared__ float tile[64][65];
+  const long long r0 = (long long)blockIdx.y * 64;
+  const int c0 = blockIdx.x * 64, t = threadIdx.x;
+  const bool by_row = cs == 1 || rs != 1;  // consecutive threads along the dimension that is dense in memory
+#pragma unroll 4
+  for (int i = t; i < 4096; i += 256) {
+    const int r = by_row ? i >> 6 : i & 63, c = by_row ? i & 63 : i >> 6;
+    float v = 0.0f;
+    if (r0 + r < rows && c0 + c < cols && (!coef || coef[r0 + r] != 0.0f)) v = Elem<T>::get(src, (r0 + r) * rs + (c0 + c) * cs);
+    tile[r][c] = v;
+  }
+  __syncthreads();
+  for (int i = t; i < 512; i += 256) {
+    const int r = i >> 3, c = (i & 7) * 8;
+    if (r0 + r >= rows || c0 + c >= ld) continue;
+    bf16x8 h, m, l;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      __bf16 a, b, e;
+      if (kPlanes == 3) {
+        split3(tile[r][c + j], a, b, e);
+        h[j] = a, m[j] = b, l[j] = e;
+      } else {
+        h[j] = (__bf16)tile[r][c + j];
+      }
+    }
+    __bf16* o = dst + (r0 + r) * ld + c0 + c;
+    *(bf16x8*)o = h;
+    if (kPlanes == 3) {
+      *(bf16x8*)(o + plane) = m;
+      *(bf16x8*)(o + 2 * plane) = l;
+    }
+  }
+}
+
+// ------------------------------------------------------------------ scores
+struct ScoreArgs {
+  Operand w, x;
+  long long K;        // padded d
+  int nkt, terms;
+  int V, n;
+  int nm, nn;         // tiles
+  const void* bias;   // element type of the inputs
+  int bias_f32;
+  float inv_t;
+  float2* stats;      // [groups][n]: m, s
+  void* e;            // E [n][ld] (fp16 or fp32) or null
+  float* z;           // scores [n][ld] or null
+  long long ld;
+};
+
+// lanes l and l + 32 hold rows 8q .. 8q+3 and 8q+4 .. 8q+7 of a 32-row block: exchange halves so that lane l has
+// all 8 values of quad pair 2p and lane l + 32 all 8 of 2p + 1 (16-byte stores of 16-bit values)
+__device__ __forceinline__ void swap_quads(unsigned& a0, unsigned& a1, unsigned& b0, unsigned& b1) {
+  auto p = __builtin_amdgcn_permlane32_swap(a0, b0, false, false);
+  auto q = __builtin_amdgcn_permlane32_swap(a1, b1, false, false);
+  a0 = p[0], a1 = q[0], b0 = p[1], b1 = q[1];
+}
+
+__device__ __forceinline__ unsigned pack_h2(float a, float b) {
+  typedef _Float16 h2 __attribute__((ext_vector_type(2)));
+  h2 v = {(_Float16)a, (_Float16)b};
+  return __builtin_bit_cast(unsigned, v);
+}
+__device__ __forceinline__ unsigned pack_b2(float a, float b) {
+  typedef __bf16 b2 __attribute__((ext_vector_type(2)));
+  b2 v = {(__bf16)a, (__bf16)b};
+  return __builtin_bit_cast(unsigned, v);
+}
+
+// e^v. kFine: the product v log2(e) is kept to twice the precision, since its rounding alone is |v| 2^-24 of the
+// result (fp32 inputs, whose gradients are wanted to fp32); bf16 inputs round D to 2^-9 anyway.
+template <bool kFine>
+__device__ __forceinline__ float exp_of(float v) {
+  const float t = v * kLog2e;
+  if (!kFine) return __builtin_amdgcn_exp2f(t);
+  const float r = fmaf(v, kLog2e, -t) + v * 1.925963033e-8f;  // log2(e) - kLog2e
+  const float e = __builtin_amdgcn_exp2f(t);
+  return e == 0.0f || v == -INFINITY ? 0.0f : fmaf(e * r, 0.6931471805599453f, e);
+}
+
+enum { kStatsOnly = 0, kExpHalf = 1, kExpFloat = 2, kScores = 3 };
+
+template <class C, int kMode>
+__global__ __launch_bounds__(C::kThreads) void scores_kernel(ScoreArgs p) {
+  int tm, tn;
+  if (!tile_of(p.nm, p.nn, tm, tn)) return;
+  f32x16 acc[C::kFM][C::kFN] = {};
+  gemm_loop<C, kKC, kKC>(p.w, p.x, tm * C::kBM, tn * C::kBN, p.K, p.K, 0, p.nkt, p.terms, acc);
+  static_assert(C::kFM % 2 == 0, "a wave holds whole groups");
+  const int wave = threadIdx.x >> 6, l = threadIdx.x & 63, hi = l >> 5;
+  const int v0 = tm * C::kBM + (wave / C::kWN) * C::kFM * 32, i0 = tn * C::kBN + (wave % C::kWN) * C::kFN * 32;
+#pragma unroll
+  for (int g = 0; g < C::kFM / 2; ++g) {
+    const int vg = v0 + g * kGroup;
+    if (vg >= p.V) break;
+    float b[2][16];
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) {
+        const int v = vg + h * 32 + 8 * (r >> 2) + 4 * hi + (r & 3);
+        b[h][r] = v >= p.V ? -INFINITY
+                  : !p.bias ? 0.0f
+                  : p.bias_f32 ? ((const float*)p.bias)[v]
+                               : (float)((const __bf16*)p.bias)[v];
+      }
+#pragma unroll
+    for (int j = 0; j < C::kFN; ++j) {
+      const int i = i0 + j * 32 + (l & 31);
+      float z[2][16], m = -INFINITY;
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+          // a class past the end is -inf whatever the product holds (its operand rows read as zero)
+          z[h][r] = (acc[2 * g + h][j][r] + b[h][r]) * p.inv_t;
+          m = fmaxf(m, z[h][r]);
+        }
+      m = fmaxf(m, __shfl_xor(m, 32, 64));
+      const float m0 = m == -INFINITY ? 0.0f : m;
+      float s = 0.0f;
+      if (kMode == kScores && i < p.n) {
+        float* o = p.z + (long long)i * p.ld + vg + 4 * hi;
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+          for (int q = 0; q < 4; ++q)
+            *(float4*)(o + h * 32 + 8 * q) = make_float4(z[h][4 * q], z[h][4 * q + 1], z[h][4 * q + 2], z[h][4 * q + 3]);
+      }
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+          z[h][r] = exp_of<kMode == kExpFloat>(z[h][r] - m0);
+          s += z[h][r];
+        }
+      s += __shfl_xor(s, 32, 64);
+      if (hi == 0 && i < p.n) p.stats[(long long)(vg / kGroup) * p.n + i] = make_float2(m, s);
+      if (kMode == kExpFloat && i < p.n) {
+        float* o = (float*)p.e + (long long)i * p.ld + vg + 4 * hi;
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+          for (int q = 0; q < 4; ++q)
+            *(float4*)(o + h * 32 + 8 * q) = make_float4(z[h][4 * q], z[h][4 * q + 1], z[h][4 * q + 2], z[h][4 * q + 3]);
+      }
+      if (kMode == kExpHalf) {
+        unsigned short* o = (unsigned short*)p.e + (long long)i * p.ld + vg + 8 * hi;
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+          for (int q = 0; q < 4; q += 2) {
+            const float k = 32768.0f;
+            unsigned a0 = pack_h2(z[h][4 * q] * k, z[h][4 * q + 1] * k), a1 = pack_h2(z[h][4 * q + 2] * k, z[h][4 * q + 3] * k);
+            unsigned b0 = pack_h2(z[h][4 * q + 4] * k, z[h][4 * q + 5] * k), b1 = pack_h2(z[h][4 * q + 6] * k, z[h][4 * q + 7] * k);
+            swap_quads(a0, a1, b0, b1);
+            if (i < p.n) *(uint4*)(o + h * 32 + 8 * q) = make_uint4(a0, a1, b0, b1);
+          }
+      }
+    }
+  }
+}
+
+// ------------------------------------------------------------------ targets
+// z of each row's target classes by plain fp32 dot products: one wave per row, x's row in registers is not
+// needed again often enough to hold, so both operands stream through L1.
+struct TargetArgs {
+  const void *x, *w, *bias;
+  long long xrs, xcs, wrs, wcs;
+  const void* idx;     // [n][k], int64 or int32
+  int idx64, k, n, d, V, f32;
+  float inv_t;
+  float* zt;           // [n][k]
+};
+
+__device__ __forceinline__ long long index_at(const void* p, int is64, long long i) {
+  return is64 ? ((const long long*)p)[i] : (long long)((const int*)p)[i];
+}
+
+template <typename T>
+__global__ __launch_bounds__(256) void target_kernel(TargetArgs p) {
+  const long long item = (long long)blockIdx.x * 4 + (threadIdx.x >> 6);
+  if (item >= (long long)p.n * p.k) return;
+  const int l = threadIdx.x & 63;
+  const long long row = item / p.k, v = index_at(p.idx, p.idx64, item);
+  float s = 0.0f;
+  if (v >= 0 && v < p.V) {
+    const T *x = (const T*)p.x + row * p.xrs, *w = (const T*)p.w + v * p.wrs;
+    float s2 = 0.0f;
+    int c = l;
+    for (; c + 64 < p.d; c += 128) {
+      s = fmaf(Elem<T>::get(x, c * p.xcs), Elem<T>::get(w, c * p.wcs), s);
+      s2 = fmaf(Elem<T>::get(x, (c + 64) * p.xcs), Elem<T>::get(w, (c + 64) * p.wcs), s2);
+    }
+    if (c < p.d) s = fmaf(Elem<T>::get(x, c * p.xcs), Elem<T>::get(w, c * p.wcs), s);
+    s = wave_sumf(s + s2);
+    if (p.bias) s += Elem<T>::get((const T*)p.bias, v);
+  }
+  if (l == 0) p.zt[item] = s * p.inv_t;
+}
+
+// ------------------------------------------------------------------ rows
+struct RowArgs {
+  const float2* stats;  // [groups][n]
+  int groups, n, base;  // base: one more class with score 0, index V
+  int V, k, mode;       // mode 0: label, 1: teacher list renormalised, 2: teacher list with its normaliser
+  const void* idx;
+  int idx64;
+  long long ignore;
+  const float *tl, *tlse, *weight, *zt;
+  float temp;
+  float *lse, *loss;    // outputs
+  float* coef;          // [n] g T s  (0: the row has no gradient)
+  float2* norm;         // [n] maximum and 1 / sum: p = e^(z - max) / sum, without the rounding of lse
+  float* q;             // [n][k] g T q_j
+  int rb;               // rows per block (a power of two, <= 16)
+};
+
+__global__ __launch_bounds__(256) void row_kernel(RowArgs p) {
+  __shared__ float sm[256], ss[256];
+  const int t = threadIdx.x, rl = t & (p.rb - 1), strip = t / p.rb, strips = 256 / p.rb;
+  const long long row = (long long)blockIdx.x * p.rb + rl;
+  // running maximum and sum over this thread's groups
+  float m = -INFINITY, s = 0.0f;
+  if (row < p.n) {
+    for (int g = strip; g < p.groups; g += strips) {
+      const float2 a = p.stats[(long long)g * p.n + row];
+      if (a.x > m) {
+        s = (m == -INFINITY ? 0.0f : s * exp_of<true>(m - a.x)) + a.y;
+        m = a.x;
+      } else if (a.x != -INFINITY) {
+        s += a.y * exp_of<true>(a.x - m);
+      } else if (a.y != 0.0f) {
+        s += a.y;  // NaN scores: the maximum passed over them
+      }
+    }
+    if (p.base && strip == 0) {
+      const float nm = fmaxf(m, 0.0f);
+      s = (m == -INFINITY ? 0.0f : s * exp_of<true>(m - nm)) + exp_of<true>(-nm);
+      m = nm;
+    }
+  }
+  sm[t] = m;
+  ss[t] = s;
+  __syncthreads();
+  for (int h = 128; h >= p.rb; h >>= 1) {
+    if (t < h) {
+      const float m1 = sm[t], m2 = sm[t + h], nm = fmaxf(m1, m2), n0 = nm == -INFINITY ? 0.0f : nm;
+      ss[t] = ss[t] * exp_of<true>(m1 - n0) + ss[t + h] * exp_of<true>(m2 - n0);
+      sm[t] = nm;
+    }
+    __syncthreads();
+  }
+  if (t < p.rb && row < p.n) {
+    if (p.norm) p.norm[row] = make_float2(sm[t], 1.0f / ss[t]);
+    sm[t] = sm[t] + logf(ss[t]);
+    p.lse[row] = sm[t];
+  }
+  __syncthreads();
+  if (!p.loss) return;
+  // targets: one wave per row in turn
+  const int wave = t >> 6, l = t & 63;
+  for (int r = wave; r < p.rb; r += 4) {
+    const long long i = (long long)blockIdx.x * p.rb + r;
+    if (i >= p.n) break;
+    const float lse = sm[r], g = p.weight ? p.weight[i] : 1.0f;
+    float norm = 0.0f;
+    if (p.mode == 1) {  // renormalise the list: log sum e^(t/T) over its entries
+      float mx = -INFINITY;
+      for (int j = l; j < p.k; j += 64)
+        if (index_at(p.idx, p.idx64, i * p.k + j) >= 0) mx = fmaxf(mx, p.tl[i * p.k + j] / p.temp);
+#pragma unroll
+      for (int o = 32; o; o >>= 1) mx = fmaxf(mx, __shfl_xor(mx, o, 64));
+      if (mx == -INFINITY) mx = 0.0f;
+      float e = 0.0f;
+      for (int j = l; j < p.k; j += 64)
+        if (index_at(p.idx, p.idx64, i * p.k + j) >= 0) e += expf(p.tl[i * p.k + j] / p.temp - mx);
+      e = wave_sumf(e);
+      norm = e == 0.0f ? 0.0f : mx + logf(e);  // nothing but -inf: every q_j is 0
+    } else if (p.mode == 2) {
+      norm = p.tlse[i];
+    }
+    float sq = 0.0f, ls = 0.0f;
+    for (int j = l; j < p.k; j += 64) {
+      const long long v = index_at(p.idx, p.idx64, i * p.k + j);
+      float q = 0.0f, term = 0.0f;
+      const bool skip = p.mode == 0 ? v == p.ignore : v < 0;
+      if (!skip) {
+        if (v < 0 || v >= p.V + p.base) {
+          term = NAN;  // a class that does not exist
+        } else {
+          const float lq = p.mode == 0 ? 0.0f : p.tl[i * p.k + j] / p.temp - norm;
+          q = p.mode == 0 ? 1.0f : expf(lq);
+          if (q > 0.0f || q != q) term = q * (lq + lse - p.zt[i * p.k + j]);
+        }
+      }
+      if (p.q) p.q[i * p.k + j] = q * g * p.temp;
+      sq += q;
+      ls += term;
+    }
+    sq = wave_sumf(sq);
+    ls = wave_sumf(ls);
+    if (l == 0) {
+      const float c = g * p.temp * sq;
+      p.loss[i] = (g == 0.0f || (sq == 0.0f && ls == ls)) ? 0.0f : g * p.temp * p.temp * ls;
+      if (p.coef) p.coef[i] = c;
+    }
+  }
+}
+
+// ------------------------------------------------------------------ score gradient
+struct DArgs {
+  const float2* stats;
+  const float2* norm;
+  const float *coef, *q, *zt;
+  const void* idx;
+  int idx64, n, V, k;
+  void* e;              // E in; bf16 inputs: D out in place
+  __bf16* d;            // fp32 inputs: D planes
+  long long ld, plane;
+  float* part;          // [row blocks][ld] bias gradient partials, or null
+};
+
+constexpr int kDRows = 64;    // rows per block
+constexpr int kDCols = 512;   // columns per block: one wave = one row's 512 columns, 8 per lane
+
+template <bool kF32>
+__global__ __launch_bounds__(256) void dscore_kernel(DArgs p) {
+  const int wave = threadIdx.x >> 6, l = threadIdx.x & 63;
+  const int c = blockIdx.x * kDCols + l * 8;
+  const long long r0 = (long long)blockIdx.y * kDRows;
+  const int r1 = (int)min((long long)kDRows, p.n - r0);
+  float db[8] = {};
+  const bool live = c < p.ld;
+  for (int r = wave; r < r1; r += 4) {
+    const long long i = r0 + r;
+    const float2 nr = p.norm[i];
+    const float c0w = p.coef[i], co = c0w * nr.y;
+    float d[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) d[j] = 0.0f;
+    if (c0w != 0.0f) {
+      if (live) {
+        const float m = p.stats[(long long)(c / kGroup) * p.n + i].x;
+        // E is e^(z - m) with m = 0 for a group that has only -inf
+        const float f = co * exp_of<kF32>((m == -INFINITY ? 0.0f : m) - nr.x);
+        if (kF32) {
+          const float4 *e = (const float4*)((const float*)p.e + i * p.ld + c), a = e[0], b = e[1];
+          d[0] = a.x * f, d[1] = a.y * f, d[2] = a.z * f, d[3] = a.w * f;
+          d[4] = b.x * f, d[5] = b.y * f, d[6] = b.z * f, d[7] = b.w * f;
+        } else {
+          typedef _Float16 h8 __attribute__((ext_vector_type(8)));
+          const h8 a = *(const h8*)((const _Float16*)p.e + i * p.ld + c);
+          const float k = f * (1.0f / 32768.0f);
+#pragma unroll
+          for (int j = 0; j < 8; ++j) d[j] = (float)a[j] * k;
+        }
+      }
+      // target classes: p is taken from the fp32 score, and every entry of the list on that class is subtracted
+      // (first all probabilities, then all targets: a class named twice is counted twice)
+      const int c0 = blockIdx.x * kDCols;
+#pragma unroll
+      for (int pass = 0; pass < 2; ++pass)
+        for (int j0 = 0; j0 < p.k; j0 += 64) {
+          const long long v = j0 + l < p.k ? index_at(p.idx, p.idx64, i * p.k + j0 + l) : -1;
+          const int at = v >= c0 && v < c0 + kDCols && v < p.V ? (int)(v - c0) : -1;
+          for (unsigned long long h = __ballot(at >= 0); h; h &= h - 1) {
+            const int b = __builtin_ctzll(h), vb = __builtin_amdgcn_readlane(at, b);
+            const long long e = i * p.k + j0 + b;
+            const float x = pass == 0 ? co * exp_of<kF32>(p.zt[e] - nr.x) : p.q[e];
+#pragma unroll
+            for (int u = 0; u < 8; ++u)
+              if (vb == l * 8 + u) d[u] = pass == 0 ? x : d[u] - x;
+          }
+        }
+    }
+    if (live) {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) db[j] += d[j];
+      if (kF32) {
+        bf16x8 h, m, lo;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          __bf16 a, b, e;
+          split3(d[j], a, b, e);
+          h[j] = a, m[j] = b, lo[j] = e;
+        }
+        __bf16* o = p.d + i * p.ld + c;
+        *(bf16x8*)o = h;
+        *(bf16x8*)(o + p.plane) = m;
+        *(bf16x8*)(o + 2 * p.plane) = lo;
+      } else {
+        *(uint4*)((unsigned short*)p.e + i * p.ld + c) =
+            make_uint4(pack_b2(d[0], d[1]), pack_b2(d[2], d[3]), pack_b2(d[4], d[5]), pack_b2(d[6], d[7]));
+      }
+    }
+  }
+  if (!p.part) return;
+  __shared__ float sh[4][kDCols];
+#pragma unroll
+  for (int j = 0; j < 8; ++j) sh[wave][l * 8 + j] = db[j];
+  __syncthreads();
+  for (int u = threadIdx.x; u < kDCols; u += 256) {
+    const int col = blockIdx.x * kDCols + u;
+    if (col < p.ld) p.part[(long long)blockIdx.y * p.ld + col] = (sh[0][u] + sh[1][u]) + (sh[2][u] + sh[3][u]);
+  }
+}
+
+// bias gradient: partials summed in block order; `acc` carries pieces of rows (first: overwritten)
+template <typename T>
+__global__ __launch_bounds__(256) void db_kernel(const float* __restrict__ part, int nb, long long ld, int V,
+                                                 float* __restrict__ acc, int first, T* __restrict__ out) {
+  const int v = blockIdx.x * 256 + threadIdx.x;
+  if (v >= V) return;
+  float s = first ? 0.0f : acc[v];
+  for (int b = 0; b < nb; ++b) s += part[b * ld + v];
+  if (out)
+    Elem<T>::put(out, v, s);
+  else
+    acc[v] = s;
+}
+
+// ------------------------------------------------------------------ gradient products
+struct GradArgs {
+  Operand a, b;
+  long long ka, kb;        // extent of K in each operand's memory
+  int nkt, terms, splits;  // K steps in all, cut into `splits` runs
+  int M, N, nm, nn;        // result [N][M], M contiguous
+  void* out;               // T [N][ldo]
+  long long ldo;
+  float* acc;              // [splits][N][M] fp32
+  int mode;                // 0: out = C  1: acc[split] = C  2: acc += C  3: out = acc + C
+};
+
+template <class C, int kLA, int kLB, typename T>
+__global__ __launch_bounds__(C::kThreads) void grad_kernel(GradArgs p) {
+  int tm, tn;
+  if (!tile_of(p.nm, p.nn * p.splits, tm, tn)) return;
+  const int split = tn / p.nn;
+  tn -= split * p.nn;
+  const int per = (p.nkt + p.splits - 1) / p.splits, kt0 = split * per, nkt = min(per, p.nkt - kt0);
+  f32x16 acc[C::kFM][C::kFN] = {};
+  if (nkt > 0) gemm_loop<C, kLA, kLB>(p.a, p.b, tm * C::kBM, tn * C::kBN, p.ka, p.kb, kt0, nkt, p.terms, acc);
+  const int wave = threadIdx.x >> 6, l = threadIdx.x & 63, hi = l >> 5;
+  const int m0 = tm * C::kBM + (wave / C::kWN) * C::kFM * 32, n0 = tn * C::kBN + (wave % C::kWN) * C::kFN * 32;
+  const bool vec = (p.ldo & 7) == 0 && ((uintptr_t)p.out & 15) == 0, avec = (p.M & 3) == 0;
+#pragma unroll
+  for (int j = 0; j < C::kFN; ++j) {
+    const int n = n0 + j * 32 + (l & 31);
+    if (n >= p.N) continue;
+#pragma unroll
+    for (int i = 0; i < C::kFM; ++i)
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        const int m = m0 + i * 32 + 8 * q + 4 * hi;
+        if (m >= p.M) continue;
+        float v[4] = {acc[i][j][4 * q], acc[i][j][4 * q + 1], acc[i][j][4 * q + 2], acc[i][j][4 * q + 3]};
+        if (p.mode) {
+          float* a = p.acc + ((long long)split * p.N + n) * p.M + m;
+          if (avec) {
+            if (p.mode != 1) {
+              const float4 o = *(const float4*)a;
+              v[0] += o.x, v[1] += o.y, v[2] += o.z, v[3] += o.w;
+            }
+            if (p.mode != 3) *(float4*)a = make_float4(v[0], v[1], v[2], v[3]);
+          } else {
+            for (int u = 0; u < 4; ++u)
+              if (m + u < p.M) {
+                if (p.mode != 1) v[u] += a[u];
+                if (p.mode != 3) a[u] = v[u];
+              }
+          }
+        }
+        if (p.mode == 0 || p.mode == 3) {
+          T* o = (T*)p.out + (long long)n * p.ldo + m;
+          if (vec && m + 4 <= p.M) {
+            if (sizeof(T) == 4)
+              *(float4*)o = make_float4(v[0], v[1], v[2], v[3]);
+            else
+              *(uint2*)o = make_uint2(pack_b2(v[0], v[1]), pack_b2(v[2], v[3]));
+          } else {
+            for (int u = 0; u < 4; ++u)
+              if (m + u < p.M) Elem<T>::put(o, u, v[u]);
+          }
+        }
+      }
+  }
+}
+
+// out = sum over splits, in split order
+template <typename T>
+__global__ __launch_bounds__(256) void split_sum_kernel(const float* __restrict__ acc, int splits, long long rows, int cols,
+                                                        T* __restrict__ out, long long ldo) {
+  const long long total = rows * cols;
+  for (long long i = blockIdx.x * 256LL + threadIdx.x; i < total; i += (long long)gridDim.x * 256) {
+    float s = 0.0f;
+    for (int k = 0; k < splits; ++k) s += acc[k * total + i];
+    Elem<T>::put(out, i / cols * ldo + i % cols, s);
+  }
+}
+
+// ------------------------------------------------------------------ top k
+// One block per row. Scores are in z [n][ld], group maxima in stats. With kc = k + kSpare candidates:
+//   1. the kc-th largest group maximum tau (radix select); the kc best of all scores lie in the kc groups with the
+//      largest maxima, ties to the lower group: each of them holds a score that beats everything outside
+//   2. the scores >= tau of those groups, as 64-bit keys (score order, then lower class)
+//   3. the kc largest keys
+//   4. their scores again as 64-bit sums, so that the order returned is that of the exact scores, and
+//      the k largest of them in order
+constexpr int kSpare = 8;
+constexpr int kTopMax = 256;       // k at most
+constexpr int kTopKeys = 16384;    // group keys held in LDS; beyond, they are read again from memory
+
+struct TopArgs {
+  const float2* stats;
+  const float* z;
+  long long ld;
+  int n, V, d, groups, kc, k;
+  const void *x, *w, *bias;
+  long long xrs, xcs, wrs, wcs;
+  double inv_t;
+  float* values;
+  long long* classes;
+};
+
+__device__ __forceinline__ unsigned order_key(float v) {
+  if (v != v) return 0xffffffffu;  // NaN above everything
+  const unsigned u = __builtin_bit_cast(unsigned, v);
+  return u & 0x80000000u ? ~u : u | 0x80000000u;
+}
+__device__ __forceinline__ unsigned long long order_key(double v) {
+  if (v != v) return ~0ull;
+  const unsigned long long u = __builtin_bit_cast(unsigned long long, v);
+  return u >> 63 ? ~u : u | 1ull << 63;
+}
+
+// k-th largest (k >= 1) of `count` keys; on return `above` keys are larger than the result. All threads call it.
+template <typename K, class F>
+__device__ K radix_kth(int count, int k, F key, int* hist, int* pick, int& above) {
+  K found = 0, mask = 0;
+  above = 0;
+  for (int shift = (int)sizeof(K) * 8 - 8; shift >= 0; shift -= 8) {
+    for (int b = threadIdx.x; b < 256; b += blockDim.x) hist[b] = 0;
+    __syncthreads();
+    for (int i = threadIdx.x; i < count; i += blockDim.x) {
+      const K v = key(i);
+      if ((v & mask) == found) atomicAdd(&hist[(int)(v >> shift) & 255], 1);
+    }
+    __syncthreads();
+    if (threadIdx.x < 64) {  // bins from the top, four per lane
+      int c[4], sum = 0;
+#pragma unroll
+      for (int u = 0; u < 4; ++u) sum += c[u] = hist[255 - (threadIdx.x * 4 + u)];
+      int incl = sum;
+#pragma unroll
+      for (int o = 1; o < 64; o <<= 1) {
+        const int t = __shfl_up(incl, o, 64);
+        if ((int)threadIdx.x >= o) incl += t;
+      }
+      int before = incl - sum;
+      const int want = k - above;
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        if (before < want && want <= before + c[u]) {
+          pick[0] = 255 - (threadIdx.x * 4 + u);
+          pick[1] = before;
+        }
+        before += c[u];
+      }
+    }
+    __syncthreads();
+    found |= (K)pick[0] << shift;
+    mask |= (K)255 << shift;
+    above += pick[1];
+  }
+  __syncthreads();
+  return found;
+}
+
+template <typename T>
+__global__ __launch_bounds__(256) void topk_kernel(TopArgs p) {
+  extern __shared__ __align__(16) char head_smem[];
+  __shared__ int hist[256], pick[2], cnt, wcnt[4];
+  __shared__ int sel[kTopMax + kSpare];
+  __shared__ double zs[kTopMax + kSpare];
+  __shared__ int cls[kTopMax + kSpare];
+  unsigned long long* keys = (unsigned long long*)head_smem;  // kc * kGroup
+  unsigned* gk = (unsigned*)head_smem;                        // groups; done with before the keys are written
+  const int row = blockIdx.x, t = threadIdx.x, wave = t >> 6, l = t & 63;
+  const bool held = p.groups <= kTopKeys;
+  const float2* st = p.stats + row;
+  int nsel = p.groups;
+  unsigned tau = 0;
+  if (p.groups > p.kc) {
+    if (held)
+      for (int g = t; g < p.groups; g += 256) gk[g] = order_key(st[(long long)g * p.n].x);
+    __syncthreads();
+    auto gkey = [&](int g) { return held ? gk[g] : order_key(st[(long long)g * p.n].x); };
+    int above;
+    tau = radix_kth<unsigned>(p.groups, p.kc, gkey, hist, pick, above);
+    const int equal = p.kc - above;  // of the groups at tau, the first `equal`
+    if (t == 0) cnt = 0;
+    __syncthreads();
+    int seen = 0;
+    for (int g0 = 0; g0 < p.groups; g0 += 256) {
+      const unsigned key = g0 + t < p.groups ? gkey(g0 + t) : 0u;
+      const bool in = g0 + t < p.groups, eq = in && key == tau;
+      const unsigned long long m = __ballot(eq);
+      if (l == 0) wcnt[wave] = __popcll(m);
+      __syncthreads();
+      int rank = seen + __popcll(m & ((1ull << l) - 1));
+      for (int w = 0; w < 4; ++w) {
+        if (w < wave) rank += wcnt[w];
+        seen += wcnt[w];
+      }
+      if ((in && key > tau) || (eq && rank < equal)) sel[atomicAdd(&cnt, 1)] = g0 + t;
+      __syncthreads();
+    }
+    nsel = p.kc;
+  }
+  if (t == 0) cnt = 0;
+  __syncthreads();
+  const float* z = p.z + (long long)row * p.ld;
+  for (int s = wave; s < nsel; s += 4) {
+    const int v = (p.groups > p.kc ? sel[s] : s) * kGroup + l;
+    const unsigned o = v < p.V ? order_key(z[v]) : 0u;
+    const bool take = v < p.V && o >= tau;
+    const unsigned long long m = __ballot(take);
+    int base = 0;
+    if (l == 0) base = atomicAdd(&cnt, __popcll(m));
+    base = __builtin_amdgcn_readfirstlane(base);
+    if (take) keys[base + __popcll(m & ((1ull << l) - 1))] = (unsigned long long)o << 32 | (unsigned)~v;
+  }
+  __syncthreads();
+  const int total = cnt;
+  unsigned long long least = 0;
+  if (total > p.kc) {
+    int above;
+    least = radix_kth<unsigned long long>(total, p.kc, [&](int i) { return keys[i]; }, hist, pick, above);
+  }
+  if (t == 0) cnt = 0;
+  __syncthreads();
+  for (int i = t; i < total; i += 256)
+    if (keys[i] >= least) cls[atomicAdd(&cnt, 1)] = (int)~(unsigned)keys[i];
+  __syncthreads();
+  // exact scores of the kc candidates, a wave each
+  const T *x = (const T*)p.x + row * p.xrs, *bias = (const T*)p.bias;
+  for (int c = wave; c < p.kc; c += 4) {
+    const T* w = (const T*)p.w + (long long)cls[c] * p.wrs;
+    double s = 0.0;
+    for (int j = l; j < p.d; j += 64) s = fma((double)Elem<T>::get(x, j * p.xcs), (double)Elem<T>::get(w, j * p.wcs), s);
+    s = wave_sum(s);
+    if (l == 0) zs[c] = (s + (bias ? (double)Elem<T>::get(bias, cls[c]) : 0.0)) * p.inv_t;
+  }
+  __syncthreads();
+  for (int c = t; c < p.kc; c += 256) {
+    const unsigned long long mine = order_key(zs[c]);
+    const int v = cls[c];
+    int rank = 0;
+    for (int o = 0; o < p.kc; ++o) {
+      const unsigned long long other = order_key(zs[o]);
+      rank += other > mine || (other == mine && cls[o] < v);
+    }
+    if (rank < p.k) {
+      p.values[(long long)row * p.k + rank] = (float)zs[c];
+      p.classes[(long long)row * p.k + rank] = v;
+    }
+  }
+}
+
+// ------------------------------------------------------------------ host side
+inline int grid8(long long tiles) { return (int)((tiles + 7) / 8 * 8); }
+
+typedef TileCfg<256, 256, 2, 4, 2> CfgBig;
+typedef TileCfg<128, 128, 2, 2, 2> CfgMid;
+typedef TileCfg<128, 32, 2, 1, 4> CfgSlim;
+
+template <class C>
+void scores_launch(ScoreArgs p, int mode, hipStream_t s) {
+  p.nm = ceil_div(p.V, C::kBM);
+  p.nn = ceil_div(p.n, C::kBN);
+  const int g = grid8((long long)p.nm * p.nn);
+#define YTK_SC(M)                                                    \
+  {                                                                  \
+    scores_kernel<C, M><<<g, C::kThreads, C::kLds, s>>>(p);          \
+  }
+  if (mode == kStatsOnly) YTK_SC(kStatsOnly)
+  else if (mode == kExpHalf) YTK_SC(kExpHalf)
+  else if (mode == kExpFloat) YTK_SC(kExpFloat)
+  else YTK_SC(kScores)
+#undef YTK_SC
+  YTK_LAUNCH_CHECK();
+}
+
+template <class C, int LA, int LB, typename T>
+void grad_launch(GradArgs p, hipStream_t s) {
+  p.nm = ceil_div(p.M, C::kBM);
+  p.nn = ceil_div(p.N, C::kBN);
+  grad_kernel<C, LA, LB, T><<<grid8((long long)p.nm * p.nn * p.splits), C::kThreads, C::kLds, s>>>(p);
+  YTK_LAUNCH_CHECK();
+}
+
+}  // namespace ytk
+
+using namespace ytk;
+
+// ------------------------------------------------------------------ plan
+// Sizes and workspace of one call. The same code lays the workspace out for the size query and for the call.
+struct HeadIn {  // lp of the entry points, in this order
+  long long n, d, V, k, f32, xrs, xcs, wrs, wcs, idx64, ignore, base, mode, want_dx, want_dw, has_bias, piece_bytes, x_al, w_al;
+};
+constexpr int kHeadIn = 19;
+
+static HeadIn head_in(const long long* lp) {
+  HeadIn h;
+  static_assert(sizeof(HeadIn) == kHeadIn * sizeof(long long), "");
+  memcpy(&h, lp, sizeof(h));
+  if (h.n < 1 || h.d < 1 || h.V < 1 || h.k < 1) throw std::invalid_argument("class head: empty problem");
+  if (h.V > (1LL << 22) - 64 || h.d > (1LL << 22) - 64 || h.n > (1LL << 31) - 65536)
+    throw std::invalid_argument("class head: more than 4M classes or features, or 2G rows");
+  return h;
+}
+
+struct HeadPlan {
+  int planes, terms;
+  long long kp, ld, groups, piece;
+  bool pack_x, pack_w, grads;
+  int splits_dx, splits_dw;
+  bool many;  // more than one piece of rows
+  long long o_x, o_w, o_xg, o_e, o_d, o_stats, o_zt, o_q, o_coef, o_norm, o_part, o_dbacc, o_dwacc, o_split, bytes;
+};
+
+static long long up(long long v, long long m) { return (v + m - 1) / m * m; }
+
+// Big tiles when they fill the card's 256 CUs, otherwise a quarter of the size
+static bool use_big(long long m, long long n) {
+  return (long long)ceil_div(m, CfgBig::kBM) * ceil_div(n, CfgBig::kBN) >= 256;
+}
+
+// runs of the K dimension so that a product with few tiles still fills the card (about two blocks per CU); each
+// run keeps at least 8 K steps
+static int split_of(long long m, long long n, long long nkt) {
+  if (use_big(m, n)) return 1;
+  const long long tiles = (long long)ceil_div(m, CfgMid::kBM) * ceil_div(n, CfgMid::kBN);
+  return (int)std::max(1LL, std::min(std::min(512 / std::max(tiles, 1LL), nkt / 8), 64LL));
+}
+
+static HeadPlan head_plan(const HeadIn& h, bool topk) {
+  HeadPlan p = {};
+  p.planes = h.f32 ? 3 : 1;
+  p.terms = h.f32 ? 6 : 1;
+  p.kp = up(h.d, 64);
+  p.ld = up(h.V, 64);
+  p.groups = p.ld / kGroup;
+  p.grads = h.want_dx || h.want_dw;
+  p.pack_x = h.f32 || !h.x_al;
+  p.pack_w = h.f32 || !h.w_al;
+  const long long per = topk ? p.ld * 4 : p.grads ? p.ld * (h.f32 ? 10 : 2) : p.groups * 8;
+  p.piece = std::min(h.n, std::max(256LL, h.piece_bytes / per / 256 * 256));
+  p.many = p.piece < h.n;
+  p.splits_dx = h.want_dx ? split_of(h.d, p.piece, p.ld / 64) : 1;
+  p.splits_dw = h.want_dw && !p.many ? split_of(h.d, h.V, ceil_div(p.piece, 64)) : 1;
+  long long o = 0;
+  auto take = [&](bool want, long long bytes) {
+    const long long at = o;
+    if (want) o += up(bytes, 256);
+    return at;
+  };
+  p.o_x = take(p.pack_x, h.n * p.kp * 2 * p.planes);
+  p.o_w = take(p.pack_w, h.V * p.kp * 2 * p.planes);
+  p.o_xg = take(h.want_dw, p.piece * p.kp * 2 * p.planes);
+  p.o_e = take(p.grads || topk, p.piece * p.ld * (h.f32 || topk ? 4 : 2));
+  p.o_d = take(p.grads && h.f32, p.piece * p.ld * 6);
+  p.o_stats = take(true, p.groups * p.piece * 8);
+  p.o_zt = take(!topk, p.piece * h.k * 4);
+  p.o_q = take(p.grads, p.piece * h.k * 4);
+  p.o_coef = take(p.grads, p.piece * 4);
+  p.o_norm = take(p.grads, p.piece * 8);
+  const bool db = h.want_dw && h.has_bias;
+  p.o_part = take(db, ceil_div(p.piece, kDRows) * p.ld * 4);
+  p.o_dbacc = take(db, h.V * 4);
+  p.o_dwacc = take(h.want_dw && p.many, h.V * h.d * 4);
+  p.o_split = take(p.splits_dx > 1 || p.splits_dw > 1,
+                   std::max(p.splits_dx > 1 ? p.splits_dx * p.piece * h.d : 0, p.splits_dw > 1 ? p.splits_dw * h.V * h.d : 0) * 4);
+  p.bytes = o;
+  return p;
+}
+
+template <typename T>
+static void pack(const void* src, long long rs, long long cs, long long rows, long long cols, char* dst, long long ld,
+                 const float* coef, hipStream_t s) {
+  const dim3 g(ceil_div(ld, 64), ceil_div(rows, 64));
+  pack_kernel<T, sizeof(T) == 4 ? 3 : 1><<<g, 256, 0, s>>>((const T*)src, rs, cs, rows, (int)cols, (__bf16*)dst, ld, rows * ld, coef);
+  YTK_LAUNCH_CHECK();
+}
+
+// grid.y is at most 65535: rows beyond 64 * 65535 go in further launches, planes keep the distance of the whole
+template <typename T>
+static void pack_rows(const void* src, long long rs, long long cs, long long rows, long long cols, char* dst, long long ld,
+                      const float* coef, hipStream_t s) {
+  constexpr long long kMost = 64LL * 65535;
+  if (rows <= kMost) return pack<T>(src, rs, cs, rows, cols, dst, ld, coef, s);
+  for (long long r = 0; r < rows; r += kMost) {
+    const long long m = std::min(kMost, rows - r);
+    const dim3 g(ceil_div(ld, 64), ceil_div(m, 64));
+    pack_kernel<T, sizeof(T) == 4 ? 3 : 1><<<g, 256, 0, s>>>((const T*)src + r * rs, rs, cs, m, (int)cols, (__bf16*)dst + r * ld, ld,
+                                                              rows * ld, coef ? coef + r : nullptr);
+    YTK_LAUNCH_CHECK();
+  }
+}
+
+template <int LA, int LB, typename T>
+static void grad_product(GradArgs g, bool big, hipStream_t s) {
+  if (big)
+    grad_launch<CfgBig, LA, LB, T>(g, s);
+  else
+    grad_launch<CfgMid, LA, LB, T>(g, s);
+}
+
+template <typename T>
+static void split_sum(const float* acc, int splits, long long rows, long long cols, void* out, hipStream_t s) {
+  const int blocks = (int)std::min<long long>((rows * cols + 255) / 256, 4096);
+  split_sum_kernel<T><<<blocks, 256, 0, s>>>(acc, splits, rows, (int)cols, (T*)out, cols);
+  YTK_LAUNCH_CHECK();
+}
+
+struct HeadOps {  // operands of the products for one call
+  Operand w, x;
+};
+
+static HeadOps head_operands(const HeadIn& h, const HeadPlan& p, const void* x, const void* w, char* ws, hipStream_t s) {
+  HeadOps o;
+  if (p.pack_x) {
+    if (h.f32)
+      pack_rows<float>(x, h.xrs, h.xcs, h.n, h.d, ws + p.o_x, p.kp, nullptr, s);
+    else
+      pack_rows<__bf16>(x, h.xrs, h.xcs, h.n, h.d, ws + p.o_x, p.kp, nullptr, s);
+    o.x = {ws + p.o_x, p.kp * 2, h.n * p.kp * 2, (int)h.n};
+  } else {
+    o.x = {(const char*)x, h.xrs * 2, 0, (int)h.n};
+  }
+  if (p.pack_w) {
+    if (h.f32)
+      pack_rows<float>(w, h.wrs, h.wcs, h.V, h.d, ws + p.o_w, p.kp, nullptr, s);
+    else
+      pack_rows<__bf16>(w, h.wrs, h.wcs, h.V, h.d, ws + p.o_w, p.kp, nullptr, s);
+    o.w = {ws + p.o_w, p.kp * 2, h.V * p.kp * 2, (int)h.V};
+  } else {
+    o.w = {(const char*)w, h.wrs * 2, 0, (int)h.V};
+  }
+  return o;
+}
+
+static Operand rows_from(Operand o, long long r0, long long rows) {
+  o.p += r0 * o.pitch;
+  o.ext = (int)rows;
+  return o;
+}
+
+static void scores(const HeadIn& h, const HeadPlan& p, const HeadOps& o, long long r0, long long rows, const void* bias, float temp,
+                   char* ws, int mode, hipStream_t s) {
+  ScoreArgs a = {};
+  a.w = o.w;
+  a.x = rows_from(o.x, r0, rows);
+  a.K = p.kp;
+  a.nkt = (int)(p.kp / 64);
+  a.terms = p.terms;
+  a.V = (int)h.V;
+  a.n = (int)rows;
+  a.bias = bias;
+  a.bias_f32 = (int)h.f32;
+  a.inv_t = 1.0f / temp;
+  a.stats = (float2*)(ws + p.o_stats);
+  a.e = ws + p.o_e;
+  a.z = (float*)(ws + p.o_e);
+  a.ld = p.ld;
+  if (rows <= 64)
+    scores_launch<CfgSlim>(a, mode, s);
+  else if (use_big(h.V, rows))
+    scores_launch<CfgBig>(a, mode, s);
+  else
+    scores_launch<CfgMid>(a, mode, s);
+}
+
+static void rows_pass(RowArgs a, hipStream_t s) {
+  a.rb = 1;
+  while (a.rb < 16 && a.rb < a.n) a.rb *= 2;
+  row_kernel<<<ceil_div(a.n, a.rb), 256, 0, s>>>(a);
+  YTK_LAUNCH_CHECK();
+}
+
+extern "C" long long ytk_head_loss_ws(const long long* lp) { return head_plan(head_in(lp), false).bytes; }
+
+// ptrs: x, w, bias, idx, tl, tlse, weight, ws, loss, lse, dx, dw, db
+extern "C" void ytk_head_loss(const uintptr_t* ptrs, const long long* lp, double temp_, uintptr_t stream) {
+  const HeadIn h = head_in(lp);
+  const HeadPlan p = head_plan(h, false);
+  hipStream_t s = (hipStream_t)stream;
+  const float temp = (float)temp_;
+  const char *x = (const char*)ptrs[0], *idx = (const char*)ptrs[3];
+  const void *w = (const void*)ptrs[1], *bias = (const void*)ptrs[2];
+  const float *tl = (const float*)ptrs[4], *tlse = (const float*)ptrs[5], *weight = (const float*)ptrs[6];
+  char* ws = (char*)ptrs[7];
+  float *loss = (float*)ptrs[8], *lse = (float*)ptrs[9];
+  const int el = h.f32 ? 4 : 2;
+  const HeadOps o = head_operands(h, p, x, w, ws, s);
+  for (long long r0 = 0; r0 < h.n; r0 += p.piece) {
+    const long long rows = std::min(p.piece, h.n - r0);
+    const bool first = r0 == 0, last = r0 + rows == h.n;
+    scores(h, p, o, r0, rows, bias, temp, ws, !p.grads ? kStatsOnly : h.f32 ? kExpFloat : kExpHalf, s);
+    TargetArgs t = {};
+    t.x = x + r0 * h.xrs * el;
+    t.w = w;
+    t.bias = bias;
+    t.xrs = h.xrs, t.xcs = h.xcs, t.wrs = h.wrs, t.wcs = h.wcs;
+    t.idx = idx + r0 * h.k * (h.idx64 ? 8 : 4);
+    t.idx64 = (int)h.idx64;
+    t.k = (int)h.k, t.n = (int)rows, t.d = (int)h.d, t.V = (int)h.V, t.f32 = (int)h.f32;
+    t.inv_t = 1.0f / temp;
+    t.zt = (float*)(ws + p.o_zt);
+    if (h.f32)
+      target_kernel<float><<<ceil_div(rows * h.k, 4), 256, 0, s>>>(t);
+    else
+      target_kernel<__bf16><<<ceil_div(rows * h.k, 4), 256, 0, s>>>(t);
+    YTK_LAUNCH_CHECK();
+    RowArgs r = {};
+    r.stats = (const float2*)(ws + p.o_stats);
+    r.groups = (int)p.groups, r.n = (int)rows, r.base = (int)h.base;
+    r.V = (int)h.V, r.k = (int)h.k, r.mode = (int)h.mode;
+    r.idx = t.idx, r.idx64 = t.idx64, r.ignore = h.ignore;
+    r.tl = tl ? tl + r0 * h.k : nullptr, r.tlse = tlse ? tlse + r0 : nullptr;
+    r.weight = weight ? weight + r0 : nullptr;
+    r.zt = t.zt, r.temp = temp;
+    r.lse = lse + r0, r.loss = loss + r0;
+    r.coef = p.grads ? (float*)(ws + p.o_coef) : nullptr;
+    r.q = p.grads ? (float*)(ws + p.o_q) : nullptr;
+    r.norm = p.grads ? (float2*)(ws + p.o_norm) : nullptr;
+    rows_pass(r, s);
+    if (!p.grads) continue;
+
+    const bool db = h.want_dw && h.has_bias;
+    DArgs d = {};
+    d.stats = r.stats, d.norm = r.norm, d.coef = r.coef, d.q = r.q, d.zt = r.zt;
+    d.idx = t.idx, d.idx64 = t.idx64, d.n = (int)rows, d.V = (int)h.V, d.k = (int)h.k;
+    d.e = ws + p.o_e, d.d = (__bf16*)(ws + p.o_d), d.ld = p.ld, d.plane = rows * p.ld;
+    d.part = db ? (float*)(ws + p.o_part) : nullptr;
+    const dim3 dg(ceil_div(p.ld, kDCols), ceil_div(rows, kDRows));
+    if (h.f32)
+      dscore_kernel<true><<<dg, 256, 0, s>>>(d);
+    else
+      dscore_kernel<false><<<dg, 256, 0, s>>>(d);
+    YTK_LAUNCH_CHECK();
+    if (db) {
+      float* acc = (float*)(ws + p.o_dbacc);
+      if (h.f32)
+        db_kernel<float><<<ceil_div(h.V, 256), 256, 0, s>>>(d.part, (int)dg.y, p.ld, (int)h.V, acc, first, last ? (float*)ptrs[12] : nullptr);
+      else
+        db_kernel<__bf16><<<ceil_div(h.V, 256), 256, 0, s>>>(d.part, (int)dg.y, p.ld, (int)h.V, acc, first, last ? (__bf16*)ptrs[12] : nullptr);
+      YTK_LAUNCH_CHECK();
+    }
+    // D as an operand: rows = score rows, K contiguous for dx, K strided for dw
+    const Operand D = {h.f32 ? ws + p.o_d : ws + p.o_e, p.ld * 2, rows * p.ld * 2, (int)rows};
+    if (h.want_dx) {
+      GradArgs g = {};
+      g.a = o.w;
+      g.a.ext = (int)(p.pack_w ? p.kp : h.d);
+      g.b = D;
+      g.ka = h.V, g.kb = p.ld;
+      g.nkt = (int)(p.ld / 64), g.terms = p.terms, g.splits = p.splits_dx;
+      g.M = (int)h.d, g.N = (int)rows;
+      g.out = (char*)ptrs[10] + r0 * h.d * el, g.ldo = h.d;
+      g.acc = (float*)(ws + p.o_split);
+      g.mode = g.splits > 1 ? 1 : 0;
+      const bool big = g.splits == 1 && use_big(g.M, g.N);
+      if (h.f32) {
+        grad_product<kKS, kKC, float>(g, big, s);
+        if (g.splits > 1) split_sum<float>(g.acc, g.splits, rows, h.d, g.out, s);
+      } else {
+        grad_product<kKS, kKC, __bf16>(g, big, s);
+        if (g.splits > 1) split_sum<__bf16>(g.acc, g.splits, rows, h.d, g.out, s);
+      }
+    }
+    if (h.want_dw) {
+      if (h.f32)
+        pack_rows<float>(x + r0 * h.xrs * el, h.xrs, h.xcs, rows, h.d, ws + p.o_xg, p.kp, r.coef, s);
+      else
+        pack_rows<__bf16>(x + r0 * h.xrs * el, h.xrs, h.xcs, rows, h.d, ws + p.o_xg, p.kp, r.coef, s);
+      GradArgs g = {};
+      g.a = {ws + p.o_xg, p.kp * 2, rows * p.kp * 2, (int)p.kp};
+      g.b = D;
+      g.b.ext = (int)p.ld;
+      g.ka = g.kb = rows;
+      g.nkt = ceil_div(rows, 64), g.terms = p.terms, g.splits = p.splits_dw;
+      g.M = (int)h.d, g.N = (int)h.V;
+      g.out = (void*)ptrs[11], g.ldo = h.d;
+      g.acc = (float*)(ws + (p.many ? p.o_dwacc : p.o_split));
+      g.mode = g.splits > 1 ? 1 : !p.many ? 0 : first ? 1 : last ? 3 : 2;
+      const bool big = g.splits == 1 && use_big(g.M, g.N);
+      if (h.f32) {
+        grad_product<kKS, kKS, float>(g, big, s);
+        if (g.splits > 1) split_sum<float>(g.acc, g.splits, h.V, h.d, g.out, s);
+      } else {
+        grad_product<kKS, kKS, __bf16>(g, big, s);
+        if (g.splits > 1) split_sum<__bf16>(g.acc, g.splits, h.V, h.d, g.out, s);
+      }
+    }
+  }
+}
+
+extern "C" long long ytk_head_topk_ws(const long long* lp) { return head_plan(head_in(lp), true).bytes; }
+
+// ptrs: x, w, bias, ws, values, classes, lse
+extern "C" void ytk_head_topk(const uintptr_t* ptrs, const long long* lp, double temp_, uintptr_t stream) {
+  const HeadIn h = head_in(lp);
+  if (h.k > kTopMax || h.k > h.V) throw std::invalid_argument("head_topk: k is at most 256 and at most the number of classes");
+  const HeadPlan p = head_plan(h, true);
+  hipStream_t s = (hipStream_t)stream;
+  const char* x = (const char*)ptrs[0];
+  const void *w = (const void*)ptrs[1], *bias = (const void*)ptrs[2];
+  char* ws = (char*)ptrs[3];
+  const int el = h.f32 ? 4 : 2;
+  const HeadOps o = head_operands(h, p, x, w, ws, s);
+  for (long long r0 = 0; r0 < h.n; r0 += p.piece) {
+    const long long rows = std::min(p.piece, h.n - r0);
+    scores(h, p, o, r0, rows, bias, (float)temp_, ws, kScores, s);
+    RowArgs r = {};
+    r.stats = (const float2*)(ws + p.o_stats);
+    r.groups = (int)p.groups, r.n = (int)rows, r.V = (int)h.V;
+    r.lse = (float*)ptrs[6] + r0;
+    rows_pass(r, s);
+    TopArgs t = {};
+    t.stats = r.stats;
+    t.z = (const float*)(ws + p.o_e);
+    t.ld = p.ld;
+    t.n = (int)rows, t.V = (int)h.V, t.d = (int)h.d, t.groups = (int)p.groups;
+    t.k = (int)h.k, t.kc = (int)std::min(h.k + kSpare, h.V);
+    t.x = x + r0 * h.xrs * el, t.w = w, t.bias = bias;
+    t.xrs = h.xrs, t.xcs = h.xcs, t.wrs = h.wrs, t.wcs = h.wcs;
+    t.inv_t = 1.0 / temp_;
+    t.values = (float*)ptrs[4] + r0 * h.k;
+    t.classes = (long long*)ptrs[5] + r0 * h.k;
+    const size_t lds = std::max<size_t>(std::min<long long>(t.kc, p.groups) * kGroup * 8,
+                                        p.groups > t.kc && p.groups <= kTopKeys ? p.groups * 4 : 0);
+    if (h.f32)
+      topk_kernel<float><<<(int)rows, 256, lds, s>>>(t);
+    else
+      topk_kernel<__bf16><<<(int)rows, 256, lds, s>>>(t);
+    YTK_LAUNCH_CHECK();
+  }
+}

@@ -1,0 +1,250 @@
+// Matrix-product core of the class head (head.hip): C[m][n] = sum_k A[m][k] B[n][k] in bf16 on the
+// matrix cores, fp32 accumulators, gfx950 only.
+//
+// One block computes a kBM x kBN tile in K steps of 64. An operand lies in memory either with K
+// contiguous (kKC: row r holds its K values) or with K strided (kKS: row k holds the values of all m or n);
+// the three products of a softmax head need all of them from the same row-major x, w and D:
+//   scores  z^T[v][i] = sum_d w[v][d] x[i][d]   A = w (KC)  B = x (KC)
+//   dx^T[d][i]        = sum_v w[v][d] D[i][v]   A = w (KS)  B = D (KC)
+//   dw^T[d][v]        = sum_i x[i][d] D[i][v]   A = x (KS)  B = D (KS)
+// M is always the dimension that is contiguous in the result, because a 32x32 accumulator holds four
+// consecutive m per lane.
+//
+// Tiles go from global memory straight into LDS (buffer_load ... lds, 16 B a lane). The buffer descriptor ends at
+// the operand's last byte, so rows past the end (of M, N or K) read as zero and need no branch.
+// The DMA writes LDS linearly, so the bank swizzle is applied to the SOURCE address: a KC row is 128 B = eight
+// 16-B chunks, chunk c of row r sits at c ^ (r & 7); a KS row is cut into 64-B units, unit u of
+// row k sits at u ^ f(k). KC fragments are ds_read_b128; KS fragments are read transposed
+// (ds_read_b64_tr_b16: 16 lanes exchange a 4 x 16 block).
+#pragma once
+#include "common.h"
+
+namespace ytk {
+
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef __bf16 bf16x4 __attribute__((ext_vector_type(4)));
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+typedef int i32x4 __attribute__((ext_vector_type(4)));
+
+enum { kKC = 0, kKS = 1 };
+
+// fp32 operands are three bf16 planes (hi, mid, lo: 24 bits); a product takes the six plane pairs whose
+// weight is above 2^-24. Plane of A and B for term t, small terms first so that they are not lost.
+struct TermTable {
+  unsigned a, b;  // 2 bits per term
+};
+__host__ __device__ constexpr unsigned term_pack(int t0, int t1, int t2, int t3, int t4, int t5) {
+  return t0 | t1 << 2 | t2 << 4 | t3 << 6 | t4 << 8 | t5 << 10;
+}
+constexpr unsigned kTermA = term_pack(2, 0, 1, 1, 0, 0);
+constexpr unsigned kTermB = term_pack(0, 2, 1, 0, 1, 0);
+
+struct Operand {
+  const char* p;    // plane 0
+  long long pitch;  // bytes per memory row
+  long long plane;  // bytes from plane to plane
+  int ext;          // extent of M (or N)
+};
+
+__device__ __forceinline__ void dma16(unsigned voff, i32x4 rsrc, unsigned lds) {
+  asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tbuffer_load_dwordx4 %0, %1, 0 offen lds" ::"v"(voff), "s"(rsrc), "s"(lds)
+               : "memory");
+}
+template <int N>
+__device__ __forceinline__ void wait_vm() {
+  asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory");
+}
+__device__ __forceinline__ void wait_lgkm() { asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory"); }
+
+// one operand's side of the tile: kT = tile extent, kNW waves load it, kFB 32-wide fragments per wave
+template <int kL, int kT, int kNW, int kFB>
+struct Side {
+  static constexpr int kBytes = kT * 128;
+  static constexpr int kLoads = kT / 8 / kNW;  // DMA instructions per wave and stage
+  static_assert(kT % (8 * kNW) == 0, "tile not divisible among the waves");
+  static constexpr int kRow = kT * 2;          // KS: LDS bytes per k row
+  static constexpr int kUnits = kRow / 64;
+  unsigned voff[kLoads];
+  unsigned lds0;                // wave's first LDS byte of a stage
+  unsigned rd[kL == kKC ? 4 : kFB];
+  const char* base;
+  long long rem;                // bytes to the operand's end
+  long long step, plane;
+
+  static __device__ __forceinline__ int swz(int row) { return ((row & 3) | (((row >> 3) & 1) << 2)) & (kUnits - 1); }
+
+  __device__ __forceinline__ void init(const Operand& o, int t0, long long K, int kt0, int wave, int frag0, unsigned lds) {
+    const int l = threadIdx.x & 63;
+    if (kL == kKC) {
+#pragma unroll
+      for (int i = 0; i < kLoads; ++i) {
+        const int row = (i * kNW + wave) * 8 + (l >> 3);
+        voff[i] = (unsigned)(row * o.pitch) + (((l & 7) ^ (row & 7)) << 4);
+      }
+      base = o.p + (long long)t0 * o.pitch + kt0 * 128LL;
+      rem = (long long)(o.ext - t0 - 1) * o.pitch + (K - kt0 * 64LL) * 2;
+      step = 128;
+#pragma unroll
+      for (int s = 0; s < 4; ++s) {
+        const int row = frag0 * 32 + (l & 31);
+        rd[s] = lds + row * 128 + (((s * 2 + (l >> 5)) ^ (row & 7)) << 4);
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < kLoads; ++i) {
+        const int byte = (i * kNW + wave) * 1024 + l * 16;
+        const int row = byte / kRow, chunk = (byte % kRow) / 16;
+        voff[i] = (unsigned)(row * o.pitch) + ((((chunk >> 2) ^ swz(row)) << 2 | (chunk & 3)) << 4);
+      }
+      base = o.p + kt0 * 64LL * o.pitch + t0 * 2LL;
+      rem = (K - kt0 * 64LL - 1) * o.pitch + (long long)(o.ext - t0) * 2;
+      step = 64 * o.pitch;
+      const int g = l >> 4, i16 = l & 15, row = (g >> 1) * 8 + (i16 >> 2);
+#pragma unroll
+      for (int b = 0; b < kFB; ++b)
+        rd[b] = lds + row * kRow + (((frag0 + b) ^ swz(row)) << 6) + (g & 1) * 32 + (i16 & 3) * 8;
+    }
+    plane = o.plane;
+    lds0 = lds + wave * 1024;
+  }
+
+  // stage of K step `kt` (relative to kt0), plane `pl`, into LDS stage offset `so`
+  __device__ __forceinline__ void issue(int kt, int pl, unsigned so) const {
+    const unsigned long long a = (unsigned long long)(base + kt * step + pl * plane);
+    long long r = rem - kt * step;
+    r = r < 0 ? 0 : r > 0x7fffffffLL ? 0x7fffffffLL : r;
+    i32x4 d;
+    d[0] = (int)(unsigned)a;
+    d[1] = (int)((a >> 32) & 0xffff);
+    d[2] = (int)r;
+    d[3] = 0x00020000;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) d[i] = __builtin_amdgcn_readfirstlane(d[i]);
+#pragma unroll
+    for (int i = 0; i < kLoads; ++i) dma16(voff[i], d, __builtin_amdgcn_readfirstlane(lds0 + so + i * kNW * 1024));
+  }
+
+  __device__ __forceinline__ bf16x8 frag(int b, int s, unsigned so) const {
+    typedef __attribute__((address_space(3))) char lc;
+    typedef __attribute__((address_space(3))) bf16x8 l8;
+    typedef __attribute__((address_space(3))) bf16x4 l4;
+    // constant parts as pointer arithmetic: they become the instruction's offset
+    if (kL == kKC) return *(const l8*)((const lc*)(uintptr_t)(rd[s] + so) + b * 4096);
+    const lc* q = (const lc*)(uintptr_t)(rd[b] + so) + s * 16 * kRow;
+    const bf16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4bf16((l4*)q);
+    const bf16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4bf16((l4*)(q + 4 * kRow));
+    return __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+  }
+};
+
+template <int BM, int BN, int WM, int WN, int S>
+struct TileCfg {
+  static constexpr int kBM = BM, kBN = BN, kWM = WM, kWN = WN, kStages = S;
+  static constexpr int kNW = WM * WN, kThreads = 64 * kNW;
+  static constexpr int kFM = BM / WM / 32, kFN = BN / WN / 32;  // 32x32 blocks per wave
+  static constexpr unsigned kStageBytes = (BM + BN) * 128;
+  static constexpr unsigned kLds = S * kStageBytes;
+};
+
+// (ka, kb: extent of K in each operand's memory; a KC operand's is a multiple of 64)
+// acc += A[m0.., kt0*64 ..] B[n0.., ...]^T over `nkt` K steps and `terms` plane pairs (1 or 6)
+template <class C, int kLA, int kLB>
+__device__ __forceinline__ void gemm_loop(const Operand& A, const Operand& B, int m0, int n0, long long ka, long long kb,
+                                          int kt0, int nkt, int terms, f32x16 (&acc)[C::kFM][C::kFN]) {
+  extern __shared__ __align__(1024) char head_smem[];
+  typedef __attribute__((address_space(3))) char lc;
+  const unsigned lds = (unsigned)(uintptr_t)(lc*)head_smem;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int wm = wave / C::kWN, wn = wave % C::kWN;
+  Side<kLA, C::kBM, C::kNW, C::kFM> a;
+  Side<kLB, C::kBN, C::kNW, C::kFN> b;
+  a.init(A, m0, ka, kt0, wave, wm * C::kFM, lds);
+  b.init(B, n0, kb, kt0, wave, wn * C::kFN, lds + C::kBM * 128);
+  constexpr int kLoads = Side<kLA, C::kBM, C::kNW, C::kFM>::kLoads + Side<kLB, C::kBN, C::kNW, C::kFN>::kLoads;
+  const int iters = nkt * terms;
+  int ikt = 0, iterm = 0;  // next stage to issue
+  const unsigned ta = terms == 1 ? 0u : kTermA, tb = terms == 1 ? 0u : kTermB;
+  auto issue = [&](unsigned so) {
+    a.issue(ikt, (ta >> (2 * iterm)) & 3, so);
+    b.issue(ikt, (tb >> (2 * iterm)) & 3, so);
+    if (++iterm == terms) {
+      iterm = 0;
+      ++ikt;
+    }
+  };
+#pragma unroll
+  for (int s = 0; s < C::kStages; ++s)
+    if (s < iters) issue(s * C::kStageBytes);
+  if (iters > C::kStages - 1)
+    wait_vm<(C::kStages - 1) * kLoads>();
+  else
+    wait_vm<0>();
+  __builtin_amdgcn_s_barrier();
+
+  bf16x8 fa[2][C::kFM], fb[2][C::kFN];
+  auto read = [&](int p, int s, unsigned so) {
+#pragma unroll
+    for (int i = 0; i < C::kFM; ++i) fa[p][i] = a.frag(i, s, so);
+#pragma unroll
+    for (int j = 0; j < C::kFN; ++j) fb[p][j] = b.frag(j, s, so);
+  };
+  auto mma = [&](int p) {
+#pragma unroll
+    for (int i = 0; i < C::kFM; ++i)
+#pragma unroll
+      for (int j = 0; j < C::kFN; ++j)
+        acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(fa[p][i], fb[p][j], acc[i][j], 0, 0, 0);
+  };
+  // one quarter: the next quarter's fragments are read between this quarter's products
+  constexpr int kReads = C::kFM * (kLA == kKC ? 1 : 2) + C::kFN * (kLB == kKC ? 1 : 2), kMma = C::kFM * C::kFN;
+  auto weave = [&]() {
+    constexpr int per = (kReads + kMma - 1) / kMma;
+#pragma unroll
+    for (int i = 0; i < kMma; ++i) {
+      __builtin_amdgcn_sched_group_barrier(0x100, per, 0);  // LDS reads
+      __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);    // matrix product
+    }
+    __builtin_amdgcn_sched_barrier(0);
+  };
+  unsigned so = 0;
+  read(0, 0, 0);
+  for (int it = 0; it < iters; ++it) {
+    read(1, 1, so);
+    mma(0);
+    weave();
+    read(0, 2, so);
+    mma(1);
+    weave();
+    read(1, 3, so);
+    mma(0);
+    weave();
+    // every read of this stage has returned, and the next stage has landed: one barrier hands this
+    // buffer back to the DMA while the last quarter's products still run
+    wait_lgkm();
+    if (it + C::kStages <= iters)
+      wait_vm<(C::kStages - 2) * kLoads>();
+    else
+      wait_vm<0>();
+    __builtin_amdgcn_s_barrier();
+    if (it + C::kStages < iters) issue(so);
+    so = so + C::kStageBytes == C::kLds ? 0u : so + C::kStageBytes;
+    // (after the last step this reads a stage that holds old data; nothing uses it)
+    read(0, 0, so);
+    mma(1);
+    weave();
+  }
+}
+
+// block -> tile: each XCD (blocks go to them round robin) works through a contiguous run of the tile
+// order, and the order walks 8 m tiles before the next n tile, so the 32 CUs behind one L2 share their panels.
+__device__ __forceinline__ bool tile_of(int nm, int nn, int& tm, int& tn) {
+  const int T = nm * nn, chunk = (T + 7) / 8;
+  const int id = (int)(blockIdx.x & 7) * chunk + (int)(blockIdx.x >> 3);
+  if ((int)(blockIdx.x >> 3) >= chunk || id >= T) return false;
+  const int gsz = 8 * nn, g = id / gsz, r = id % gsz, gm = nm - g * 8 < 8 ? nm - g * 8 : 8;
+  tm = g * 8 + r % gm;
+  tn = r / gm;
+  return true;
+}
+
+}  // namespace ytk
