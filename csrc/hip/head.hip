@@ -102,8 +102,7 @@ __global__ __launch_bounds__(256) void pack_kernel(const T* __restrict__ src, lo
 // ------------------------------------------------------------------ scores
 struct ScoreArgs {
   Operand w, x;
-  long long K;        // padded d
-  int nkt, terms;
+  int K, terms;       // padded d; plane pairs
   int V, n;
   int nm, nn;         // tiles
   const void* bias;   // element type of the inputs
@@ -152,7 +151,7 @@ __global__ __launch_bounds__(C::kThreads) void scores_kernel(ScoreArgs p) {
   int tm, tn;
   if (!tile_of(p.nm, p.nn, tm, tn)) return;
   f32x16 acc[C::kFM][C::kFN] = {};
-  gemm_loop<C, kKC, kKC>(p.w, p.x, tm * C::kBM, tn * C::kBN, p.K, p.K, 0, p.nkt, p.terms, acc);
+  gemm_loop<C, kKC, kKC>(p.w, p.x, tm * C::kBM, tn * C::kBN, p.K, p.K, 0, p.K / C::kBK, p.terms, acc);
   static_assert(C::kFM % 2 == 0, "a wave holds whole groups");
   const int wave = threadIdx.x >> 6, l = threadIdx.x & 63, hi = l >> 5;
   const int v0 = tm * C::kBM + (wave / C::kWN) * C::kFM * 32, i0 = tn * C::kBN + (wave % C::kWN) * C::kFN * 32;
@@ -229,13 +228,12 @@ __global__ __launch_bounds__(C::kThreads) void scores_kernel(ScoreArgs p) {
 }
 
 // ------------------------------------------------------------------ targets
-// z of each row's target classes by plain fp32 dot products: one wave per row, x's row in registers is not
-// needed again often enough to hold, so both operands stream through L1.
+// z of each row's target classes by plain fp32 dot products.
 struct TargetArgs {
   const void *x, *w, *bias;
   long long xrs, xcs, wrs, wcs;
   const void* idx;     // [n][k], int64 or int32
-  int idx64, k, n, d, V, f32;
+  int idx64, k, n, d, V, vec;
   float inv_t;
   float* zt;           // [n][k]
 };
@@ -244,26 +242,80 @@ __device__ __forceinline__ long long index_at(const void* p, int is64, long long
   return is64 ? ((const long long*)p)[i] : (long long)((const int*)p)[i];
 }
 
-template <typename T>
-__global__ __launch_bounds__(256) void target_kernel(TargetArgs p) {
-  const long long item = (long long)blockIdx.x * 4 + (threadIdx.x >> 6);
-  if (item >= (long long)p.n * p.k) return;
+// 16 bytes of a row as fp32
+__device__ __forceinline__ void load16(const float* p, float (&v)[4]) {
+  const float4 a = *(const float4*)p;
+  v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w;
+}
+__device__ __forceinline__ void load16(const __bf16* p, float (&v)[8]) {
+  const bf16x8 a = *(const bf16x8*)p;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) v[i] = (float)a[i];
+}
+
+// a wave's dot products of one x row with kW w rows, summed in A (fp32, or fp64 of exact or fp64 products).
+// `vec`: rows of whole, aligned 16-byte pieces; otherwise element by element with any stride.
+template <typename T, typename A, int kW>
+__device__ __forceinline__ void row_dots(const T* x, long long xcs, const T* const (&w)[kW], long long wcs, int d, bool vec, A (&s)[kW]) {
   const int l = threadIdx.x & 63;
-  const long long row = item / p.k, v = index_at(p.idx, p.idx64, item);
-  float s = 0.0f;
-  if (v >= 0 && v < p.V) {
-    const T *x = (const T*)p.x + row * p.xrs, *w = (const T*)p.w + v * p.wrs;
-    float s2 = 0.0f;
-    int c = l;
-    for (; c + 64 < p.d; c += 128) {
-      s = fmaf(Elem<T>::get(x, c * p.xcs), Elem<T>::get(w, c * p.wcs), s);
-      s2 = fmaf(Elem<T>::get(x, (c + 64) * p.xcs), Elem<T>::get(w, (c + 64) * p.wcs), s2);
+#pragma unroll
+  for (int i = 0; i < kW; ++i) s[i] = 0;
+  constexpr int kE = 16 / sizeof(T);
+  auto add = [](A& s, float a, float b) {
+    if (sizeof(A) == 8 && sizeof(T) == 2)
+      s += (A)(a * b);  // exact: 8 x 8 bits
+    else
+      s = fma((A)a, (A)b, s);
+  };
+  if (vec) {
+#pragma unroll 2
+    for (int c = l * kE; c < d; c += 64 * kE) {
+      float a[kE], b[kW][kE];
+      load16(x + c, a);
+#pragma unroll
+      for (int i = 0; i < kW; ++i) load16(w[i] + c, b[i]);
+#pragma unroll
+      for (int i = 0; i < kW; ++i)
+#pragma unroll
+        for (int e = 0; e < kE; ++e) add(s[i], a[e], b[i][e]);
     }
-    if (c < p.d) s = fmaf(Elem<T>::get(x, c * p.xcs), Elem<T>::get(w, c * p.wcs), s);
-    s = wave_sumf(s + s2);
-    if (p.bias) s += Elem<T>::get((const T*)p.bias, v);
+  } else {  // in the same order, so that the result does not depend on the strides
+    for (int c = l * kE; c < d; c += 64 * kE)
+      for (int e = 0; e < min(kE, d - c); ++e) {
+        const float a = Elem<T>::get(x, (c + e) * xcs);
+#pragma unroll
+        for (int i = 0; i < kW; ++i) add(s[i], a, Elem<T>::get(w[i], (c + e) * wcs));
+      }
   }
-  if (l == 0) p.zt[item] = s * p.inv_t;
+#pragma unroll
+  for (int i = 0; i < kW; ++i)
+#pragma unroll
+    for (int o = 32; o; o >>= 1) s[i] += __shfl_xor(s[i], o, 64);
+}
+
+// kW targets of one row per wave: their loads are in flight together
+template <typename T, int kW>
+__global__ __launch_bounds__(256) void target_kernel(TargetArgs p) {
+  const int l = threadIdx.x & 63, runs = (p.k + kW - 1) / kW;
+  const long long item = (long long)blockIdx.x * 4 + (threadIdx.x >> 6);
+  if (item >= (long long)p.n * runs) return;
+  const long long row = item / runs, first = row * p.k + item % runs * kW;
+  const int m = min(kW, (int)((row + 1) * p.k - first));
+  const T* w[kW];
+  long long v[kW];
+#pragma unroll
+  for (int i = 0; i < kW; ++i) {
+    v[i] = i < m ? index_at(p.idx, p.idx64, first + i) : -1;
+    if (v[i] >= p.V) v[i] = -1;
+    w[i] = (const T*)p.w + (v[i] < 0 ? 0 : v[i]) * p.wrs;  // entries without a class read class 0
+  }
+  float s[kW];
+  row_dots<T, float, kW>((const T*)p.x + row * p.xrs, p.xcs, w, p.wcs, p.d, p.vec, s);
+  if (l == 0) {
+#pragma unroll
+    for (int i = 0; i < kW; ++i)
+      if (i < m) p.zt[first + i] = v[i] < 0 ? 0.0f : (s[i] + (p.bias ? Elem<T>::get((const T*)p.bias, v[i]) : 0.0f)) * p.inv_t;
+  }
 }
 
 // ------------------------------------------------------------------ rows
@@ -393,72 +445,86 @@ constexpr int kDCols = 512;   // columns per block: one wave = one row's 512 col
 
 template <bool kF32>
 __global__ __launch_bounds__(256) void dscore_kernel(DArgs p) {
+  typedef _Float16 h8 __attribute__((ext_vector_type(8)));
+  constexpr int kB = kF32 ? 2 : 4;  // rows at once: their loads are in flight together
   const int wave = threadIdx.x >> 6, l = threadIdx.x & 63;
-  const int c = blockIdx.x * kDCols + l * 8;
-  const long long r0 = (long long)blockIdx.y * kDRows;
-  const int r1 = (int)min((long long)kDRows, p.n - r0);
+  const int c0 = blockIdx.x * kDCols, c = c0 + l * 8;
+  const long long r0 = (long long)blockIdx.y * kDRows + wave * (kDRows / 4);
+  const int rows = (int)min((long long)(kDRows / 4), p.n - r0);  // may be negative
   float db[8] = {};
   const bool live = c < p.ld;
-  for (int r = wave; r < r1; r += 4) {
-    const long long i = r0 + r;
-    const float2 nr = p.norm[i];
-    const float c0w = p.coef[i], co = c0w * nr.y;
-    float d[8];
+  const long long cl = live ? c : 0;  // lanes past the end read column 0 and write nothing
+  const float2* st = p.stats + cl / kGroup * p.n;
+  for (int rb = 0; rb < rows; rb += kB) {
+    float d[kB][8], m[kB], cw[kB];
+    float2 nr[kB];
+    long long v[kB];
 #pragma unroll
-    for (int j = 0; j < 8; ++j) d[j] = 0.0f;
-    if (c0w != 0.0f) {
-      if (live) {
-        const float m = p.stats[(long long)(c / kGroup) * p.n + i].x;
-        // E is e^(z - m) with m = 0 for a group that has only -inf
-        const float f = co * exp_of<kF32>((m == -INFINITY ? 0.0f : m) - nr.x);
-        if (kF32) {
-          const float4 *e = (const float4*)((const float*)p.e + i * p.ld + c), a = e[0], b = e[1];
-          d[0] = a.x * f, d[1] = a.y * f, d[2] = a.z * f, d[3] = a.w * f;
-          d[4] = b.x * f, d[5] = b.y * f, d[6] = b.z * f, d[7] = b.w * f;
-        } else {
-          typedef _Float16 h8 __attribute__((ext_vector_type(8)));
-          const h8 a = *(const h8*)((const _Float16*)p.e + i * p.ld + c);
-          const float k = f * (1.0f / 32768.0f);
-#pragma unroll
-          for (int j = 0; j < 8; ++j) d[j] = (float)a[j] * k;
-        }
-      }
-      // target classes: p is taken from the fp32 score, and every entry of the list on that class is subtracted
-      // (first all probabilities, then all targets: a class named twice is counted twice)
-      const int c0 = blockIdx.x * kDCols;
-#pragma unroll
-      for (int pass = 0; pass < 2; ++pass)
-        for (int j0 = 0; j0 < p.k; j0 += 64) {
-          const long long v = j0 + l < p.k ? index_at(p.idx, p.idx64, i * p.k + j0 + l) : -1;
-          const int at = v >= c0 && v < c0 + kDCols && v < p.V ? (int)(v - c0) : -1;
-          for (unsigned long long h = __ballot(at >= 0); h; h &= h - 1) {
-            const int b = __builtin_ctzll(h), vb = __builtin_amdgcn_readlane(at, b);
-            const long long e = i * p.k + j0 + b;
-            const float x = pass == 0 ? co * exp_of<kF32>(p.zt[e] - nr.x) : p.q[e];
-#pragma unroll
-            for (int u = 0; u < 8; ++u)
-              if (vb == l * 8 + u) d[u] = pass == 0 ? x : d[u] - x;
-          }
-        }
-    }
-    if (live) {
-#pragma unroll
-      for (int j = 0; j < 8; ++j) db[j] += d[j];
+    for (int b = 0; b < kB; ++b) {
+      const long long i = min(r0 + rb + b, (long long)p.n - 1);
+      cw[b] = rb + b < rows ? p.coef[i] : 0.0f;
+      nr[b] = p.norm[i];
+      m[b] = st[i].x;
+      v[b] = l < p.k ? index_at(p.idx, p.idx64, i * p.k + l) : -1;
       if (kF32) {
-        bf16x8 h, m, lo;
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          __bf16 a, b, e;
-          split3(d[j], a, b, e);
-          h[j] = a, m[j] = b, lo[j] = e;
-        }
-        __bf16* o = p.d + i * p.ld + c;
-        *(bf16x8*)o = h;
-        *(bf16x8*)(o + p.plane) = m;
-        *(bf16x8*)(o + 2 * p.plane) = lo;
+        const float4 *e = (const float4*)((const float*)p.e + i * p.ld + cl), x = e[0], y = e[1];
+        d[b][0] = x.x, d[b][1] = x.y, d[b][2] = x.z, d[b][3] = x.w;
+        d[b][4] = y.x, d[b][5] = y.y, d[b][6] = y.z, d[b][7] = y.w;
       } else {
-        *(uint4*)((unsigned short*)p.e + i * p.ld + c) =
-            make_uint4(pack_b2(d[0], d[1]), pack_b2(d[2], d[3]), pack_b2(d[4], d[5]), pack_b2(d[6], d[7]));
+        const h8 x = *(const h8*)((const _Float16*)p.e + i * p.ld + cl);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) d[b][j] = (float)x[j];
+      }
+    }
+#pragma unroll
+    for (int b = 0; b < kB; ++b) {
+      if (rb + b >= rows) break;
+      const long long i = r0 + rb + b;
+      const float co = cw[b] * nr[b].y;
+      if (cw[b] != 0.0f) {
+        // E is e^(z - m) with m = 0 for a group that has only -inf
+        const float f = co * exp_of<kF32>((m[b] == -INFINITY ? 0.0f : m[b]) - nr[b].x) * (kF32 ? 1.0f : 1.0f / 32768.0f);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) d[b][j] *= f;
+        // target classes: p is taken from the fp32 score, and every entry of the list on that class is subtracted
+        // (first all probabilities, then all targets: a class named twice is counted twice)
+#pragma unroll
+        for (int pass = 0; pass < 2; ++pass)
+          for (int j0 = 0; j0 < p.k; j0 += 64) {
+            const long long vv = j0 == 0 ? v[b] : j0 + l < p.k ? index_at(p.idx, p.idx64, i * p.k + j0 + l) : -1;
+            const int at = vv >= c0 && vv < c0 + kDCols && vv < p.V ? (int)(vv - c0) : -1;
+            for (unsigned long long h = __ballot(at >= 0); h; h &= h - 1) {
+              const int bit = __builtin_ctzll(h), vb = __builtin_amdgcn_readlane(at, bit);
+              const long long e = i * p.k + j0 + bit;
+              const float x = pass == 0 ? co * exp_of<kF32>(p.zt[e] - nr[b].x) : p.q[e];
+#pragma unroll
+              for (int u = 0; u < 8; ++u)
+                if (vb == l * 8 + u) d[b][u] = pass == 0 ? x : d[b][u] - x;
+            }
+          }
+      } else {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) d[b][j] = 0.0f;
+      }
+      if (live) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) db[j] += d[b][j];
+        if (kF32) {
+          bf16x8 h, mi, lo;
+#pragma unroll
+          for (int j = 0; j < 8; ++j) {
+            __bf16 x, y, z;
+            split3(d[b][j], x, y, z);
+            h[j] = x, mi[j] = y, lo[j] = z;
+          }
+          __bf16* o = p.d + i * p.ld + c;
+          *(bf16x8*)o = h;
+          *(bf16x8*)(o + p.plane) = mi;
+          *(bf16x8*)(o + 2 * p.plane) = lo;
+        } else {
+          *(uint4*)((unsigned short*)p.e + i * p.ld + c) =
+              make_uint4(pack_b2(d[b][0], d[b][1]), pack_b2(d[b][2], d[b][3]), pack_b2(d[b][4], d[b][5]), pack_b2(d[b][6], d[b][7]));
+        }
       }
     }
   }
@@ -491,7 +557,7 @@ __global__ __launch_bounds__(256) void db_kernel(const float* __restrict__ part,
 struct GradArgs {
   Operand a, b;
   long long ka, kb;        // extent of K in each operand's memory
-  int nkt, terms, splits;  // K steps in all, cut into `splits` runs
+  int K, terms, splits;    // products run over K (at most ka, kb), cut into `splits` runs of whole 64s
   int M, N, nm, nn;        // result [N][M], M contiguous
   void* out;               // T [N][ldo]
   long long ldo;
@@ -505,7 +571,8 @@ __global__ __launch_bounds__(C::kThreads) void grad_kernel(GradArgs p) {
   if (!tile_of(p.nm, p.nn * p.splits, tm, tn)) return;
   const int split = tn / p.nn;
   tn -= split * p.nn;
-  const int per = (p.nkt + p.splits - 1) / p.splits, kt0 = split * per, nkt = min(per, p.nkt - kt0);
+  const int per = (p.K + 64 * p.splits - 1) / (64 * p.splits) * 64, k0 = split * per, k1 = min(k0 + per, p.K);
+  const int kt0 = k0 / C::kBK, nkt = (k1 - k0 + C::kBK - 1) / C::kBK;
   f32x16 acc[C::kFM][C::kFN] = {};
   if (nkt > 0) gemm_loop<C, kLA, kLB>(p.a, p.b, tm * C::kBM, tn * C::kBN, p.ka, p.kb, kt0, nkt, p.terms, acc);
   const int wave = threadIdx.x >> 6, l = threadIdx.x & 63, hi = l >> 5;
@@ -582,7 +649,7 @@ struct TopArgs {
   const float2* stats;
   const float* z;
   long long ld;
-  int n, V, d, groups, kc, k;
+  int n, V, d, groups, kc, k, vec;
   const void *x, *w, *bias;
   long long xrs, xcs, wrs, wcs;
   double inv_t;
@@ -645,22 +712,22 @@ __device__ K radix_kth(int count, int k, F key, int* hist, int* pick, int& above
 }
 
 template <typename T>
-__global__ __launch_bounds__(256) void topk_kernel(TopArgs p) {
+__global__ __launch_bounds__(1024) void topk_kernel(TopArgs p) {
   extern __shared__ __align__(16) char head_smem[];
-  __shared__ int hist[256], pick[2], cnt, wcnt[4];
+  __shared__ int hist[256], pick[2], cnt, wcnt[16];
   __shared__ int sel[kTopMax + kSpare];
   __shared__ double zs[kTopMax + kSpare];
   __shared__ int cls[kTopMax + kSpare];
   unsigned long long* keys = (unsigned long long*)head_smem;  // kc * kGroup
   unsigned* gk = (unsigned*)head_smem;                        // groups; done with before the keys are written
-  const int row = blockIdx.x, t = threadIdx.x, wave = t >> 6, l = t & 63;
+  const int row = blockIdx.x, t = threadIdx.x, nt = blockDim.x, wave = t >> 6, waves = nt >> 6, l = t & 63;
   const bool held = p.groups <= kTopKeys;
   const float2* st = p.stats + row;
   int nsel = p.groups;
   unsigned tau = 0;
   if (p.groups > p.kc) {
     if (held)
-      for (int g = t; g < p.groups; g += 256) gk[g] = order_key(st[(long long)g * p.n].x);
+      for (int g = t; g < p.groups; g += nt) gk[g] = order_key(st[(long long)g * p.n].x);
     __syncthreads();
     auto gkey = [&](int g) { return held ? gk[g] : order_key(st[(long long)g * p.n].x); };
     int above;
@@ -669,14 +736,14 @@ __global__ __launch_bounds__(256) void topk_kernel(TopArgs p) {
     if (t == 0) cnt = 0;
     __syncthreads();
     int seen = 0;
-    for (int g0 = 0; g0 < p.groups; g0 += 256) {
+    for (int g0 = 0; g0 < p.groups; g0 += nt) {
       const unsigned key = g0 + t < p.groups ? gkey(g0 + t) : 0u;
       const bool in = g0 + t < p.groups, eq = in && key == tau;
       const unsigned long long m = __ballot(eq);
       if (l == 0) wcnt[wave] = __popcll(m);
       __syncthreads();
       int rank = seen + __popcll(m & ((1ull << l) - 1));
-      for (int w = 0; w < 4; ++w) {
+      for (int w = 0; w < waves; ++w) {
         if (w < wave) rank += wcnt[w];
         seen += wcnt[w];
       }
@@ -688,7 +755,7 @@ __global__ __launch_bounds__(256) void topk_kernel(TopArgs p) {
   if (t == 0) cnt = 0;
   __syncthreads();
   const float* z = p.z + (long long)row * p.ld;
-  for (int s = wave; s < nsel; s += 4) {
+  for (int s = wave; s < nsel; s += waves) {
     const int v = (p.groups > p.kc ? sel[s] : s) * kGroup + l;
     const unsigned o = v < p.V ? order_key(z[v]) : 0u;
     const bool take = v < p.V && o >= tau;
@@ -707,20 +774,23 @@ __global__ __launch_bounds__(256) void topk_kernel(TopArgs p) {
   }
   if (t == 0) cnt = 0;
   __syncthreads();
-  for (int i = t; i < total; i += 256)
+  for (int i = t; i < total; i += nt)
     if (keys[i] >= least) cls[atomicAdd(&cnt, 1)] = (int)~(unsigned)keys[i];
   __syncthreads();
-  // exact scores of the kc candidates, a wave each
+  // exact scores of the kc candidates, two at a time per wave
   const T *x = (const T*)p.x + row * p.xrs, *bias = (const T*)p.bias;
-  for (int c = wave; c < p.kc; c += 4) {
-    const T* w = (const T*)p.w + (long long)cls[c] * p.wrs;
-    double s = 0.0;
-    for (int j = l; j < p.d; j += 64) s = fma((double)Elem<T>::get(x, j * p.xcs), (double)Elem<T>::get(w, j * p.wcs), s);
-    s = wave_sum(s);
-    if (l == 0) zs[c] = (s + (bias ? (double)Elem<T>::get(bias, cls[c]) : 0.0)) * p.inv_t;
+  for (int c = wave * 2; c < p.kc; c += waves * 2) {
+    const int o = c + 1 < p.kc ? c + 1 : c;
+    const T* w[2] = {(const T*)p.w + (long long)cls[c] * p.wrs, (const T*)p.w + (long long)cls[o] * p.wrs};
+    double s[2];
+    row_dots<T, double, 2>(x, p.xcs, w, p.wcs, p.d, p.vec, s);
+    if (l == 0) {
+      zs[c] = (s[0] + (bias ? (double)Elem<T>::get(bias, cls[c]) : 0.0)) * p.inv_t;
+      if (o != c) zs[o] = (s[1] + (bias ? (double)Elem<T>::get(bias, cls[o]) : 0.0)) * p.inv_t;
+    }
   }
   __syncthreads();
-  for (int c = t; c < p.kc; c += 256) {
+  for (int c = t; c < p.kc; c += nt) {
     const unsigned long long mine = order_key(zs[c]);
     const int v = cls[c];
     int rank = 0;
@@ -736,11 +806,44 @@ __global__ __launch_bounds__(256) void topk_kernel(TopArgs p) {
 }
 
 // ------------------------------------------------------------------ host side
+static long long up(long long v, long long m) { return (v + m - 1) / m * m; }
+
 inline int grid8(long long tiles) { return (int)((tiles + 7) / 8 * 8); }
 
-typedef TileCfg<256, 256, 2, 4, 2> CfgBig;
-typedef TileCfg<128, 128, 2, 2, 2> CfgMid;
-typedef TileCfg<128, 32, 2, 1, 4> CfgSlim;
+// Tiles, with the rate of a long product (32768 x 8192 x 4096 and its two transposes, random data):
+typedef TileCfg<256, 256, 2, 4, 32, 5> CfgBig;   // 1.39 PFLOP/s; all 160 KB of LDS, one block per CU
+typedef TileCfg<128, 256, 2, 4, 64, 3> CfgWide;  // 1.25 - 1.35
+typedef TileCfg<128, 128, 2, 2, 32, 4> CfgMid;   // 0.85 - 1.05 (bound by L2 reads), two blocks per CU
+typedef TileCfg<128, 32, 2, 1, 64, 4> CfgSlim;   // few rows: bound by reading w
+
+enum { kBig = 0, kWide = 1, kMid = 2 };
+
+// Estimated time of an M x N x K product in units of one CU's multiply-adds: rounds of blocks over the 256 CUs,
+// each paying its tile's products at the tile's rate, and about 4 us (10^7 multiply-adds) to start and finish;
+// K cut into `splits` runs costs the partial sums' traffic.
+static double tile_cost(int cfg, long long m, long long n, long long k, int terms, int splits) {
+  const int bm = cfg == kBig ? 256 : 128, bn = cfg == kMid ? 128 : 256, per_cu = cfg == kMid ? 2 : 1;
+  const double rate = cfg == kBig ? 1.0 : cfg == kWide ? 0.92 : 0.7;
+  const long long blocks = (long long)ceil_div(m, bm) * ceil_div(n, bn) * splits;
+  const long long rounds = (blocks + 256 * per_cu - 1) / (256 * per_cu);
+  const double one = (double)bm * bn * (double)up((k + splits - 1) / splits, 64) * terms / rate * std::min<long long>(per_cu, (blocks + 255) / 256);
+  return rounds * (one + 1e7) + (splits > 1 ? 5e6 + (double)m * n * splits * 5.0 : 0.0);
+}
+
+static int pick_tile(long long m, long long n, long long k, int terms, int max_splits, int* splits) {
+  int best = kBig;
+  double cost = 1e300;
+  for (int c = kBig; c <= kMid; ++c)
+    for (int s = 1; s <= max_splits && (s == 1 || k / s >= 512 / terms); s = s < 4 ? s + 1 : s + s / 4) {
+      const double t = tile_cost(c, m, n, k, terms, s);
+      if (t < cost) {
+        cost = t;
+        best = c;
+        if (splits) *splits = s;
+      }
+    }
+  return best;
+}
 
 template <class C>
 void scores_launch(ScoreArgs p, int mode, hipStream_t s) {
@@ -783,8 +886,9 @@ static HeadIn head_in(const long long* lp) {
   static_assert(sizeof(HeadIn) == kHeadIn * sizeof(long long), "");
   memcpy(&h, lp, sizeof(h));
   if (h.n < 1 || h.d < 1 || h.V < 1 || h.k < 1) throw std::invalid_argument("class head: empty problem");
-  if (h.V > (1LL << 22) - 64 || h.d > (1LL << 22) - 64 || h.n > (1LL << 31) - 65536)
-    throw std::invalid_argument("class head: more than 4M classes or features, or 2G rows");
+  // 256 rows of an operand span less than 2^31 bytes (head_gemm.h)
+  if (h.V > (1LL << 21) || h.d > (1LL << 21) || h.n > (1LL << 31) - 65536)
+    throw std::invalid_argument("class head: more than 2M classes or features, or 2G rows");
   return h;
 }
 
@@ -792,25 +896,10 @@ struct HeadPlan {
   int planes, terms;
   long long kp, ld, groups, piece;
   bool pack_x, pack_w, grads;
-  int splits_dx, splits_dw;
+  int splits_dx, splits_dw, tile_dx, tile_dw;
   bool many;  // more than one piece of rows
   long long o_x, o_w, o_xg, o_e, o_d, o_stats, o_zt, o_q, o_coef, o_norm, o_part, o_dbacc, o_dwacc, o_split, bytes;
 };
-
-static long long up(long long v, long long m) { return (v + m - 1) / m * m; }
-
-// Big tiles when they fill the card's 256 CUs, otherwise a quarter of the size
-static bool use_big(long long m, long long n) {
-  return (long long)ceil_div(m, CfgBig::kBM) * ceil_div(n, CfgBig::kBN) >= 256;
-}
-
-// runs of the K dimension so that a product with few tiles still fills the card (about two blocks per CU); each
-// run keeps at least 8 K steps
-static int split_of(long long m, long long n, long long nkt) {
-  if (use_big(m, n)) return 1;
-  const long long tiles = (long long)ceil_div(m, CfgMid::kBM) * ceil_div(n, CfgMid::kBN);
-  return (int)std::max(1LL, std::min(std::min(512 / std::max(tiles, 1LL), nkt / 8), 64LL));
-}
 
 static HeadPlan head_plan(const HeadIn& h, bool topk) {
   HeadPlan p = {};
@@ -823,10 +912,14 @@ static HeadPlan head_plan(const HeadIn& h, bool topk) {
   p.pack_x = h.f32 || !h.x_al;
   p.pack_w = h.f32 || !h.w_al;
   const long long per = topk ? p.ld * 4 : p.grads ? p.ld * (h.f32 ? 10 : 2) : p.groups * 8;
-  p.piece = std::min(h.n, std::max(256LL, h.piece_bytes / per / 256 * 256));
+  // (at most 2M rows: the grids of the row passes count rows / 64 in 16 bits and rows * k in 31)
+  p.piece = std::min(h.n, std::min(1LL << 21, std::max(256LL, h.piece_bytes / per / 256 * 256)));
   p.many = p.piece < h.n;
-  p.splits_dx = h.want_dx ? split_of(h.d, p.piece, p.ld / 64) : 1;
-  p.splits_dw = h.want_dw && !p.many ? split_of(h.d, h.V, ceil_div(p.piece, 64)) : 1;
+  p.splits_dx = p.splits_dw = 1;
+  // partial sums of at most a quarter of the pieces' bytes (64 runs at most); pieces of rows already sum into dw
+  auto most = [&](long long rows) { return (int)std::max(1LL, std::min(64LL, h.piece_bytes / 4 / (rows * h.d * 4))); };
+  if (h.want_dx) p.tile_dx = pick_tile(h.d, p.piece, h.V, p.terms, most(p.piece), &p.splits_dx);
+  if (h.want_dw) p.tile_dw = pick_tile(h.d, h.V, p.piece, p.terms, p.many ? 1 : most(h.V), &p.splits_dw);
   long long o = 0;
   auto take = [&](bool want, long long bytes) {
     const long long at = o;
@@ -877,9 +970,11 @@ static void pack_rows(const void* src, long long rs, long long cs, long long row
 }
 
 template <int LA, int LB, typename T>
-static void grad_product(GradArgs g, bool big, hipStream_t s) {
-  if (big)
+static void grad_product(GradArgs g, int tile, hipStream_t s) {
+  if (tile == kBig)
     grad_launch<CfgBig, LA, LB, T>(g, s);
+  else if (tile == kWide)
+    grad_launch<CfgWide, LA, LB, T>(g, s);
   else
     grad_launch<CfgMid, LA, LB, T>(g, s);
 }
@@ -929,8 +1024,7 @@ static void scores(const HeadIn& h, const HeadPlan& p, const HeadOps& o, long lo
   ScoreArgs a = {};
   a.w = o.w;
   a.x = rows_from(o.x, r0, rows);
-  a.K = p.kp;
-  a.nkt = (int)(p.kp / 64);
+  a.K = (int)p.kp;
   a.terms = p.terms;
   a.V = (int)h.V;
   a.n = (int)rows;
@@ -941,12 +1035,30 @@ static void scores(const HeadIn& h, const HeadPlan& p, const HeadOps& o, long lo
   a.e = ws + p.o_e;
   a.z = (float*)(ws + p.o_e);
   a.ld = p.ld;
+  const int tile = pick_tile(h.V, rows, p.kp, p.terms, 1, nullptr);
   if (rows <= 64)
     scores_launch<CfgSlim>(a, mode, s);
-  else if (use_big(h.V, rows))
+  else if (tile == kBig)
     scores_launch<CfgBig>(a, mode, s);
+  else if (tile == kWide)
+    scores_launch<CfgWide>(a, mode, s);
   else
     scores_launch<CfgMid>(a, mode, s);
+}
+
+// whole, aligned 16-byte pieces in the rows of x and w
+static int dots_vec(const HeadIn& h, const void* x, const void* w) {
+  const long long e = h.f32 ? 4 : 8;
+  return h.xcs == 1 && h.wcs == 1 && h.d % e == 0 && h.xrs % e == 0 && h.wrs % e == 0 && ((uintptr_t)x & 15) == 0 && ((uintptr_t)w & 15) == 0;
+}
+
+template <typename T>
+static void targets(const TargetArgs& t, hipStream_t s) {
+  if (t.k == 1)
+    target_kernel<T, 1><<<ceil_div(t.n, 4), 256, 0, s>>>(t);
+  else
+    target_kernel<T, 4><<<ceil_div((long long)t.n * ceil_div(t.k, 4), 4), 256, 0, s>>>(t);
+  YTK_LAUNCH_CHECK();
 }
 
 static void rows_pass(RowArgs a, hipStream_t s) {
@@ -982,14 +1094,13 @@ extern "C" void ytk_head_loss(const uintptr_t* ptrs, const long long* lp, double
     t.xrs = h.xrs, t.xcs = h.xcs, t.wrs = h.wrs, t.wcs = h.wcs;
     t.idx = idx + r0 * h.k * (h.idx64 ? 8 : 4);
     t.idx64 = (int)h.idx64;
-    t.k = (int)h.k, t.n = (int)rows, t.d = (int)h.d, t.V = (int)h.V, t.f32 = (int)h.f32;
+    t.k = (int)h.k, t.n = (int)rows, t.d = (int)h.d, t.V = (int)h.V, t.vec = dots_vec(h, x, w);
     t.inv_t = 1.0f / temp;
     t.zt = (float*)(ws + p.o_zt);
     if (h.f32)
-      target_kernel<float><<<ceil_div(rows * h.k, 4), 256, 0, s>>>(t);
+      targets<float>(t, s);
     else
-      target_kernel<__bf16><<<ceil_div(rows * h.k, 4), 256, 0, s>>>(t);
-    YTK_LAUNCH_CHECK();
+      targets<__bf16>(t, s);
     RowArgs r = {};
     r.stats = (const float2*)(ws + p.o_stats);
     r.groups = (int)p.groups, r.n = (int)rows, r.base = (int)h.base;
@@ -1033,17 +1144,16 @@ extern "C" void ytk_head_loss(const uintptr_t* ptrs, const long long* lp, double
       g.a.ext = (int)(p.pack_w ? p.kp : h.d);
       g.b = D;
       g.ka = h.V, g.kb = p.ld;
-      g.nkt = (int)(p.ld / 64), g.terms = p.terms, g.splits = p.splits_dx;
+      g.K = (int)h.V, g.terms = p.terms, g.splits = p.splits_dx;
       g.M = (int)h.d, g.N = (int)rows;
       g.out = (char*)ptrs[10] + r0 * h.d * el, g.ldo = h.d;
       g.acc = (float*)(ws + p.o_split);
       g.mode = g.splits > 1 ? 1 : 0;
-      const bool big = g.splits == 1 && use_big(g.M, g.N);
       if (h.f32) {
-        grad_product<kKS, kKC, float>(g, big, s);
+        grad_product<kKS, kKC, float>(g, p.tile_dx, s);
         if (g.splits > 1) split_sum<float>(g.acc, g.splits, rows, h.d, g.out, s);
       } else {
-        grad_product<kKS, kKC, __bf16>(g, big, s);
+        grad_product<kKS, kKC, __bf16>(g, p.tile_dx, s);
         if (g.splits > 1) split_sum<__bf16>(g.acc, g.splits, rows, h.d, g.out, s);
       }
     }
@@ -1057,17 +1167,16 @@ extern "C" void ytk_head_loss(const uintptr_t* ptrs, const long long* lp, double
       g.b = D;
       g.b.ext = (int)p.ld;
       g.ka = g.kb = rows;
-      g.nkt = ceil_div(rows, 64), g.terms = p.terms, g.splits = p.splits_dw;
+      g.K = (int)rows, g.terms = p.terms, g.splits = p.splits_dw;
       g.M = (int)h.d, g.N = (int)h.V;
       g.out = (void*)ptrs[11], g.ldo = h.d;
       g.acc = (float*)(ws + (p.many ? p.o_dwacc : p.o_split));
       g.mode = g.splits > 1 ? 1 : !p.many ? 0 : first ? 1 : last ? 3 : 2;
-      const bool big = g.splits == 1 && use_big(g.M, g.N);
       if (h.f32) {
-        grad_product<kKS, kKS, float>(g, big, s);
+        grad_product<kKS, kKS, float>(g, p.tile_dw, s);
         if (g.splits > 1) split_sum<float>(g.acc, g.splits, h.V, h.d, g.out, s);
       } else {
-        grad_product<kKS, kKS, __bf16>(g, big, s);
+        grad_product<kKS, kKS, __bf16>(g, p.tile_dw, s);
         if (g.splits > 1) split_sum<__bf16>(g.acc, g.splits, h.V, h.d, g.out, s);
       }
     }
@@ -1100,6 +1209,7 @@ extern "C" void ytk_head_topk(const uintptr_t* ptrs, const long long* lp, double
     t.z = (const float*)(ws + p.o_e);
     t.ld = p.ld;
     t.n = (int)rows, t.V = (int)h.V, t.d = (int)h.d, t.groups = (int)p.groups;
+    t.vec = dots_vec(h, x, w);
     t.k = (int)h.k, t.kc = (int)std::min(h.k + kSpare, h.V);
     t.x = x + r0 * h.xrs * el, t.w = w, t.bias = bias;
     t.xrs = h.xrs, t.xcs = h.xcs, t.wrs = h.wrs, t.wcs = h.wcs;
@@ -1108,10 +1218,11 @@ extern "C" void ytk_head_topk(const uintptr_t* ptrs, const long long* lp, double
     t.classes = (long long*)ptrs[5] + r0 * h.k;
     const size_t lds = std::max<size_t>(std::min<long long>(t.kc, p.groups) * kGroup * 8,
                                         p.groups > t.kc && p.groups <= kTopKeys ? p.groups * 4 : 0);
+    const int threads = rows < 256 ? 1024 : 256;  // fewer rows than CUs: more waves for each
     if (h.f32)
-      topk_kernel<float><<<(int)rows, 256, lds, s>>>(t);
+      topk_kernel<float><<<(int)rows, threads, lds, s>>>(t);
     else
-      topk_kernel<__bf16><<<(int)rows, 256, lds, s>>>(t);
+      topk_kernel<__bf16><<<(int)rows, threads, lds, s>>>(t);
     YTK_LAUNCH_CHECK();
   }
 }

@@ -1,7 +1,7 @@
 // Matrix-product core of the class head (head.hip): C[m][n] = sum_k A[m][k] B[n][k] in bf16 on the
 // matrix cores, fp32 accumulators, gfx950 only.
 //
-// One block computes a kBM x kBN tile in K steps of 64. An operand lies in memory either with K
+// One block computes a kBM x kBN tile in K steps of kBK = 64 or 32. An operand lies in memory either with K
 // contiguous (kKC: row r holds its K values) or with K strided (kKS: row k holds the values of all m or n);
 // the three products of a softmax head need all of them from the same row-major x, w and D:
 //   scores  z^T[v][i] = sum_d w[v][d] x[i][d]   A = w (KC)  B = x (KC)
@@ -46,8 +46,9 @@ struct Operand {
   int ext;          // extent of M (or N)
 };
 
-__device__ __forceinline__ void dma16(unsigned voff, i32x4 rsrc, unsigned lds) {
-  asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tbuffer_load_dwordx4 %0, %1, 0 offen lds" ::"v"(voff), "s"(rsrc), "s"(lds)
+__device__ __forceinline__ void dma16(unsigned voff, i32x4 rsrc, unsigned soff, unsigned lds) {
+  asm volatile("s_mov_b32 m0, %3\n\ts_nop 0\n\tbuffer_load_dwordx4 %0, %1, %2 offen lds" ::"v"(voff), "s"(rsrc), "s"(soff),
+               "s"(lds)
                : "memory");
 }
 template <int N>
@@ -57,16 +58,20 @@ __device__ __forceinline__ void wait_vm() {
 __device__ __forceinline__ void wait_lgkm() { asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory"); }
 
 // one operand's side of the tile: kT = tile extent, kNW waves load it, kFB 32-wide fragments per wave
-template <int kL, int kT, int kNW, int kFB>
+template <int kL, int kT, int kNW, int kFB, int kBK>
 struct Side {
-  static constexpr int kBytes = kT * 128;
-  static constexpr int kLoads = kT / 8 / kNW;  // DMA instructions per wave and stage
-  static_assert(kT % (8 * kNW) == 0, "tile not divisible among the waves");
+  static constexpr int kBytes = kT * kBK * 2;       // per stage
+  static constexpr int kLoads = kBytes / 1024 / kNW;  // DMA instructions per wave and stage
+  static_assert(kBytes % (1024 * kNW) == 0, "tile not divisible among the waves");
+  static constexpr int kCh = kBK / 8, kRpi = 64 / kCh;  // KC: 16-B chunks per row, rows per DMA instruction
+  static_assert(kBK == 32 || kBK == 64, "");
+  // KC swizzle: a ds_read_b128 serves rows {0-3, 12-15, 20-23, 24-27} of a fragment (or 16 in a row) together
+  static __device__ __forceinline__ int swc(int row) { return kBK == 64 ? (row >> 1) & 7 : (row >> 2) & 3; }
   static constexpr int kRow = kT * 2;          // KS: LDS bytes per k row
   static constexpr int kUnits = kRow / 64;
   unsigned voff[kLoads];
   unsigned lds0;                // wave's first LDS byte of a stage
-  unsigned rd[kL == kKC ? 4 : kFB];
+  unsigned rd[kL == kKC ? kBK / 16 : kFB];
   const char* base;
   long long rem;                // bytes to the operand's end
   long long step, plane;
@@ -78,16 +83,16 @@ struct Side {
     if (kL == kKC) {
 #pragma unroll
       for (int i = 0; i < kLoads; ++i) {
-        const int row = (i * kNW + wave) * 8 + (l >> 3);
-        voff[i] = (unsigned)(row * o.pitch) + (((l & 7) ^ (row & 7)) << 4);
+        const int row = (i * kNW + wave) * kRpi + l / kCh;
+        voff[i] = (unsigned)(row * o.pitch) + (((l & (kCh - 1)) ^ swc(row)) << 4);
       }
-      base = o.p + (long long)t0 * o.pitch + kt0 * 128LL;
-      rem = (long long)(o.ext - t0 - 1) * o.pitch + (K - kt0 * 64LL) * 2;
-      step = 128;
+      base = o.p + (long long)t0 * o.pitch + kt0 * (kBK * 2LL);
+      rem = (long long)(o.ext - t0 - 1) * o.pitch + (K - kt0 * (long long)kBK) * 2;
+      step = kBK * 2;
 #pragma unroll
-      for (int s = 0; s < 4; ++s) {
+      for (int s = 0; s < kBK / 16; ++s) {
         const int row = frag0 * 32 + (l & 31);
-        rd[s] = lds + row * 128 + (((s * 2 + (l >> 5)) ^ (row & 7)) << 4);
+        rd[s] = lds + row * kBK * 2 + (((s * 2 + (l >> 5)) ^ swc(row)) << 4);
       }
     } else {
 #pragma unroll
@@ -96,9 +101,9 @@ struct Side {
         const int row = byte / kRow, chunk = (byte % kRow) / 16;
         voff[i] = (unsigned)(row * o.pitch) + ((((chunk >> 2) ^ swz(row)) << 2 | (chunk & 3)) << 4);
       }
-      base = o.p + kt0 * 64LL * o.pitch + t0 * 2LL;
-      rem = (K - kt0 * 64LL - 1) * o.pitch + (long long)(o.ext - t0) * 2;
-      step = 64 * o.pitch;
+      base = o.p + kt0 * (long long)kBK * o.pitch + t0 * 2LL;
+      rem = (K - kt0 * (long long)kBK - 1) * o.pitch + (long long)(o.ext - t0) * 2;
+      step = kBK * o.pitch;
       const int g = l >> 4, i16 = l & 15, row = (g >> 1) * 8 + (i16 >> 2);
 #pragma unroll
       for (int b = 0; b < kFB; ++b)
@@ -108,20 +113,28 @@ struct Side {
     lds0 = lds + wave * 1024;
   }
 
-  // stage of K step `kt` (relative to kt0), plane `pl`, into LDS stage offset `so`
-  __device__ __forceinline__ void issue(int kt, int pl, unsigned so) const {
-    const unsigned long long a = (unsigned long long)(base + kt * step + pl * plane);
-    long long r = rem - kt * step;
-    r = r < 0 ? 0 : r > 0x7fffffffLL ? 0x7fffffffLL : r;
+  // Buffer descriptor and scalar offset of K step `kt` (relative to kt0), plane `pl`; no records where there is
+  // none. A KC tile spans less than 2^31 bytes (checked by the host), so K is the scalar offset;
+  // a KS operand may be longer than 2^32 bytes, so K moves the base.
+  struct Src {
     i32x4 d;
-    d[0] = (int)(unsigned)a;
-    d[1] = (int)((a >> 32) & 0xffff);
-    d[2] = (int)r;
-    d[3] = 0x00020000;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) d[i] = __builtin_amdgcn_readfirstlane(d[i]);
-#pragma unroll
-    for (int i = 0; i < kLoads; ++i) dma16(voff[i], d, __builtin_amdgcn_readfirstlane(lds0 + so + i * kNW * 1024));
+    unsigned soff;
+  };
+  __device__ __forceinline__ Src src(int kt, int pl, bool some) const {
+    const long long k = kL == kKC ? 0 : kt * step;
+    const unsigned long long a = (unsigned long long)(base + k + pl * plane);
+    const unsigned long long r = (unsigned long long)(rem - k);
+    Src s;
+    s.d[0] = __builtin_amdgcn_readfirstlane((int)(unsigned)a);
+    s.d[1] = __builtin_amdgcn_readfirstlane((int)((a >> 32) & 0xffff));
+    s.d[2] = __builtin_amdgcn_readfirstlane(!some || (r >> 63) ? 0 : (r >> 31) ? 0x7fffffff : (int)(unsigned)r);
+    s.d[3] = 0x00020000;
+    s.soff = kL == kKC ? __builtin_amdgcn_readfirstlane(kt * (kBK * 2)) : 0u;
+    return s;
+  }
+  // this wave's i-th piece of the stage at LDS offset `so`
+  __device__ __forceinline__ void issue(int i, const Src& s, unsigned so) const {
+    dma16(voff[i], s.d, s.soff, __builtin_amdgcn_readfirstlane(lds0 + so + i * kNW * 1024));
   }
 
   __device__ __forceinline__ bf16x8 frag(int b, int s, unsigned so) const {
@@ -129,7 +142,7 @@ struct Side {
     typedef __attribute__((address_space(3))) bf16x8 l8;
     typedef __attribute__((address_space(3))) bf16x4 l4;
     // constant parts as pointer arithmetic: they become the instruction's offset
-    if (kL == kKC) return *(const l8*)((const lc*)(uintptr_t)(rd[s] + so) + b * 4096);
+    if (kL == kKC) return *(const l8*)((const lc*)(uintptr_t)(rd[s] + so) + b * 64 * kBK);
     const lc* q = (const lc*)(uintptr_t)(rd[b] + so) + s * 16 * kRow;
     const bf16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4bf16((l4*)q);
     const bf16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4bf16((l4*)(q + 4 * kRow));
@@ -137,17 +150,18 @@ struct Side {
   }
 };
 
-template <int BM, int BN, int WM, int WN, int S>
+template <int BM, int BN, int WM, int WN, int BK, int S>
 struct TileCfg {
-  static constexpr int kBM = BM, kBN = BN, kWM = WM, kWN = WN, kStages = S;
+  static constexpr int kBM = BM, kBN = BN, kWM = WM, kWN = WN, kBK = BK, kStages = S;
   static constexpr int kNW = WM * WN, kThreads = 64 * kNW;
   static constexpr int kFM = BM / WM / 32, kFN = BN / WN / 32;  // 32x32 blocks per wave
-  static constexpr unsigned kStageBytes = (BM + BN) * 128;
+  static constexpr unsigned kStageBytes = (BM + BN) * BK * 2;
   static constexpr unsigned kLds = S * kStageBytes;
 };
 
 // (ka, kb: extent of K in each operand's memory; a KC operand's is a multiple of 64)
-// acc += A[m0.., kt0*64 ..] B[n0.., ...]^T over `nkt` K steps and `terms` plane pairs (1 or 6)
+// acc += A[m0.., kt0*kBK ..] B[n0.., ...]^T over `nkt` K steps and `terms` plane pairs (1 or 6). Both operands have
+// K left at every step: (kt0 + nkt - 1) * kBK < min(ka, kb).
 template <class C, int kLA, int kLB>
 __device__ __forceinline__ void gemm_loop(const Operand& A, const Operand& B, int m0, int n0, long long ka, long long kb,
                                           int kt0, int nkt, int terms, f32x16 (&acc)[C::kFM][C::kFN]) {
@@ -156,83 +170,96 @@ __device__ __forceinline__ void gemm_loop(const Operand& A, const Operand& B, in
   const unsigned lds = (unsigned)(uintptr_t)(lc*)head_smem;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int wm = wave / C::kWN, wn = wave % C::kWN;
-  Side<kLA, C::kBM, C::kNW, C::kFM> a;
-  Side<kLB, C::kBN, C::kNW, C::kFN> b;
+  typedef Side<kLA, C::kBM, C::kNW, C::kFM, C::kBK> SideA;
+  typedef Side<kLB, C::kBN, C::kNW, C::kFN, C::kBK> SideB;
+  SideA a;
+  SideB b;
   a.init(A, m0, ka, kt0, wave, wm * C::kFM, lds);
-  b.init(B, n0, kb, kt0, wave, wn * C::kFN, lds + C::kBM * 128);
-  constexpr int kLoads = Side<kLA, C::kBM, C::kNW, C::kFM>::kLoads + Side<kLB, C::kBN, C::kNW, C::kFN>::kLoads;
+  b.init(B, n0, kb, kt0, wave, wn * C::kFN, lds + SideA::kBytes);
+  constexpr int kLoads = SideA::kLoads + SideB::kLoads;
   const int iters = nkt * terms;
   int ikt = 0, iterm = 0;  // next stage to issue
   const unsigned ta = terms == 1 ? 0u : kTermA, tb = terms == 1 ? 0u : kTermB;
-  auto issue = [&](unsigned so) {
-    a.issue(ikt, (ta >> (2 * iterm)) & 3, so);
-    b.issue(ikt, (tb >> (2 * iterm)) & 3, so);
+  typename SideA::Src da;
+  typename SideB::Src db;
+  auto next = [&]() {
+    const bool some = ikt < nkt;
+    da = a.src(some ? ikt : 0, (ta >> (2 * iterm)) & 3, some);
+    db = b.src(some ? ikt : 0, (tb >> (2 * iterm)) & 3, some);
     if (++iterm == terms) {
       iterm = 0;
       ++ikt;
     }
   };
+  auto piece = [&](int i, unsigned so) {
+    if (i < SideA::kLoads)
+      a.issue(i, da, so);
+    else
+      b.issue(i - SideA::kLoads, db, so);
+  };
+  constexpr int S = C::kStages;
+  static_assert(S >= 3, "");
+  // S - 1 stages under way; a stage past the last is filled with zeros that nothing reads, so that every step
+  // issues and waits for the same number of loads
 #pragma unroll
-  for (int s = 0; s < C::kStages; ++s)
-    if (s < iters) issue(s * C::kStageBytes);
-  if (iters > C::kStages - 1)
-    wait_vm<(C::kStages - 1) * kLoads>();
-  else
-    wait_vm<0>();
+  for (int s = 0; s < S - 1; ++s) {
+    next();
+#pragma unroll
+    for (int i = 0; i < kLoads; ++i) piece(i, s * C::kStageBytes);
+  }
+  wait_vm<(S - 2) * kLoads>();
   __builtin_amdgcn_s_barrier();
 
   bf16x8 fa[2][C::kFM], fb[2][C::kFN];
-  auto read = [&](int p, int s, unsigned so) {
-#pragma unroll
-    for (int i = 0; i < C::kFM; ++i) fa[p][i] = a.frag(i, s, so);
-#pragma unroll
-    for (int j = 0; j < C::kFN; ++j) fb[p][j] = b.frag(j, s, so);
-  };
-  auto mma = [&](int p) {
-#pragma unroll
-    for (int i = 0; i < C::kFM; ++i)
-#pragma unroll
-      for (int j = 0; j < C::kFN; ++j)
-        acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(fa[p][i], fb[p][j], acc[i][j], 0, 0, 0);
-  };
-  // one quarter: the next quarter's fragments are read between this quarter's products
-  constexpr int kReads = C::kFM * (kLA == kKC ? 1 : 2) + C::kFN * (kLB == kKC ? 1 : 2), kMma = C::kFM * C::kFN;
-  auto weave = [&]() {
-    constexpr int per = (kReads + kMma - 1) / kMma;
-#pragma unroll
-    for (int i = 0; i < kMma; ++i) {
-      __builtin_amdgcn_sched_group_barrier(0x100, per, 0);  // LDS reads
-      __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);    // matrix product
-    }
-    __builtin_amdgcn_sched_barrier(0);
-  };
-  unsigned so = 0;
-  read(0, 0, 0);
-  for (int it = 0; it < iters; ++it) {
-    read(1, 1, so);
-    mma(0);
-    weave();
-    read(0, 2, so);
-    mma(1);
-    weave();
-    read(1, 3, so);
-    mma(0);
-    weave();
-    // every read of this stage has returned, and the next stage has landed: one barrier hands this
-    // buffer back to the DMA while the last quarter's products still run
-    wait_lgkm();
-    if (it + C::kStages <= iters)
-      wait_vm<(C::kStages - 2) * kLoads>();
+  auto read = [&](int r, int p, int q, unsigned so) {
+    if (r < C::kFN)
+      fb[p][r] = b.frag(r, q, so);
     else
-      wait_vm<0>();
-    __builtin_amdgcn_s_barrier();
-    if (it + C::kStages < iters) issue(so);
-    so = so + C::kStageBytes == C::kLds ? 0u : so + C::kStageBytes;
-    // (after the last step this reads a stage that holds old data; nothing uses it)
-    read(0, 0, so);
-    mma(1);
-    weave();
+      fa[p][r - C::kFN] = a.frag(r - C::kFN, q, so);
+  };
+  // kQ quarters per K step, each kFM rows of products. The next quarter's kR fragments are read during the first
+  // half of a quarter (they have returned by its end), the DMA is issued in the second half: in one
+  // burst, the loads stall every wave at the memory unit (1.20 -> 1.34 PFLOP/s at 32768 x 8192 x 4096).
+  constexpr int kQ = C::kBK / 16, kR = C::kFM + C::kFN, kHalf = C::kFM / 2, kSlots = kQ * (C::kFM - kHalf);
+  // DMA instructions that may still be under way when the next stage has landed
+  constexpr int kAhead = (S - 3) * kLoads + (kQ - 1) * (C::kFM - kHalf) * kLoads / kSlots;
+  unsigned so = 0, fill = (S - 1) * C::kStageBytes;  // stage being read, stage being filled
+#pragma unroll
+  for (int r = 0; r < kR; ++r) read(r, 0, 0, 0);
+  for (int it = 0; it < iters; ++it) {
+    next();
+    const unsigned after = so + C::kStageBytes == C::kLds ? 0u : so + C::kStageBytes;
+#pragma unroll
+    for (int q = 0; q < kQ; ++q) {
+      if (q == kQ - 1) {
+        // every read of this stage has returned and the next stage has landed: one barrier hands this buffer
+        // to the DMA of the next step, while the products of the last quarter, already in registers, follow
+        wait_lgkm();
+        wait_vm<kAhead>();
+        __builtin_amdgcn_s_barrier();
+      }
+#pragma unroll
+      for (int i = 0; i < C::kFM; ++i) {
+#pragma unroll
+        for (int j = 0; j < C::kFN; ++j)
+          acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(fa[q & 1][i], fb[q & 1][j], acc[i][j], 0, 0, 0);
+        if (i < kHalf) {
+          // (after the last step: from a stage whose data nothing uses)
+#pragma unroll
+          for (int r = i * kR / kHalf; r < (i + 1) * kR / kHalf; ++r)
+            read(r, (q + 1) & 1, (q + 1) % kQ, q == kQ - 1 ? after : so);
+        } else {
+          const int slot = q * (C::kFM - kHalf) + i - kHalf;
+#pragma unroll
+          for (int u = slot * kLoads / kSlots; u < (slot + 1) * kLoads / kSlots; ++u) piece(u, fill);
+        }
+        __builtin_amdgcn_sched_barrier(0);
+      }
+    }
+    so = after;
+    fill = fill + C::kStageBytes == C::kLds ? 0u : fill + C::kStageBytes;
   }
+  wait_vm<0>();  // no DMA outlives the block
 }
 
 // block -> tile: each XCD (blocks go to them round robin) works through a contiguous run of the tile

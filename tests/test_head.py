@@ -366,6 +366,18 @@ def test_loss_larger(cuda, dtype, n, d, V):
         assert torch.equal(a, c)  # bitwise reproducible
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", BOTH)
+def test_loss_many_rows(cuda, dtype):
+    """More rows than one piece holds at most, few classes."""
+    n = (1 << 21) + 777
+    x, w, y, b = make(n, 3, 4, dtype, cuda, bias=True)
+    r = head.softmax_head_loss(x, w, y, bias=b)
+    Ref(x, w, *label_targets(y), bias=b).check(r, db=True)
+    v, c, _ = head.head_topk(x, w, 2, bias=b)
+    assert torch.equal(c, topk_ref(x, w, b, 1.0, 2)[1])
+
+
 # ------------------------------------------------------------------ distillation
 @pytest.mark.gpu
 @pytest.mark.parametrize("dtype", BOTH)

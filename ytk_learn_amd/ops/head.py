@@ -29,7 +29,7 @@ from ._ext import hip, ptr, stream
 # bytes of exponentials (or scores, head_topk) that live at a time; rows beyond are taken in further pieces
 PIECE_BYTES = 2 << 30
 MAX_LIST = 256           # entries of a teacher's list, and k of head_topk
-MAX_DIM = (1 << 22) - 64  # classes, features
+MAX_DIM = 1 << 21         # classes, features
 _TYPES = (torch.float32, torch.bfloat16)
 
 
@@ -66,7 +66,7 @@ def _check(x, w, bias, temperature, **rows):
 def _aligned(t):
     """Whether the products can read the rows in place: 16-byte pieces, whole steps of 64 columns."""
     return int(t.dtype == torch.bfloat16 and t.stride(1) == 1 and t.shape[1] % 64 == 0 and t.stride(0) % 8 == 0
-               and t.stride(0) >= t.shape[1] and t.data_ptr() % 16 == 0 and t.stride(0) < 1 << 22)
+               and t.stride(0) >= t.shape[1] and t.data_ptr() % 16 == 0 and t.stride(0) <= 1 << 21)
 
 
 def _strided(t):
