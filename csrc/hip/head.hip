@@ -102,11 +102,11 @@ __global__ __launch_bounds__(256) void pack_kernel(const T* __restrict__ src, lo
 // ------------------------------------------------------------------ scores
 struct ScoreArgs {
   Operand w, x;
-  int K, terms;       // padded d; plane pairs
+  int K;              // padded d
   int V, n;
   int nm, nn;         // tiles
   const void* bias;   // element type of the inputs
-  int bias_f32;
+  int f32;            // inputs (and bias)
   float inv_t;
   float2* stats;      // [groups][n]: m, s
   void* e;            // E [n][ld] (fp16 or fp32) or null
@@ -144,87 +144,117 @@ __device__ __forceinline__ float exp_of(float v) {
   return e == 0.0f || v == -INFINITY ? 0.0f : fmaf(e * r, 0.6931471805599453f, e);
 }
 
-enum { kStatsOnly = 0, kExpHalf = 1, kExpFloat = 2, kScores = 3 };
+// what a call keeps of its scores: nothing (bf16, fp32 inputs), E (bf16, fp32), the scores
+enum { kStatsOnly = 0, kExpHalf = 1, kExpFloat = 2, kScores = 3, kStatsFloat = 4 };
 
-template <class C, int kMode>
+// Maxima are in the unit of the stats: log2 units for bf16 inputs with a loss (the exponential is one fma and
+// one exp2 from the accumulator), natural ones otherwise (fp32: a finer exponential; top k: the stored scores' own).
+template <int kMode>
+constexpr bool kBase2 = kMode == kStatsOnly || kMode == kExpHalf;
+
+template <class C, int kMode, int kTerms>
 __global__ __launch_bounds__(C::kThreads) void scores_kernel(ScoreArgs p) {
-  int tm, tn;
-  if (!tile_of(p.nm, p.nn, tm, tn)) return;
-  f32x16 acc[C::kFM][C::kFN] = {};
-  gemm_loop<C, kKC, kKC>(p.w, p.x, tm * C::kBM, tn * C::kBN, p.K, p.K, 0, p.K / C::kBK, p.terms, acc);
   static_assert(C::kFM % 2 == 0, "a wave holds whole groups");
   const int wave = threadIdx.x >> 6, l = threadIdx.x & 63, hi = l >> 5;
-  const int v0 = tm * C::kBM + (wave / C::kWN) * C::kFM * 32, i0 = tn * C::kBN + (wave % C::kWN) * C::kFN * 32;
+  gemm_tiles<C, kKC, kKC, kTerms>(
+      p.w, p.x, p.K, p.K,
+      [&](int j, int& m0, int& n0, int& kt0, int& nkt) {
+        int tm, tn;
+        if (!tile_of(j, p.nm, p.nn, tm, tn)) return false;
+        m0 = tm * C::kBM, n0 = tn * C::kBN, kt0 = 0, nkt = p.K / C::kBK;
+        return true;
+      },
+      [&](int, int m0, int n0, f32x16(&acc)[C::kFM][C::kFN]) {
+        const int v0 = m0 + (wave / C::kWN) * C::kFM * 32, i0 = n0 + (wave % C::kWN) * C::kFN * 32;
 #pragma unroll
-  for (int g = 0; g < C::kFM / 2; ++g) {
-    const int vg = v0 + g * kGroup;
-    if (vg >= p.V) break;
-    float b[2][16];
+        for (int g = 0; g < C::kFM / 2; ++g) {
+          const int vg = v0 + g * kGroup;
+          if (vg >= p.V) break;
+          if (p.bias) {  // (past the last class: the last one's bias, and -inf below)
+            float b[2][16];
 #pragma unroll
-    for (int h = 0; h < 2; ++h)
+            for (int h = 0; h < 2; ++h)
 #pragma unroll
-      for (int r = 0; r < 16; ++r) {
-        const int v = vg + h * 32 + 8 * (r >> 2) + 4 * hi + (r & 3);
-        b[h][r] = v >= p.V ? -INFINITY
-                  : !p.bias ? 0.0f
-                  : p.bias_f32 ? ((const float*)p.bias)[v]
-                               : (float)((const __bf16*)p.bias)[v];
-      }
+              for (int r = 0; r < 16; ++r) {
+                const int v = min(vg + h * 32 + 8 * (r >> 2) + 4 * hi + (r & 3), p.V - 1);
+                b[h][r] = kTerms == 6 ? ((const float*)p.bias)[v] : (float)((const __bf16*)p.bias)[v];
+              }
 #pragma unroll
-    for (int j = 0; j < C::kFN; ++j) {
-      const int i = i0 + j * 32 + (l & 31);
-      float z[2][16], m = -INFINITY;
+            for (int h = 0; h < 2; ++h)
 #pragma unroll
-      for (int h = 0; h < 2; ++h)
+              for (int j = 0; j < C::kFN; ++j)
 #pragma unroll
-        for (int r = 0; r < 16; ++r) {
-          // a class past the end is -inf whatever the product holds (its operand rows read as zero)
-          z[h][r] = (acc[2 * g + h][j][r] + b[h][r]) * p.inv_t;
-          m = fmaxf(m, z[h][r]);
-        }
-      m = fmaxf(m, __shfl_xor(m, 32, 64));
-      const float m0 = m == -INFINITY ? 0.0f : m;
-      float s = 0.0f;
-      if (kMode == kScores && i < p.n) {
-        float* o = p.z + (long long)i * p.ld + vg + 4 * hi;
-#pragma unroll
-        for (int h = 0; h < 2; ++h)
-#pragma unroll
-          for (int q = 0; q < 4; ++q)
-            *(float4*)(o + h * 32 + 8 * q) = make_float4(z[h][4 * q], z[h][4 * q + 1], z[h][4 * q + 2], z[h][4 * q + 3]);
-      }
-#pragma unroll
-      for (int h = 0; h < 2; ++h)
-#pragma unroll
-        for (int r = 0; r < 16; ++r) {
-          z[h][r] = exp_of<kMode == kExpFloat>(z[h][r] - m0);
-          s += z[h][r];
-        }
-      s += __shfl_xor(s, 32, 64);
-      if (hi == 0 && i < p.n) p.stats[(long long)(vg / kGroup) * p.n + i] = make_float2(m, s);
-      if (kMode == kExpFloat && i < p.n) {
-        float* o = (float*)p.e + (long long)i * p.ld + vg + 4 * hi;
-#pragma unroll
-        for (int h = 0; h < 2; ++h)
-#pragma unroll
-          for (int q = 0; q < 4; ++q)
-            *(float4*)(o + h * 32 + 8 * q) = make_float4(z[h][4 * q], z[h][4 * q + 1], z[h][4 * q + 2], z[h][4 * q + 3]);
-      }
-      if (kMode == kExpHalf) {
-        unsigned short* o = (unsigned short*)p.e + (long long)i * p.ld + vg + 8 * hi;
-#pragma unroll
-        for (int h = 0; h < 2; ++h)
-#pragma unroll
-          for (int q = 0; q < 4; q += 2) {
-            const float k = 32768.0f;
-            unsigned a0 = pack_h2(z[h][4 * q] * k, z[h][4 * q + 1] * k), a1 = pack_h2(z[h][4 * q + 2] * k, z[h][4 * q + 3] * k);
-            unsigned b0 = pack_h2(z[h][4 * q + 4] * k, z[h][4 * q + 5] * k), b1 = pack_h2(z[h][4 * q + 6] * k, z[h][4 * q + 7] * k);
-            swap_quads(a0, a1, b0, b1);
-            if (i < p.n) *(uint4*)(o + h * 32 + 8 * q) = make_uint4(a0, a1, b0, b1);
+                for (int r = 0; r < 16; ++r) acc[2 * g + h][j][r] += b[h][r];
           }
-      }
-    }
-  }
+          if (vg + kGroup > p.V) {  // a class past the end is -inf (its operand rows read as zero)
+            const int left = p.V - vg - 4 * hi;
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+#pragma unroll
+              for (int r = 0; r < 16; ++r)
+#pragma unroll
+                for (int j = 0; j < C::kFN; ++j)
+                  if (h * 32 + 8 * (r >> 2) + (r & 3) >= left) acc[2 * g + h][j][r] = -INFINITY;
+          }
+          const float c = kBase2<kMode> ? p.inv_t * kLog2e : p.inv_t;
+#pragma unroll
+          for (int j = 0; j < C::kFN; ++j) {
+            const int i = i0 + j * 32 + (l & 31);
+            float mx = -INFINITY;
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+#pragma unroll
+              for (int r = 0; r < 16; ++r) mx = fmaxf(mx, acc[2 * g + h][j][r]);
+            const float m = fmaxf(mx, __shfl_xor(mx, 32, 64)) * c;
+            const float m0 = m == -INFINITY ? 0.0f : m;
+            if (kMode == kScores && i < p.n) {
+              float* o = p.z + (long long)i * p.ld + vg + 4 * hi;
+#pragma unroll
+              for (int h = 0; h < 2; ++h)
+#pragma unroll
+                for (int q = 0; q < 4; ++q) {
+                  const f32x16& t = acc[2 * g + h][j];
+                  *(float4*)(o + h * 32 + 8 * q) = make_float4(t[4 * q] * c, t[4 * q + 1] * c, t[4 * q + 2] * c, t[4 * q + 3] * c);
+                }
+            }
+            float s = 0.0f, e[2][16];
+            const float off = kMode == kExpHalf ? 15.0f - m0 : -m0;  // E is scaled by 2^15
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+#pragma unroll
+              for (int r = 0; r < 16; ++r) {
+                if (kBase2<kMode>)
+                  e[h][r] = __builtin_amdgcn_exp2f(fmaf(acc[2 * g + h][j][r], c, off));
+                else
+                  e[h][r] = exp_of<kMode == kExpFloat || kMode == kStatsFloat>(acc[2 * g + h][j][r] * c - m0);
+                s += e[h][r];
+              }
+            s += __shfl_xor(s, 32, 64);
+            if (kMode == kExpHalf) s *= 1.0f / 32768.0f;
+            if (hi == 0 && i < p.n) p.stats[(long long)(vg / kGroup) * p.n + i] = make_float2(m, s);
+            if (kMode == kExpFloat && i < p.n) {
+              float* o = (float*)p.e + (long long)i * p.ld + vg + 4 * hi;
+#pragma unroll
+              for (int h = 0; h < 2; ++h)
+#pragma unroll
+                for (int q = 0; q < 4; ++q)
+                  *(float4*)(o + h * 32 + 8 * q) = make_float4(e[h][4 * q], e[h][4 * q + 1], e[h][4 * q + 2], e[h][4 * q + 3]);
+            }
+            if (kMode == kExpHalf) {
+              unsigned short* o = (unsigned short*)p.e + (long long)i * p.ld + vg + 8 * hi;
+#pragma unroll
+              for (int h = 0; h < 2; ++h)
+#pragma unroll
+                for (int q = 0; q < 4; q += 2) {
+                  unsigned a0 = pack_h2(e[h][4 * q], e[h][4 * q + 1]), a1 = pack_h2(e[h][4 * q + 2], e[h][4 * q + 3]);
+                  unsigned b0 = pack_h2(e[h][4 * q + 4], e[h][4 * q + 5]), b1 = pack_h2(e[h][4 * q + 6], e[h][4 * q + 7]);
+                  swap_quads(a0, a1, b0, b1);
+                  if (i < p.n) *(uint4*)(o + h * 32 + 8 * q) = make_uint4(a0, a1, b0, b1);
+                }
+            }
+          }
+        }
+      });
 }
 
 // ------------------------------------------------------------------ targets
@@ -335,27 +365,35 @@ struct RowArgs {
   int rb;               // rows per block (a power of two, <= 16)
 };
 
+// kB2: the maxima are in log2 units
+template <bool kB2>
 __global__ __launch_bounds__(256) void row_kernel(RowArgs p) {
   __shared__ float sm[256], ss[256];
+  auto ex = [](float v) { return kB2 ? __builtin_amdgcn_exp2f(v) : exp_of<true>(v); };
   const int t = threadIdx.x, rl = t & (p.rb - 1), strip = t / p.rb, strips = 256 / p.rb;
   const long long row = (long long)blockIdx.x * p.rb + rl;
   // running maximum and sum over this thread's groups
   float m = -INFINITY, s = 0.0f;
   if (row < p.n) {
-    for (int g = strip; g < p.groups; g += strips) {
-      const float2 a = p.stats[(long long)g * p.n + row];
-      if (a.x > m) {
-        s = (m == -INFINITY ? 0.0f : s * exp_of<true>(m - a.x)) + a.y;
-        m = a.x;
-      } else if (a.x != -INFINITY) {
-        s += a.y * exp_of<true>(a.x - m);
-      } else if (a.y != 0.0f) {
-        s += a.y;  // NaN scores: the maximum passed over them
+    // four groups at a time: their loads are in flight together and share one rescaling
+    for (int g = strip; g < p.groups; g += 4 * strips) {
+      float2 a[4];
+      float nm = m;
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        const int gu = g + u * strips;
+        a[u] = gu < p.groups ? p.stats[(long long)gu * p.n + row] : make_float2(-INFINITY, 0.0f);
+        nm = fmaxf(nm, a[u].x);
       }
+      const float n0 = nm == -INFINITY ? 0.0f : nm;  // (groups of NaN scores: the maximum passed over them, s is NaN)
+      s *= ex(m - n0);
+#pragma unroll
+      for (int u = 0; u < 4; ++u) s += a[u].y * (a[u].x == -INFINITY ? 1.0f : ex(a[u].x - n0));
+      m = nm;
     }
     if (p.base && strip == 0) {
       const float nm = fmaxf(m, 0.0f);
-      s = (m == -INFINITY ? 0.0f : s * exp_of<true>(m - nm)) + exp_of<true>(-nm);
+      s = (m == -INFINITY ? 0.0f : s * ex(m - nm)) + ex(-nm);
       m = nm;
     }
   }
@@ -365,14 +403,14 @@ __global__ __launch_bounds__(256) void row_kernel(RowArgs p) {
   for (int h = 128; h >= p.rb; h >>= 1) {
     if (t < h) {
       const float m1 = sm[t], m2 = sm[t + h], nm = fmaxf(m1, m2), n0 = nm == -INFINITY ? 0.0f : nm;
-      ss[t] = ss[t] * exp_of<true>(m1 - n0) + ss[t + h] * exp_of<true>(m2 - n0);
+      ss[t] = ss[t] * ex(m1 - n0) + ss[t + h] * ex(m2 - n0);
       sm[t] = nm;
     }
     __syncthreads();
   }
   if (t < p.rb && row < p.n) {
     if (p.norm) p.norm[row] = make_float2(sm[t], 1.0f / ss[t]);
-    sm[t] = sm[t] + logf(ss[t]);
+    sm[t] = (kB2 ? sm[t] * 0.6931471805599453f : sm[t]) + logf(ss[t]);
     p.lse[row] = sm[t];
   }
   __syncthreads();
@@ -483,7 +521,8 @@ __global__ __launch_bounds__(256) void dscore_kernel(DArgs p) {
       const float co = cw[b] * nr[b].y;
       if (cw[b] != 0.0f) {
         // E is e^(z - m) with m = 0 for a group that has only -inf
-        const float f = co * exp_of<kF32>((m[b] == -INFINITY ? 0.0f : m[b]) - nr[b].x) * (kF32 ? 1.0f : 1.0f / 32768.0f);
+        const float mg = (m[b] == -INFINITY ? 0.0f : m[b]) - nr[b].x;
+        const float f = co * (kF32 ? exp_of<true>(mg) : __builtin_amdgcn_exp2f(mg - 15.0f));
 #pragma unroll
         for (int j = 0; j < 8; ++j) d[b][j] *= f;
         // target classes: p is taken from the fp32 score, and every entry of the list on that class is subtracted
@@ -496,7 +535,7 @@ __global__ __launch_bounds__(256) void dscore_kernel(DArgs p) {
             for (unsigned long long h = __ballot(at >= 0); h; h &= h - 1) {
               const int bit = __builtin_ctzll(h), vb = __builtin_amdgcn_readlane(at, bit);
               const long long e = i * p.k + j0 + bit;
-              const float x = pass == 0 ? co * exp_of<kF32>(p.zt[e] - nr[b].x) : p.q[e];
+              const float x = pass != 0 ? p.q[e] : co * (kF32 ? exp_of<true>(p.zt[e] - nr[b].x) : __builtin_amdgcn_exp2f(p.zt[e] * kLog2e - nr[b].x));
 #pragma unroll
               for (int u = 0; u < 8; ++u)
                 if (vb == l * 8 + u) d[b][u] = pass == 0 ? x : d[b][u] - x;
@@ -557,7 +596,7 @@ __global__ __launch_bounds__(256) void db_kernel(const float* __restrict__ part,
 struct GradArgs {
   Operand a, b;
   long long ka, kb;        // extent of K in each operand's memory
-  int K, terms, splits;    // products run over K (at most ka, kb), cut into `splits` runs of whole 64s
+  int K, splits;           // products run over K (at most ka, kb), cut into `splits` runs of whole 64s
   int M, N, nm, nn;        // result [N][M], M contiguous
   void* out;               // T [N][ldo]
   long long ldo;
@@ -567,58 +606,67 @@ struct GradArgs {
 
 template <class C, int kLA, int kLB, typename T>
 __global__ __launch_bounds__(C::kThreads) void grad_kernel(GradArgs p) {
-  int tm, tn;
-  if (!tile_of(p.nm, p.nn * p.splits, tm, tn)) return;
-  const int split = tn / p.nn;
-  tn -= split * p.nn;
-  const int per = (p.K + 64 * p.splits - 1) / (64 * p.splits) * 64, k0 = split * per, k1 = min(k0 + per, p.K);
-  const int kt0 = k0 / C::kBK, nkt = (k1 - k0 + C::kBK - 1) / C::kBK;
-  f32x16 acc[C::kFM][C::kFN] = {};
-  if (nkt > 0) gemm_loop<C, kLA, kLB>(p.a, p.b, tm * C::kBM, tn * C::kBN, p.ka, p.kb, kt0, nkt, p.terms, acc);
   const int wave = threadIdx.x >> 6, l = threadIdx.x & 63, hi = l >> 5;
-  const int m0 = tm * C::kBM + (wave / C::kWN) * C::kFM * 32, n0 = tn * C::kBN + (wave % C::kWN) * C::kFN * 32;
-  const bool vec = (p.ldo & 7) == 0 && ((uintptr_t)p.out & 15) == 0, avec = (p.M & 3) == 0;
+  // runs of whole 64s; the host leaves none of them empty
+  const int per = (p.K + 64 * p.splits - 1) / (64 * p.splits) * 64;
+  gemm_tiles<C, kLA, kLB, sizeof(T) == 4 ? 6 : 1>(
+      p.a, p.b, p.ka, p.kb,
+      [&](int j, int& m0, int& n0, int& kt0, int& nkt) {
+        int tm, tn;
+        if (!tile_of(j, p.nm, p.nn * p.splits, tm, tn)) return false;
+        const int k0 = tn / p.nn * per;
+        m0 = tm * C::kBM, n0 = tn % p.nn * C::kBN;
+        kt0 = k0 / C::kBK, nkt = (min(per, p.K - k0) + C::kBK - 1) / C::kBK;
+        return true;
+      },
+      [&](int j, int m0, int n0, f32x16(&acc)[C::kFM][C::kFN]) {
+        int tm, tn;
+        tile_of(j, p.nm, p.nn * p.splits, tm, tn);
+        const int split = tn / p.nn;
+        const int mw = m0 + (wave / C::kWN) * C::kFM * 32, nw = n0 + (wave % C::kWN) * C::kFN * 32;
+        const bool vec = (p.ldo & 7) == 0 && ((uintptr_t)p.out & 15) == 0, avec = (p.M & 3) == 0;
 #pragma unroll
-  for (int j = 0; j < C::kFN; ++j) {
-    const int n = n0 + j * 32 + (l & 31);
-    if (n >= p.N) continue;
+        for (int j = 0; j < C::kFN; ++j) {
+          const int n = nw + j * 32 + (l & 31);
+          if (n >= p.N) continue;
 #pragma unroll
-    for (int i = 0; i < C::kFM; ++i)
+          for (int i = 0; i < C::kFM; ++i)
 #pragma unroll
-      for (int q = 0; q < 4; ++q) {
-        const int m = m0 + i * 32 + 8 * q + 4 * hi;
-        if (m >= p.M) continue;
-        float v[4] = {acc[i][j][4 * q], acc[i][j][4 * q + 1], acc[i][j][4 * q + 2], acc[i][j][4 * q + 3]};
-        if (p.mode) {
-          float* a = p.acc + ((long long)split * p.N + n) * p.M + m;
-          if (avec) {
-            if (p.mode != 1) {
-              const float4 o = *(const float4*)a;
-              v[0] += o.x, v[1] += o.y, v[2] += o.z, v[3] += o.w;
-            }
-            if (p.mode != 3) *(float4*)a = make_float4(v[0], v[1], v[2], v[3]);
-          } else {
-            for (int u = 0; u < 4; ++u)
-              if (m + u < p.M) {
-                if (p.mode != 1) v[u] += a[u];
-                if (p.mode != 3) a[u] = v[u];
+            for (int q = 0; q < 4; ++q) {
+              const int m = mw + i * 32 + 8 * q + 4 * hi;
+              if (m >= p.M) continue;
+              float v[4] = {acc[i][j][4 * q], acc[i][j][4 * q + 1], acc[i][j][4 * q + 2], acc[i][j][4 * q + 3]};
+              if (p.mode) {
+                float* a = p.acc + ((long long)split * p.N + n) * p.M + m;
+                if (avec) {
+                  if (p.mode != 1) {
+                    const float4 o = *(const float4*)a;
+                    v[0] += o.x, v[1] += o.y, v[2] += o.z, v[3] += o.w;
+                  }
+                  if (p.mode != 3) *(float4*)a = make_float4(v[0], v[1], v[2], v[3]);
+                } else {
+                  for (int u = 0; u < 4; ++u)
+                    if (m + u < p.M) {
+                      if (p.mode != 1) v[u] += a[u];
+                      if (p.mode != 3) a[u] = v[u];
+                    }
+                }
               }
-          }
+              if (p.mode == 0 || p.mode == 3) {
+                T* o = (T*)p.out + (long long)n * p.ldo + m;
+                if (vec && m + 4 <= p.M) {
+                  if (sizeof(T) == 4)
+                    *(float4*)o = make_float4(v[0], v[1], v[2], v[3]);
+                  else
+                    *(uint2*)o = make_uint2(pack_b2(v[0], v[1]), pack_b2(v[2], v[3]));
+                } else {
+                  for (int u = 0; u < 4; ++u)
+                    if (m + u < p.M) Elem<T>::put(o, u, v[u]);
+                }
+              }
+            }
         }
-        if (p.mode == 0 || p.mode == 3) {
-          T* o = (T*)p.out + (long long)n * p.ldo + m;
-          if (vec && m + 4 <= p.M) {
-            if (sizeof(T) == 4)
-              *(float4*)o = make_float4(v[0], v[1], v[2], v[3]);
-            else
-              *(uint2*)o = make_uint2(pack_b2(v[0], v[1]), pack_b2(v[2], v[3]));
-          } else {
-            for (int u = 0; u < 4; ++u)
-              if (m + u < p.M) Elem<T>::put(o, u, v[u]);
-          }
-        }
-      }
-  }
+      });
 }
 
 // out = sum over splits, in split order
@@ -668,9 +716,10 @@ __device__ __forceinline__ unsigned long long order_key(double v) {
   return u >> 63 ? ~u : u | 1ull << 63;
 }
 
-// k-th largest (k >= 1) of `count` keys; on return `above` keys are larger than the result. All threads call it.
+// k-th largest (k >= 1) of `count` keys; on return `above` keys are larger than the result and `same` equal it. All
+// threads call it.
 template <typename K, class F>
-__device__ K radix_kth(int count, int k, F key, int* hist, int* pick, int& above) {
+__device__ K radix_kth(int count, int k, F key, int* hist, int* pick, int& above, int& same) {
   K found = 0, mask = 0;
   above = 0;
   for (int shift = (int)sizeof(K) * 8 - 8; shift >= 0; shift -= 8) {
@@ -698,6 +747,7 @@ __device__ K radix_kth(int count, int k, F key, int* hist, int* pick, int& above
         if (before < want && want <= before + c[u]) {
           pick[0] = 255 - (threadIdx.x * 4 + u);
           pick[1] = before;
+          pick[2] = c[u];
         }
         before += c[u];
       }
@@ -706,6 +756,7 @@ __device__ K radix_kth(int count, int k, F key, int* hist, int* pick, int& above
     found |= (K)pick[0] << shift;
     mask |= (K)255 << shift;
     above += pick[1];
+    same = pick[2];
   }
   __syncthreads();
   return found;
@@ -714,7 +765,7 @@ __device__ K radix_kth(int count, int k, F key, int* hist, int* pick, int& above
 template <typename T>
 __global__ __launch_bounds__(1024) void topk_kernel(TopArgs p) {
   extern __shared__ __align__(16) char head_smem[];
-  __shared__ int hist[256], pick[2], cnt, wcnt[16];
+  __shared__ int hist[256], pick[3], cnt, wcnt[16];
   __shared__ int sel[kTopMax + kSpare];
   __shared__ double zs[kTopMax + kSpare];
   __shared__ int cls[kTopMax + kSpare];
@@ -730,25 +781,31 @@ __global__ __launch_bounds__(1024) void topk_kernel(TopArgs p) {
       for (int g = t; g < p.groups; g += nt) gk[g] = order_key(st[(long long)g * p.n].x);
     __syncthreads();
     auto gkey = [&](int g) { return held ? gk[g] : order_key(st[(long long)g * p.n].x); };
-    int above;
-    tau = radix_kth<unsigned>(p.groups, p.kc, gkey, hist, pick, above);
+    int above, same;
+    tau = radix_kth<unsigned>(p.groups, p.kc, gkey, hist, pick, above, same);
     const int equal = p.kc - above;  // of the groups at tau, the first `equal`
     if (t == 0) cnt = 0;
     __syncthreads();
-    int seen = 0;
-    for (int g0 = 0; g0 < p.groups; g0 += nt) {
-      const unsigned key = g0 + t < p.groups ? gkey(g0 + t) : 0u;
-      const bool in = g0 + t < p.groups, eq = in && key == tau;
-      const unsigned long long m = __ballot(eq);
-      if (l == 0) wcnt[wave] = __popcll(m);
+    if (equal == same) {  // all of them
+      for (int g = t; g < p.groups; g += nt)
+        if (gkey(g) >= tau) sel[atomicAdd(&cnt, 1)] = g;
       __syncthreads();
-      int rank = seen + __popcll(m & ((1ull << l) - 1));
-      for (int w = 0; w < waves; ++w) {
-        if (w < wave) rank += wcnt[w];
-        seen += wcnt[w];
+    } else {
+      int seen = 0;
+      for (int g0 = 0; g0 < p.groups; g0 += nt) {
+        const unsigned key = g0 + t < p.groups ? gkey(g0 + t) : 0u;
+        const bool in = g0 + t < p.groups, eq = in && key == tau;
+        const unsigned long long m = __ballot(eq);
+        if (l == 0) wcnt[wave] = __popcll(m);
+        __syncthreads();
+        int rank = seen + __popcll(m & ((1ull << l) - 1));
+        for (int w = 0; w < waves; ++w) {
+          if (w < wave) rank += wcnt[w];
+          seen += wcnt[w];
+        }
+        if ((in && key > tau) || (eq && rank < equal)) sel[atomicAdd(&cnt, 1)] = g0 + t;
+        __syncthreads();
       }
-      if ((in && key > tau) || (eq && rank < equal)) sel[atomicAdd(&cnt, 1)] = g0 + t;
-      __syncthreads();
     }
     nsel = p.kc;
   }
@@ -767,27 +824,34 @@ __global__ __launch_bounds__(1024) void topk_kernel(TopArgs p) {
   }
   __syncthreads();
   const int total = cnt;
-  unsigned long long least = 0;
-  if (total > p.kc) {
-    int above;
-    least = radix_kth<unsigned long long>(total, p.kc, [&](int i) { return keys[i]; }, hist, pick, above);
-  }
   if (t == 0) cnt = 0;
   __syncthreads();
-  for (int i = t; i < total; i += nt)
-    if (keys[i] >= least) cls[atomicAdd(&cnt, 1)] = (int)~(unsigned)keys[i];
-  __syncthreads();
-  // exact scores of the kc candidates, two at a time per wave
-  const T *x = (const T*)p.x + row * p.xrs, *bias = (const T*)p.bias;
-  for (int c = wave * 2; c < p.kc; c += waves * 2) {
-    const int o = c + 1 < p.kc ? c + 1 : c;
-    const T* w[2] = {(const T*)p.w + (long long)cls[c] * p.wrs, (const T*)p.w + (long long)cls[o] * p.wrs};
-    double s[2];
-    row_dots<T, double, 2>(x, p.xcs, w, p.wcs, p.d, p.vec, s);
-    if (l == 0) {
-      zs[c] = (s[0] + (bias ? (double)Elem<T>::get(bias, cls[c]) : 0.0)) * p.inv_t;
-      if (o != c) zs[o] = (s[1] + (bias ? (double)Elem<T>::get(bias, cls[o]) : 0.0)) * p.inv_t;
+  if (total <= 1024) {  // (usual) a key is taken if fewer than kc are larger
+    for (int i = t; i < total; i += nt) {
+      const unsigned long long mine = keys[i];
+      int rank = 0;
+      for (int o = 0; o < total; ++o) rank += keys[o] > mine;
+      if (rank < p.kc) cls[rank] = (int)~(unsigned)mine;
     }
+  } else {
+    int above, same;
+    const unsigned long long least = radix_kth<unsigned long long>(total, p.kc, [&](int i) { return keys[i]; }, hist, pick, above, same);
+    for (int i = t; i < total; i += nt)
+      if (keys[i] >= least) cls[atomicAdd(&cnt, 1)] = (int)~(unsigned)keys[i];
+  }
+  __syncthreads();
+  // exact scores of the kc candidates, four at a time per wave
+  const T *x = (const T*)p.x + row * p.xrs, *bias = (const T*)p.bias;
+  for (int c = wave * 4; c < p.kc; c += waves * 4) {
+    const T* w[4];
+#pragma unroll
+    for (int u = 0; u < 4; ++u) w[u] = (const T*)p.w + (long long)cls[min(c + u, p.kc - 1)] * p.wrs;
+    double s[4];
+    row_dots<T, double, 4>(x, p.xcs, w, p.wcs, p.d, p.vec, s);
+    if (l == 0)
+#pragma unroll
+      for (int u = 0; u < 4; ++u)
+        if (c + u < p.kc) zs[c + u] = (s[u] + (bias ? (double)Elem<T>::get(bias, cls[c + u]) : 0.0)) * p.inv_t;
   }
   __syncthreads();
   for (int c = t; c < p.kc; c += nt) {
@@ -808,13 +872,16 @@ __global__ __launch_bounds__(1024) void topk_kernel(TopArgs p) {
 // ------------------------------------------------------------------ host side
 static long long up(long long v, long long m) { return (v + m - 1) / m * m; }
 
-inline int grid8(long long tiles) { return (int)((tiles + 7) / 8 * 8); }
+// blocks of a product: what runs at once (each block takes several tiles in turn), a multiple of the 8 XCDs
+inline int grid8(long long tiles, int per_cu) { return (int)std::min<long long>((tiles + 7) / 8 * 8, 256 * per_cu); }
 
 // Tiles, with the rate of a long product (32768 x 8192 x 4096 and its two transposes, random data):
 typedef TileCfg<256, 256, 2, 4, 32, 5> CfgBig;   // 1.39 PFLOP/s; all 160 KB of LDS, one block per CU
 typedef TileCfg<128, 256, 2, 4, 64, 3> CfgWide;  // 1.25 - 1.35
 typedef TileCfg<128, 128, 2, 2, 32, 4> CfgMid;   // 0.85 - 1.05 (bound by L2 reads), two blocks per CU
 typedef TileCfg<128, 32, 2, 1, 64, 4> CfgSlim;   // few rows: bound by reading w
+
+constexpr unsigned kLdsAll = 160 * 1024;
 
 enum { kBig = 0, kWide = 1, kMid = 2 };
 
@@ -839,7 +906,8 @@ static int pick_tile(long long m, long long n, long long k, int terms, int max_s
       if (t < cost) {
         cost = t;
         best = c;
-        if (splits) *splits = s;
+        // no empty run: as many as whole 64s of this length need
+        if (splits) *splits = ceil_div(k, up((k + s - 1) / s, 64));
       }
     }
   return best;
@@ -849,15 +917,20 @@ template <class C>
 void scores_launch(ScoreArgs p, int mode, hipStream_t s) {
   p.nm = ceil_div(p.V, C::kBM);
   p.nn = ceil_div(p.n, C::kBN);
-  const int g = grid8((long long)p.nm * p.nn);
-#define YTK_SC(M)                                                    \
-  {                                                                  \
-    scores_kernel<C, M><<<g, C::kThreads, C::kLds, s>>>(p);          \
-  }
-  if (mode == kStatsOnly) YTK_SC(kStatsOnly)
-  else if (mode == kExpHalf) YTK_SC(kExpHalf)
-  else if (mode == kExpFloat) YTK_SC(kExpFloat)
-  else YTK_SC(kScores)
+  const int g = grid8((long long)p.nm * p.nn, kLdsAll / C::kLds);
+#define YTK_SC(M, T) scores_kernel<C, M, T><<<g, C::kThreads, C::kLds, s>>>(p)
+  if (mode == kStatsOnly)
+    YTK_SC(kStatsOnly, 1);
+  else if (mode == kExpHalf)
+    YTK_SC(kExpHalf, 1);
+  else if (mode == kExpFloat)
+    YTK_SC(kExpFloat, 6);
+  else if (mode == kStatsFloat)
+    YTK_SC(kStatsFloat, 6);
+  else if (p.f32)
+    YTK_SC(kScores, 6);
+  else
+    YTK_SC(kScores, 1);
 #undef YTK_SC
   YTK_LAUNCH_CHECK();
 }
@@ -866,7 +939,7 @@ template <class C, int LA, int LB, typename T>
 void grad_launch(GradArgs p, hipStream_t s) {
   p.nm = ceil_div(p.M, C::kBM);
   p.nn = ceil_div(p.N, C::kBN);
-  grad_kernel<C, LA, LB, T><<<grid8((long long)p.nm * p.nn * p.splits), C::kThreads, C::kLds, s>>>(p);
+  grad_kernel<C, LA, LB, T><<<grid8((long long)p.nm * p.nn * p.splits, kLdsAll / C::kLds), C::kThreads, C::kLds, s>>>(p);
   YTK_LAUNCH_CHECK();
 }
 
@@ -1025,11 +1098,10 @@ static void scores(const HeadIn& h, const HeadPlan& p, const HeadOps& o, long lo
   a.w = o.w;
   a.x = rows_from(o.x, r0, rows);
   a.K = (int)p.kp;
-  a.terms = p.terms;
   a.V = (int)h.V;
   a.n = (int)rows;
   a.bias = bias;
-  a.bias_f32 = (int)h.f32;
+  a.f32 = (int)h.f32;
   a.inv_t = 1.0f / temp;
   a.stats = (float2*)(ws + p.o_stats);
   a.e = ws + p.o_e;
@@ -1061,10 +1133,14 @@ static void targets(const TargetArgs& t, hipStream_t s) {
   YTK_LAUNCH_CHECK();
 }
 
-static void rows_pass(RowArgs a, hipStream_t s) {
+static void rows_pass(RowArgs a, bool base2, hipStream_t s) {
+  // 16 rows share the lines of the group statistics, unless that leaves CUs without a block
   a.rb = 1;
-  while (a.rb < 16 && a.rb < a.n) a.rb *= 2;
-  row_kernel<<<ceil_div(a.n, a.rb), 256, 0, s>>>(a);
+  while (a.rb < 16 && a.rb * 512 <= a.n) a.rb *= 2;
+  if (base2)
+    row_kernel<true><<<ceil_div(a.n, a.rb), 256, 0, s>>>(a);
+  else
+    row_kernel<false><<<ceil_div(a.n, a.rb), 256, 0, s>>>(a);
   YTK_LAUNCH_CHECK();
 }
 
@@ -1086,7 +1162,7 @@ extern "C" void ytk_head_loss(const uintptr_t* ptrs, const long long* lp, double
   for (long long r0 = 0; r0 < h.n; r0 += p.piece) {
     const long long rows = std::min(p.piece, h.n - r0);
     const bool first = r0 == 0, last = r0 + rows == h.n;
-    scores(h, p, o, r0, rows, bias, temp, ws, !p.grads ? kStatsOnly : h.f32 ? kExpFloat : kExpHalf, s);
+    scores(h, p, o, r0, rows, bias, temp, ws, h.f32 ? (p.grads ? kExpFloat : kStatsFloat) : p.grads ? kExpHalf : kStatsOnly, s);
     TargetArgs t = {};
     t.x = x + r0 * h.xrs * el;
     t.w = w;
@@ -1113,7 +1189,7 @@ extern "C" void ytk_head_loss(const uintptr_t* ptrs, const long long* lp, double
     r.coef = p.grads ? (float*)(ws + p.o_coef) : nullptr;
     r.q = p.grads ? (float*)(ws + p.o_q) : nullptr;
     r.norm = p.grads ? (float2*)(ws + p.o_norm) : nullptr;
-    rows_pass(r, s);
+    rows_pass(r, !h.f32, s);
     if (!p.grads) continue;
 
     const bool db = h.want_dw && h.has_bias;
@@ -1144,7 +1220,7 @@ extern "C" void ytk_head_loss(const uintptr_t* ptrs, const long long* lp, double
       g.a.ext = (int)(p.pack_w ? p.kp : h.d);
       g.b = D;
       g.ka = h.V, g.kb = p.ld;
-      g.K = (int)h.V, g.terms = p.terms, g.splits = p.splits_dx;
+      g.K = (int)h.V, g.splits = p.splits_dx;
       g.M = (int)h.d, g.N = (int)rows;
       g.out = (char*)ptrs[10] + r0 * h.d * el, g.ldo = h.d;
       g.acc = (float*)(ws + p.o_split);
@@ -1167,7 +1243,7 @@ extern "C" void ytk_head_loss(const uintptr_t* ptrs, const long long* lp, double
       g.b = D;
       g.b.ext = (int)p.ld;
       g.ka = g.kb = rows;
-      g.K = (int)rows, g.terms = p.terms, g.splits = p.splits_dw;
+      g.K = (int)rows, g.splits = p.splits_dw;
       g.M = (int)h.d, g.N = (int)h.V;
       g.out = (void*)ptrs[11], g.ldo = h.d;
       g.acc = (float*)(ws + (p.many ? p.o_dwacc : p.o_split));
@@ -1203,7 +1279,7 @@ extern "C" void ytk_head_topk(const uintptr_t* ptrs, const long long* lp, double
     r.stats = (const float2*)(ws + p.o_stats);
     r.groups = (int)p.groups, r.n = (int)rows, r.V = (int)h.V;
     r.lse = (float*)ptrs[6] + r0;
-    rows_pass(r, s);
+    rows_pass(r, false, s);
     TopArgs t = {};
     t.stats = r.stats;
     t.z = (const float*)(ws + p.o_e);

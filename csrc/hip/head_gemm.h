@@ -74,11 +74,13 @@ struct Side {
   unsigned rd[kL == kKC ? kBK / 16 : kFB];
   const char* base;
   long long rem;                // bytes to the operand's end
+  unsigned koff;                // KC: bytes along K
   long long step, plane;
 
   static __device__ __forceinline__ int swz(int row) { return ((row & 3) | (((row >> 3) & 1) << 2)) & (kUnits - 1); }
 
-  __device__ __forceinline__ void init(const Operand& o, int t0, long long K, int kt0, int wave, int frag0, unsigned lds) {
+  // lane constants
+  __device__ __forceinline__ void init(const Operand& o, int wave, int frag0, unsigned lds) {
     const int l = threadIdx.x & 63;
     if (kL == kKC) {
 #pragma unroll
@@ -86,9 +88,6 @@ struct Side {
         const int row = (i * kNW + wave) * kRpi + l / kCh;
         voff[i] = (unsigned)(row * o.pitch) + (((l & (kCh - 1)) ^ swc(row)) << 4);
       }
-      base = o.p + (long long)t0 * o.pitch + kt0 * (kBK * 2LL);
-      rem = (long long)(o.ext - t0 - 1) * o.pitch + (K - kt0 * (long long)kBK) * 2;
-      step = kBK * 2;
 #pragma unroll
       for (int s = 0; s < kBK / 16; ++s) {
         const int row = frag0 * 32 + (l & 31);
@@ -101,35 +100,53 @@ struct Side {
         const int row = byte / kRow, chunk = (byte % kRow) / 16;
         voff[i] = (unsigned)(row * o.pitch) + ((((chunk >> 2) ^ swz(row)) << 2 | (chunk & 3)) << 4);
       }
-      base = o.p + kt0 * (long long)kBK * o.pitch + t0 * 2LL;
-      rem = (K - kt0 * (long long)kBK - 1) * o.pitch + (long long)(o.ext - t0) * 2;
-      step = kBK * o.pitch;
       const int g = l >> 4, i16 = l & 15, row = (g >> 1) * 8 + (i16 >> 2);
 #pragma unroll
       for (int b = 0; b < kFB; ++b)
         rd[b] = lds + row * kRow + (((frag0 + b) ^ swz(row)) << 6) + (g & 1) * 32 + (i16 & 3) * 8;
     }
-    plane = o.plane;
     lds0 = lds + wave * 1024;
   }
+  // first row (or column) and K step of a tile
+  __device__ __forceinline__ void at(const Operand& o, int t0, long long K, int kt0) {
+    if (kL == kKC) {
+      base = o.p + (long long)t0 * o.pitch + kt0 * (kBK * 2LL);
+      rem = (long long)(o.ext - t0 - 1) * o.pitch + (K - kt0 * (long long)kBK) * 2;
+      step = kBK * 2;
+    } else {
+      base = o.p + kt0 * (long long)kBK * o.pitch + t0 * 2LL;
+      rem = (K - kt0 * (long long)kBK - 1) * o.pitch + (long long)(o.ext - t0) * 2;
+      step = kBK * o.pitch;
+    }
+    plane = o.plane;
+    koff = 0;
+  }
 
-  // Buffer descriptor and scalar offset of K step `kt` (relative to kt0), plane `pl`; no records where there is
-  // none. A KC tile spans less than 2^31 bytes (checked by the host), so K is the scalar offset;
-  // a KS operand may be longer than 2^32 bytes, so K moves the base.
+  // Buffer descriptor and scalar offset of the stage to issue. A KC tile spans less than 2^31 bytes (checked by
+  // the host), so K is the scalar offset; a KS operand may be longer than 2^32 bytes, so K moves the base.
   struct Src {
     i32x4 d;
     unsigned soff;
   };
-  __device__ __forceinline__ Src src(int kt, int pl, bool some) const {
-    const long long k = kL == kKC ? 0 : kt * step;
-    const unsigned long long a = (unsigned long long)(base + k + pl * plane);
-    const unsigned long long r = (unsigned long long)(rem - k);
+  // the next K step
+  __device__ __forceinline__ void advance() {
+    if (kL == kKC) {
+      koff += kBK * 2;
+    } else {
+      base += step;
+      rem -= step;
+    }
+  }
+  __device__ __forceinline__ Src src(unsigned pl, bool some) const {
+    const unsigned long long a = (unsigned long long)(base + (pl == 0 ? 0 : pl == 1 ? plane : 2 * plane));
+    const unsigned hi = (unsigned)((unsigned long long)rem >> 32), lo = (unsigned)rem;
     Src s;
     s.d[0] = __builtin_amdgcn_readfirstlane((int)(unsigned)a);
     s.d[1] = __builtin_amdgcn_readfirstlane((int)((a >> 32) & 0xffff));
-    s.d[2] = __builtin_amdgcn_readfirstlane(!some || (r >> 63) ? 0 : (r >> 31) ? 0x7fffffff : (int)(unsigned)r);
+    // past the last stage, and at or past the operand's end: no records, zeros
+    s.d[2] = __builtin_amdgcn_readfirstlane(!some || (int)hi < 0 ? 0 : hi || lo > 0x7fffffffu ? 0x7fffffff : (int)lo);
     s.d[3] = 0x00020000;
-    s.soff = kL == kKC ? __builtin_amdgcn_readfirstlane(kt * (kBK * 2)) : 0u;
+    s.soff = kL == kKC ? __builtin_amdgcn_readfirstlane(koff) : 0u;
     return s;
   }
   // this wave's i-th piece of the stage at LDS offset `so`
@@ -159,12 +176,15 @@ struct TileCfg {
   static constexpr unsigned kLds = S * kStageBytes;
 };
 
-// (ka, kb: extent of K in each operand's memory; a KC operand's is a multiple of 64)
-// acc += A[m0.., kt0*kBK ..] B[n0.., ...]^T over `nkt` K steps and `terms` plane pairs (1 or 6). Both operands have
-// K left at every step: (kt0 + nkt - 1) * kBK < min(ka, kb).
-template <class C, int kLA, int kLB>
-__device__ __forceinline__ void gemm_loop(const Operand& A, const Operand& B, int m0, int n0, long long ka, long long kb,
-                                          int kt0, int nkt, int terms, f32x16 (&acc)[C::kFM][C::kFN]) {
+// One block's tiles, one after the other: tile(j, m0, n0, kt0, nkt) tells its j-th (false: no more; nkt >= 1 steps
+// of kBK from step kt0), done(j, m0, n0, acc) takes the accumulators. The DMA runs S - 1 stages ahead across
+// the border of two tiles, so only the epilogue's own instructions stand between their products. (Its stores share the
+// counter of the DMA, which counts down in the order of issue.)
+// ka, kb: extent of K in each operand's memory, a multiple of 64 for a KC operand; both reach every step:
+// (kt0 + nkt - 1) * kBK < min(ka, kb). kTerms: plane pairs, 1 or 6.
+template <class C, int kLA, int kLB, int kTerms, class FTile, class FDone>
+__device__ __forceinline__ void gemm_tiles(const Operand& A, const Operand& B, long long ka, long long kb, FTile tile,
+                                           FDone done) {
   extern __shared__ __align__(1024) char head_smem[];
   typedef __attribute__((address_space(3))) char lc;
   const unsigned lds = (unsigned)(uintptr_t)(lc*)head_smem;
@@ -174,21 +194,39 @@ __device__ __forceinline__ void gemm_loop(const Operand& A, const Operand& B, in
   typedef Side<kLB, C::kBN, C::kNW, C::kFN, C::kBK> SideB;
   SideA a;
   SideB b;
-  a.init(A, m0, ka, kt0, wave, wm * C::kFM, lds);
-  b.init(B, n0, kb, kt0, wave, wn * C::kFN, lds + SideA::kBytes);
+  a.init(A, wave, wm * C::kFM, lds);
+  b.init(B, wave, wn * C::kFN, lds + SideA::kBytes);
   constexpr int kLoads = SideA::kLoads + SideB::kLoads;
-  const int iters = nkt * terms;
-  int ikt = 0, iterm = 0;  // next stage to issue
-  const unsigned ta = terms == 1 ? 0u : kTermA, tb = terms == 1 ? 0u : kTermB;
+  static_assert(kTerms == 1 || kTerms == 6, "");
+  // the DMA's place in the stream of stages
+  int ij = 0, ikt = 0, iterm = 0, inkt = 0;
+  bool some;
+  auto begin = [&]() {
+    int m0 = 0, n0 = 0, kt0 = 0;
+    some = tile(ij, m0, n0, kt0, inkt);
+    if (some) {
+      a.at(A, m0, ka, kt0);
+      b.at(B, n0, kb, kt0);
+    } else {
+      inkt = 1 << 30;
+    }
+    ikt = iterm = 0;
+  };
+  begin();
+  if (!some) return;
   typename SideA::Src da;
   typename SideB::Src db;
-  auto next = [&]() {
-    const bool some = ikt < nkt;
-    da = a.src(some ? ikt : 0, (ta >> (2 * iterm)) & 3, some);
-    db = b.src(some ? ikt : 0, (tb >> (2 * iterm)) & 3, some);
-    if (++iterm == terms) {
+  auto next = [&]() {  // (past the last stage: zeros that nothing reads, so that every step issues the same loads)
+    da = a.src(kTerms == 1 ? 0u : (kTermA >> (2 * iterm)) & 3, some);
+    db = b.src(kTerms == 1 ? 0u : (kTermB >> (2 * iterm)) & 3, some);
+    if (kTerms == 1 || ++iterm == kTerms) {
       iterm = 0;
-      ++ikt;
+      a.advance();
+      b.advance();
+      if (++ikt == inkt) {
+        ++ij;
+        begin();
+      }
     }
   };
   auto piece = [&](int i, unsigned so) {
@@ -199,8 +237,6 @@ __device__ __forceinline__ void gemm_loop(const Operand& A, const Operand& B, in
   };
   constexpr int S = C::kStages;
   static_assert(S >= 3, "");
-  // S - 1 stages under way; a stage past the last is filled with zeros that nothing reads, so that every step
-  // issues and waits for the same number of loads
 #pragma unroll
   for (int s = 0; s < S - 1; ++s) {
     next();
@@ -226,48 +262,54 @@ __device__ __forceinline__ void gemm_loop(const Operand& A, const Operand& B, in
   unsigned so = 0, fill = (S - 1) * C::kStageBytes;  // stage being read, stage being filled
 #pragma unroll
   for (int r = 0; r < kR; ++r) read(r, 0, 0, 0);
-  for (int it = 0; it < iters; ++it) {
-    next();
-    const unsigned after = so + C::kStageBytes == C::kLds ? 0u : so + C::kStageBytes;
+  int m0, n0, kt0, nkt;
+  for (int j = 0; tile(j, m0, n0, kt0, nkt); ++j) {
+    f32x16 acc[C::kFM][C::kFN] = {};
+    for (int left = nkt * kTerms; left > 0; --left) {
+      const unsigned after = so + C::kStageBytes == C::kLds ? 0u : so + C::kStageBytes;
 #pragma unroll
-    for (int q = 0; q < kQ; ++q) {
-      if (q == kQ - 1) {
-        // every read of this stage has returned and the next stage has landed: one barrier hands this buffer
-        // to the DMA of the next step, while the products of the last quarter, already in registers, follow
-        wait_lgkm();
-        wait_vm<kAhead>();
-        __builtin_amdgcn_s_barrier();
-      }
-#pragma unroll
-      for (int i = 0; i < C::kFM; ++i) {
-#pragma unroll
-        for (int j = 0; j < C::kFN; ++j)
-          acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(fa[q & 1][i], fb[q & 1][j], acc[i][j], 0, 0, 0);
-        if (i < kHalf) {
-          // (after the last step: from a stage whose data nothing uses)
-#pragma unroll
-          for (int r = i * kR / kHalf; r < (i + 1) * kR / kHalf; ++r)
-            read(r, (q + 1) & 1, (q + 1) % kQ, q == kQ - 1 ? after : so);
-        } else {
-          const int slot = q * (C::kFM - kHalf) + i - kHalf;
-#pragma unroll
-          for (int u = slot * kLoads / kSlots; u < (slot + 1) * kLoads / kSlots; ++u) piece(u, fill);
+      for (int q = 0; q < kQ; ++q) {
+        if (q == kQ - 1) {
+          // every read of this stage has returned and the next stage has landed: one barrier hands this buffer
+          // to the DMA of the next step, while the products of the last quarter, already in registers, follow
+          wait_lgkm();
+          wait_vm<kAhead>();
+          __builtin_amdgcn_s_barrier();
         }
-        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int i = 0; i < C::kFM; ++i) {
+#pragma unroll
+          for (int j = 0; j < C::kFN; ++j)
+            acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(fa[q & 1][i], fb[q & 1][j], acc[i][j], 0, 0, 0);
+          if (q == 0 && i == 0) next();  // scalar work, while the first products run
+          if (i < kHalf) {
+            // (the next step's are the next tile's after a tile's last step)
+#pragma unroll
+            for (int r = i * kR / kHalf; r < (i + 1) * kR / kHalf; ++r)
+              read(r, (q + 1) & 1, (q + 1) % kQ, q == kQ - 1 ? after : so);
+          } else {
+            const int slot = q * (C::kFM - kHalf) + i - kHalf;
+#pragma unroll
+            for (int u = slot * kLoads / kSlots; u < (slot + 1) * kLoads / kSlots; ++u) piece(u, fill);
+          }
+          __builtin_amdgcn_sched_barrier(0);
+        }
       }
+      so = after;
+      fill = fill + C::kStageBytes == C::kLds ? 0u : fill + C::kStageBytes;
     }
-    so = after;
-    fill = fill + C::kStageBytes == C::kLds ? 0u : fill + C::kStageBytes;
+    done(j, m0, n0, acc);
   }
   wait_vm<0>();  // no DMA outlives the block
 }
 
-// block -> tile: each XCD (blocks go to them round robin) works through a contiguous run of the tile
-// order, and the order walks 8 m tiles before the next n tile, so the 32 CUs behind one L2 share their panels.
-__device__ __forceinline__ bool tile_of(int nm, int nn, int& tm, int& tn) {
+// j-th tile of this block: each XCD (blocks go to them round robin) works through a contiguous run of the tile
+// order, its blocks side by side, and the order walks 8 m tiles before the next n tile, so the 32 CUs behind one
+// L2 share their panels. The grid is a multiple of 8.
+__device__ __forceinline__ bool tile_of(int j, int nm, int nn, int& tm, int& tn) {
   const int T = nm * nn, chunk = (T + 7) / 8;
-  const int id = (int)(blockIdx.x & 7) * chunk + (int)(blockIdx.x >> 3);
-  if ((int)(blockIdx.x >> 3) >= chunk || id >= T) return false;
+  const int at = (int)(blockIdx.x >> 3) + j * (int)(gridDim.x >> 3), id = (int)(blockIdx.x & 7) * chunk + at;
+  if (at >= chunk || id >= T) return false;
   const int gsz = 8 * nn, g = id / gsz, r = id % gsz, gm = nm - g * 8 < 8 ? nm - g * 8 : 8;
   tm = g * 8 + r % gm;
   tn = r / gm;
