@@ -273,19 +273,22 @@ __device__ __forceinline__ long long index_at(const void* p, int is64, long long
 }
 
 // 16 bytes of a row as fp32
-__device__ __forceinline__ void load16(const float* p, float (&v)[4]) {
-  const float4 a = *(const float4*)p;
-  v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w;
+__device__ __forceinline__ void unpack16(const uint4& u, float (&v)[4]) {
+  v[0] = __builtin_bit_cast(float, u.x), v[1] = __builtin_bit_cast(float, u.y);
+  v[2] = __builtin_bit_cast(float, u.z), v[3] = __builtin_bit_cast(float, u.w);
 }
-__device__ __forceinline__ void load16(const __bf16* p, float (&v)[8]) {
-  const bf16x8 a = *(const bf16x8*)p;
+__device__ __forceinline__ void unpack16(const uint4& u, float (&v)[8]) {
+  const unsigned w[4] = {u.x, u.y, u.z, u.w};
 #pragma unroll
-  for (int i = 0; i < 8; ++i) v[i] = (float)a[i];
+  for (int i = 0; i < 4; ++i) {
+    v[2 * i] = __builtin_bit_cast(float, w[i] << 16);
+    v[2 * i + 1] = __builtin_bit_cast(float, w[i] & 0xffff0000u);
+  }
 }
 
 // a wave's dot products of one x row with kW w rows, summed in A (fp32, or fp64 of exact or fp64 products).
 // `vec`: rows of whole, aligned 16-byte pieces; otherwise element by element with any stride.
-template <typename T, typename A, int kW>
+template <typename T, typename A, int kW, int kU>
 __device__ __forceinline__ void row_dots(const T* x, long long xcs, const T* const (&w)[kW], long long wcs, int d, bool vec, A (&s)[kW]) {
   const int l = threadIdx.x & 63;
 #pragma unroll
@@ -298,16 +301,28 @@ __device__ __forceinline__ void row_dots(const T* x, long long xcs, const T* con
       s = fma((A)a, (A)b, s);
   };
   if (vec) {
-#pragma unroll 2
-    for (int c = l * kE; c < d; c += 64 * kE) {
-      float a[kE], b[kW][kE];
-      load16(x + c, a);
+    for (int c0 = l * kE; c0 < d; c0 += 64 * kE * kU) {
+      uint4 a[kU], b[kU][kW];  // kU (1 + kW) loads under way; pieces past the end are read again from the start and dropped
 #pragma unroll
-      for (int i = 0; i < kW; ++i) load16(w[i] + c, b[i]);
+      for (int u = 0; u < kU; ++u) {
+        const int c = c0 + u * 64 * kE < d ? c0 + u * 64 * kE : 0;
+        a[u] = *(const uint4*)(x + c);
 #pragma unroll
-      for (int i = 0; i < kW; ++i)
+        for (int i = 0; i < kW; ++i) b[u][i] = *(const uint4*)(w[i] + c);
+      }
 #pragma unroll
-        for (int e = 0; e < kE; ++e) add(s[i], a[e], b[i][e]);
+      for (int u = 0; u < kU; ++u) {
+        if (c0 + u * 64 * kE >= d) break;
+        float f[kE];
+        unpack16(a[u], f);
+#pragma unroll
+        for (int i = 0; i < kW; ++i) {
+          float g[kE];
+          unpack16(b[u][i], g);
+#pragma unroll
+          for (int e = 0; e < kE; ++e) add(s[i], f[e], g[e]);
+        }
+      }
     }
   } else {  // in the same order, so that the result does not depend on the strides
     for (int c = l * kE; c < d; c += 64 * kE)
@@ -340,7 +355,7 @@ __global__ __launch_bounds__(256) void target_kernel(TargetArgs p) {
     w[i] = (const T*)p.w + (v[i] < 0 ? 0 : v[i]) * p.wrs;  // entries without a class read class 0
   }
   float s[kW];
-  row_dots<T, float, kW>((const T*)p.x + row * p.xrs, p.xcs, w, p.wcs, p.d, p.vec, s);
+  row_dots<T, float, kW, kW == 1 ? 4 : 2>((const T*)p.x + row * p.xrs, p.xcs, w, p.wcs, p.d, p.vec, s);
   if (l == 0) {
 #pragma unroll
     for (int i = 0; i < kW; ++i)
@@ -683,15 +698,18 @@ __global__ __launch_bounds__(256) void split_sum_kernel(const float* __restrict_
 
 // ------------------------------------------------------------------ top k
 // One block per row. Scores are in z [n][ld], group maxima in stats. With kc = k + kSpare candidates:
-//   1. the kc-th largest group maximum tau (radix select); the kc best of all scores lie in the kc groups with the
-//      largest maxima, ties to the lower group: each of them holds a score that beats everything outside
+//   1. a threshold tau that at least kc and (ties aside) few more group maxima reach, found bit by bit with the
+//      maxima in registers: every such group holds a score >= tau, so the kc best of all scores are
+//      among the scores >= tau, and those are in these groups. Where ties leave more groups, the first kc by
+//      (maximum, lower group) do: each of them holds a score that beats everything outside.
 //   2. the scores >= tau of those groups, as 64-bit keys (score order, then lower class)
 //   3. the kc largest keys
 //   4. their scores again as 64-bit sums, so that the order returned is that of the exact scores, and
 //      the k largest of them in order
-constexpr int kSpare = 8;
+constexpr int kSpare = 8, kSlack = 24;
 constexpr int kTopMax = 256;       // k at most
-constexpr int kTopKeys = 16384;    // group keys held in LDS; beyond, they are read again from memory
+constexpr int kTopHold = 8;        // group maxima per thread
+constexpr int kTopList = 2048;     // keys held in LDS; where more reach tau (ties), they are read again from memory
 
 struct TopArgs {
   const float2* stats;
@@ -762,106 +780,188 @@ __device__ K radix_kth(int count, int k, F key, int* hist, int* pick, int& above
   return found;
 }
 
+template <int N>
+struct DotTag {
+  static constexpr int kW = N;
+};
+
 template <typename T>
 __global__ __launch_bounds__(1024) void topk_kernel(TopArgs p) {
-  extern __shared__ __align__(16) char head_smem[];
-  __shared__ int hist[256], pick[3], cnt, wcnt[16];
-  __shared__ int sel[kTopMax + kSpare];
+  __shared__ unsigned long long keys[kTopList];
+  __shared__ int hist[256], pick[3], cnt, wcnt[2][8][16];
+  __shared__ int sel[kTopMax + kSpare + kSlack];
   __shared__ double zs[kTopMax + kSpare];
   __shared__ int cls[kTopMax + kSpare];
-  unsigned long long* keys = (unsigned long long*)head_smem;  // kc * kGroup
-  unsigned* gk = (unsigned*)head_smem;                        // groups; done with before the keys are written
   const int row = blockIdx.x, t = threadIdx.x, nt = blockDim.x, wave = t >> 6, waves = nt >> 6, l = t & 63;
-  const bool held = p.groups <= kTopKeys;
   const float2* st = p.stats + row;
+  const float* z = p.z + (long long)row * p.ld;
+  auto gkey = [&](int g) { return order_key(st[(long long)g * p.n].x); };
   int nsel = p.groups;
   unsigned tau = 0;
+  if (t == 0) cnt = 0;
+  const int enough = p.kc + min(kSlack, p.kc >> 2);
   if (p.groups > p.kc) {
-    if (held)
-      for (int g = t; g < p.groups; g += nt) gk[g] = order_key(st[(long long)g * p.n].x);
-    __syncthreads();
-    auto gkey = [&](int g) { return held ? gk[g] : order_key(st[(long long)g * p.n].x); };
-    int above, same;
-    tau = radix_kth<unsigned>(p.groups, p.kc, gkey, hist, pick, above, same);
-    const int equal = p.kc - above;  // of the groups at tau, the first `equal`
-    if (t == 0) cnt = 0;
-    __syncthreads();
-    if (equal == same) {  // all of them
-      for (int g = t; g < p.groups; g += nt)
-        if (gkey(g) >= tau) sel[atomicAdd(&cnt, 1)] = g;
+    if (p.groups <= nt * kTopHold) {
+      unsigned mine[kTopHold];
+#pragma unroll
+      for (int u = 0; u < kTopHold; ++u) mine[u] = u * nt + t < p.groups ? gkey(u * nt + t) : 0u;
+      const int live = (p.groups + nt - 1) / nt;
+      // bits that all maxima share
+      unsigned hi = 0, lo = ~0u;
+#pragma unroll
+      for (int u = 0; u < kTopHold; ++u)
+        if (u * nt + t < p.groups) hi = max(hi, mine[u]), lo = min(lo, mine[u]);
+#pragma unroll
+      for (int o = 32; o; o >>= 1) hi = max(hi, (unsigned)__shfl_xor(hi, o, 64)), lo = min(lo, (unsigned)__shfl_xor(lo, o, 64));
+      if (l == 0) wcnt[1][0][wave] = (int)hi, wcnt[1][1][wave] = (int)lo;
       __syncthreads();
-    } else {
+      hi = (unsigned)wcnt[1][0][l % waves], lo = (unsigned)wcnt[1][1][l % waves];
+#pragma unroll
+      for (int o = 8; o; o >>= 1) hi = max(hi, (unsigned)__shfl_xor(hi, o, 64)), lo = min(lo, (unsigned)__shfl_xor(lo, o, 64));
+      hi = __builtin_amdgcn_readfirstlane(hi), lo = __builtin_amdgcn_readfirstlane(lo);
+      int top = hi == lo ? 0 : 32 - __builtin_clz(hi ^ lo);  // bits that differ
+      tau = top == 32 ? 0 : lo >> top << top;
+      // three bits per step: the highest of the seven thresholds above tau there that enough maxima reach
+      for (int step = 0; top > 0 && nsel > enough; ++step) {
+        const int bit = max(top - 3, 0), buf = step & 1;  // (the other buffer is written before the next barrier)
+        int mineq = 0;                                    // lane q keeps the wave's count for threshold q
+#pragma unroll
+        for (int q = 1; q < 8; ++q) {
+          int c = 0;
+#pragma unroll
+          for (int u = 0; u < kTopHold; ++u)
+            if (u < live) c += __popcll(__ballot(mine[u] >= (tau | (unsigned)q << bit)));
+          if (l == q) mineq = c;
+        }
+        if (l < 8) wcnt[buf][l][wave] = mineq;
+        __syncthreads();
+        const int w = l & 7;
+        int n = (w < waves ? wcnt[buf][l >> 3][w] : 0) + (w + 8 < waves ? wcnt[buf][l >> 3][w + 8] : 0);
+#pragma unroll
+        for (int o = 4; o; o >>= 1) n += __shfl_xor(n, o, 64);
+        const unsigned long long ok = __ballot(n >= p.kc && l >= 8);
+        if (ok) {
+          const int best = (63 - __builtin_clzll(ok)) >> 3;
+          nsel = __builtin_amdgcn_readlane(n, best * 8);
+          tau |= (unsigned)best << bit;
+        }
+        top = bit;
+      }
+      __syncthreads();
+      if (nsel <= enough) {
+#pragma unroll
+        for (int u = 0; u < kTopHold; ++u)
+          if (u * nt + t < p.groups && mine[u] >= tau) sel[atomicAdd(&cnt, 1)] = u * nt + t;
+      }
+    }
+    if (nsel > enough) {  // ties at tau, or more groups than the registers hold
+      int above, same;
+      __syncthreads();
+      tau = radix_kth<unsigned>(p.groups, p.kc, gkey, hist, pick, above, same);
       int seen = 0;
       for (int g0 = 0; g0 < p.groups; g0 += nt) {
-        const unsigned key = g0 + t < p.groups ? gkey(g0 + t) : 0u;
-        const bool in = g0 + t < p.groups, eq = in && key == tau;
+        const bool in = g0 + t < p.groups;
+        const unsigned key = in ? gkey(g0 + t) : 0u;
+        const bool eq = in && key == tau;
         const unsigned long long m = __ballot(eq);
-        if (l == 0) wcnt[wave] = __popcll(m);
+        if (l == 0) wcnt[0][0][wave] = __popcll(m);
         __syncthreads();
         int rank = seen + __popcll(m & ((1ull << l) - 1));
         for (int w = 0; w < waves; ++w) {
-          if (w < wave) rank += wcnt[w];
-          seen += wcnt[w];
+          if (w < wave) rank += wcnt[0][0][w];
+          seen += wcnt[0][0][w];
         }
-        if ((in && key > tau) || (eq && rank < equal)) sel[atomicAdd(&cnt, 1)] = g0 + t;
+        if ((in && key > tau) || (eq && rank < p.kc - above)) sel[atomicAdd(&cnt, 1)] = g0 + t;
         __syncthreads();
       }
+      nsel = p.kc;
     }
-    nsel = p.kc;
   }
+  __syncthreads();
   if (t == 0) cnt = 0;
   __syncthreads();
-  const float* z = p.z + (long long)row * p.ld;
-  for (int s = wave; s < nsel; s += waves) {
-    const int v = (p.groups > p.kc ? sel[s] : s) * kGroup + l;
-    const unsigned o = v < p.V ? order_key(z[v]) : 0u;
-    const bool take = v < p.V && o >= tau;
-    const unsigned long long m = __ballot(take);
-    int base = 0;
-    if (l == 0) base = atomicAdd(&cnt, __popcll(m));
-    base = __builtin_amdgcn_readfirstlane(base);
-    if (take) keys[base + __popcll(m & ((1ull << l) - 1))] = (unsigned long long)o << 32 | (unsigned)~v;
+  // i-th score of the groups kept
+  auto at = [&](int i) { return (p.groups > p.kc ? sel[i >> 6] : i >> 6) * kGroup + (i & 63); };
+  auto skey = [&](int i) {
+    const int v = at(i);
+    return v < p.V ? (unsigned long long)order_key(z[v]) << 32 | (unsigned)~v : 0ull;
+  };
+  constexpr int kFly = 16;  // groups in flight per wave
+  for (int s0 = wave; s0 < nsel; s0 += waves * kFly) {
+    float zv[kFly];
+    int v[kFly];
+#pragma unroll
+    for (int u = 0; u < kFly; ++u) {
+      v[u] = s0 + u * waves < nsel ? at((s0 + u * waves) * kGroup + l) : p.V;
+      zv[u] = z[min(v[u], p.V - 1)];
+    }
+#pragma unroll
+    for (int u = 0; u < kFly; ++u) {
+      const unsigned o = order_key(zv[u]);
+      const bool take = v[u] < p.V && o >= tau;
+      const unsigned long long m = __ballot(take);
+      if (!m) continue;
+      int base = 0;
+      if (l == 0) base = atomicAdd(&cnt, __popcll(m));
+      base = __builtin_amdgcn_readfirstlane(base) + __popcll(m & ((1ull << l) - 1));
+      if (take && base < kTopList) keys[base] = (unsigned long long)o << 32 | (unsigned)~v[u];
+    }
   }
   __syncthreads();
   const int total = cnt;
+  __syncthreads();
   if (t == 0) cnt = 0;
   __syncthreads();
-  if (total <= 1024) {  // (usual) a key is taken if fewer than kc are larger
+  if (total <= 512) {  // (usual) a key is taken if fewer than kc are larger
     for (int i = t; i < total; i += nt) {
       const unsigned long long mine = keys[i];
       int rank = 0;
+#pragma unroll 4
       for (int o = 0; o < total; ++o) rank += keys[o] > mine;
       if (rank < p.kc) cls[rank] = (int)~(unsigned)mine;
     }
   } else {
+    const bool listed = total <= kTopList;
+    const int count = listed ? total : nsel * kGroup;
+    auto lkey = [&](int i) { return listed ? keys[i] : skey(i); };
     int above, same;
-    const unsigned long long least = radix_kth<unsigned long long>(total, p.kc, [&](int i) { return keys[i]; }, hist, pick, above, same);
-    for (int i = t; i < total; i += nt)
-      if (keys[i] >= least) cls[atomicAdd(&cnt, 1)] = (int)~(unsigned)keys[i];
+    const unsigned long long least = radix_kth<unsigned long long>(count, p.kc, lkey, hist, pick, above, same);
+    for (int i = t; i < count; i += nt) {
+      const unsigned long long key = lkey(i);
+      if (key >= least) cls[atomicAdd(&cnt, 1)] = (int)~(unsigned)key;
+    }
   }
   __syncthreads();
-  // exact scores of the kc candidates, four at a time per wave
-  const T *x = (const T*)p.x + row * p.xrs, *bias = (const T*)p.bias;
-  for (int c = wave * 4; c < p.kc; c += waves * 4) {
-    const T* w[4];
+  // exact scores of the kc candidates, a few at a time per wave: two, further ahead, where the waves suffice
+  auto dots = [&](auto tag) {
+    constexpr int kW = decltype(tag)::kW;
+    const T *x = (const T*)p.x + row * p.xrs, *bias = (const T*)p.bias;
+    for (int c = wave * kW; c < p.kc; c += waves * kW) {
+      const T* w[kW];
 #pragma unroll
-    for (int u = 0; u < 4; ++u) w[u] = (const T*)p.w + (long long)cls[min(c + u, p.kc - 1)] * p.wrs;
-    double s[4];
-    row_dots<T, double, 4>(x, p.xcs, w, p.wcs, p.d, p.vec, s);
-    if (l == 0)
+      for (int u = 0; u < kW; ++u) w[u] = (const T*)p.w + (long long)cls[min(c + u, p.kc - 1)] * p.wrs;
+      double s[kW];
+      row_dots<T, double, kW, 8 / kW>(x, p.xcs, w, p.wcs, p.d, p.vec, s);
+      if (l == 0)
 #pragma unroll
-      for (int u = 0; u < 4; ++u)
-        if (c + u < p.kc) zs[c + u] = (s[u] + (bias ? (double)Elem<T>::get(bias, cls[c + u]) : 0.0)) * p.inv_t;
-  }
+        for (int u = 0; u < kW; ++u)
+          if (c + u < p.kc) {
+            zs[c + u] = (s[u] + (bias ? (double)Elem<T>::get(bias, cls[c + u]) : 0.0)) * p.inv_t;
+            keys[c + u] = order_key(zs[c + u]);
+          }
+    }
+  };
+  if (p.kc <= 2 * waves)
+    dots(DotTag<2>());
+  else
+    dots(DotTag<4>());
   __syncthreads();
   for (int c = t; c < p.kc; c += nt) {
-    const unsigned long long mine = order_key(zs[c]);
+    const unsigned long long mine = keys[c];
     const int v = cls[c];
     int rank = 0;
-    for (int o = 0; o < p.kc; ++o) {
-      const unsigned long long other = order_key(zs[o]);
-      rank += other > mine || (other == mine && cls[o] < v);
-    }
+#pragma unroll 4
+    for (int o = 0; o < p.kc; ++o) rank += keys[o] > mine || (keys[o] == mine && cls[o] < v);
     if (rank < p.k) {
       p.values[(long long)row * p.k + rank] = (float)zs[c];
       p.classes[(long long)row * p.k + rank] = v;
@@ -1292,13 +1392,11 @@ extern "C" void ytk_head_topk(const uintptr_t* ptrs, const long long* lp, double
     t.inv_t = 1.0 / temp_;
     t.values = (float*)ptrs[4] + r0 * h.k;
     t.classes = (long long*)ptrs[5] + r0 * h.k;
-    const size_t lds = std::max<size_t>(std::min<long long>(t.kc, p.groups) * kGroup * 8,
-                                        p.groups > t.kc && p.groups <= kTopKeys ? p.groups * 4 : 0);
     const int threads = rows < 256 ? 1024 : 256;  // fewer rows than CUs: more waves for each
     if (h.f32)
-      topk_kernel<float><<<(int)rows, threads, lds, s>>>(t);
+      topk_kernel<float><<<(int)rows, threads, 0, s>>>(t);
     else
-      topk_kernel<__bf16><<<(int)rows, threads, lds, s>>>(t);
+      topk_kernel<__bf16><<<(int)rows, threads, 0, s>>>(t);
     YTK_LAUNCH_CHECK();
   }
 }
