@@ -65,15 +65,22 @@ __global__ __launch_bounds__(256) void pack_kernel(const T* __restrict__ src, lo
                                                    int cols, __bf16* __restrict__ dst, long long ld, long long plane,
                                                    const float* __restrict__ coef) {
   __shared__ float tile[64][65];
+  __shared__ int live[64];
   const long long r0 = (long long)blockIdx.y * 64;
   const int c0 = blockIdx.x * 64, t = threadIdx.x;
   const bool by_row = cs == 1 || rs != 1;  // consecutive threads along the dimension that is dense in memory
-#pragma unroll 4
-  for (int i = t; i < 4096; i += 256) {
-    const int r = by_row ? i >> 6 : i & 63, c = by_row ? i & 63 : i >> 6;
-    float v = 0.0f;
-    if (r0 + r < rows && c0 + c < cols && (!coef || coef[r0 + r] != 0.0f)) v = Elem<T>::get(src, (r0 + r) * rs + (c0 + c) * cs);
-    tile[r][c] = v;
+  if (t < 64) live[t] = r0 + t < rows && (!coef || coef[r0 + t] != 0.0f);
+  __syncthreads();
+  T v[16];  // loads first, then LDS; places outside read element 0
+#pragma unroll
+  for (int u = 0; u < 16; ++u) {
+    const int i = u * 256 + t, r = by_row ? i >> 6 : i & 63, c = by_row ? i & 63 : i >> 6;
+    v[u] = src[r0 + r < rows && c0 + c < cols ? (r0 + r) * rs + (c0 + c) * cs : 0];
+  }
+#pragma unroll
+  for (int u = 0; u < 16; ++u) {
+    const int i = u * 256 + t, r = by_row ? i >> 6 : i & 63, c = by_row ? i & 63 : i >> 6;
+    tile[r][c] = live[r] && c0 + c < cols ? (float)v[u] : 0.0f;
   }
   __syncthreads();
   for (int i = t; i < 512; i += 256) {
@@ -491,9 +498,13 @@ struct DArgs {
   __bf16* d;            // fp32 inputs: D planes
   long long ld, plane;
   float* part;          // [row blocks][ld] bias gradient partials, or null
+  int rw;               // rows per wave
+  char* x;              // packed x of these rows, or null: rows without a gradient are cleared in it before they meet D
+  long long xpitch, xplane;
+  int planes;
 };
 
-constexpr int kDRows = 64;    // rows per block
+constexpr int kDRows = 16;    // rows per wave at most, four waves per block
 constexpr int kDCols = 512;   // columns per block: one wave = one row's 512 columns, 8 per lane
 
 template <bool kF32>
@@ -502,8 +513,8 @@ __global__ __launch_bounds__(256) void dscore_kernel(DArgs p) {
   constexpr int kB = kF32 ? 2 : 4;  // rows at once: their loads are in flight together
   const int wave = threadIdx.x >> 6, l = threadIdx.x & 63;
   const int c0 = blockIdx.x * kDCols, c = c0 + l * 8;
-  const long long r0 = (long long)blockIdx.y * kDRows + wave * (kDRows / 4);
-  const int rows = (int)min((long long)(kDRows / 4), p.n - r0);  // may be negative
+  const long long r0 = ((long long)blockIdx.y * 4 + wave) * p.rw;
+  const int rows = (int)min((long long)p.rw, p.n - r0);  // may be negative
   float db[8] = {};
   const bool live = c < p.ld;
   const long long cl = live ? c : 0;  // lanes past the end read column 0 and write nothing
@@ -559,6 +570,11 @@ __global__ __launch_bounds__(256) void dscore_kernel(DArgs p) {
       } else {
 #pragma unroll
         for (int j = 0; j < 8; ++j) d[b][j] = 0.0f;
+        // 0 * x must be 0 whatever this x holds
+        if (blockIdx.x == 0 && p.x)
+          for (int q = 0; q < p.planes; ++q)
+            for (long long u = l * 16; u < p.xpitch; u += 1024)
+              *(uint4*)(p.x + q * p.xplane + i * p.xpitch + u) = make_uint4(0, 0, 0, 0);
       }
       if (live) {
 #pragma unroll
@@ -979,6 +995,7 @@ inline int grid8(long long tiles, int per_cu) { return (int)std::min<long long>(
 typedef TileCfg<256, 256, 2, 4, 32, 5> CfgBig;   // 1.39 PFLOP/s; all 160 KB of LDS, one block per CU
 typedef TileCfg<128, 256, 2, 4, 64, 3> CfgWide;  // 1.25 - 1.35
 typedef TileCfg<128, 128, 2, 2, 32, 4> CfgMid;   // 0.85 - 1.05 (bound by L2 reads), two blocks per CU
+typedef TileCfg<128, 128, 2, 2, 32, 10> CfgDeep; // the same tile where one round of blocks does: nine stages under way
 typedef TileCfg<128, 32, 2, 1, 64, 4> CfgSlim;   // few rows: bound by reading w
 
 constexpr unsigned kLdsAll = 160 * 1024;
@@ -995,6 +1012,11 @@ static double tile_cost(int cfg, long long m, long long n, long long k, int term
   const long long rounds = (blocks + 256 * per_cu - 1) / (256 * per_cu);
   const double one = (double)bm * bn * (double)up((k + splits - 1) / splits, 64) * terms / rate * std::min<long long>(per_cu, (blocks + 255) / 256);
   return rounds * (one + 1e7) + (splits > 1 ? 5e6 + (double)m * n * splits * 5.0 : 0.0);
+}
+
+// one round of Mid tiles: a block alone on its CU, so the latency of its K steps counts
+static bool use_deep(long long m, long long n, int splits) {
+  return (long long)ceil_div(m, CfgMid::kBM) * ceil_div(n, CfgMid::kBN) * splits <= 256;
 }
 
 static int pick_tile(long long m, long long n, long long k, int terms, int max_splits, int* splits) {
@@ -1069,7 +1091,7 @@ struct HeadPlan {
   int planes, terms;
   long long kp, ld, groups, piece;
   bool pack_x, pack_w, grads;
-  int splits_dx, splits_dw, tile_dx, tile_dw;
+  int splits_dx, splits_dw, tile_dx, tile_dw, rw;
   bool many;  // more than one piece of rows
   long long o_x, o_w, o_xg, o_e, o_d, o_stats, o_zt, o_q, o_coef, o_norm, o_part, o_dbacc, o_dwacc, o_split, bytes;
 };
@@ -1101,7 +1123,7 @@ static HeadPlan head_plan(const HeadIn& h, bool topk) {
   };
   p.o_x = take(p.pack_x, h.n * p.kp * 2 * p.planes);
   p.o_w = take(p.pack_w, h.V * p.kp * 2 * p.planes);
-  p.o_xg = take(h.want_dw, p.piece * p.kp * 2 * p.planes);
+  p.o_xg = take(h.want_dw && !p.pack_x, p.piece * p.kp * 2);
   p.o_e = take(p.grads || topk, p.piece * p.ld * (h.f32 || topk ? 4 : 2));
   p.o_d = take(p.grads && h.f32, p.piece * p.ld * 6);
   p.o_stats = take(true, p.groups * p.piece * 8);
@@ -1110,7 +1132,10 @@ static HeadPlan head_plan(const HeadIn& h, bool topk) {
   p.o_coef = take(p.grads, p.piece * 4);
   p.o_norm = take(p.grads, p.piece * 8);
   const bool db = h.want_dw && h.has_bias;
-  p.o_part = take(db, ceil_div(p.piece, kDRows) * p.ld * 4);
+  // rows per wave of the D pass: fewer where there would be fewer than about 2048 blocks
+  p.rw = kDRows;
+  while (p.rw > 1 && ceil_div(p.piece, 4 * p.rw) * ceil_div(p.ld, kDCols) < 2048) p.rw /= 2;
+  p.o_part = take(db, ceil_div(p.piece, 4 * p.rw) * p.ld * 4);
   p.o_dbacc = take(db, h.V * 4);
   p.o_dwacc = take(h.want_dw && p.many, h.V * h.d * 4);
   p.o_split = take(p.splits_dx > 1 || p.splits_dw > 1,
@@ -1148,6 +1173,8 @@ static void grad_product(GradArgs g, int tile, hipStream_t s) {
     grad_launch<CfgBig, LA, LB, T>(g, s);
   else if (tile == kWide)
     grad_launch<CfgWide, LA, LB, T>(g, s);
+  else if (use_deep(g.M, g.N, g.splits))
+    grad_launch<CfgDeep, LA, LB, T>(g, s);
   else
     grad_launch<CfgMid, LA, LB, T>(g, s);
 }
@@ -1214,6 +1241,8 @@ static void scores(const HeadIn& h, const HeadPlan& p, const HeadOps& o, long lo
     scores_launch<CfgBig>(a, mode, s);
   else if (tile == kWide)
     scores_launch<CfgWide>(a, mode, s);
+  else if (use_deep(h.V, rows, 1))
+    scores_launch<CfgDeep>(a, mode, s);
   else
     scores_launch<CfgMid>(a, mode, s);
 }
@@ -1298,7 +1327,12 @@ extern "C" void ytk_head_loss(const uintptr_t* ptrs, const long long* lp, double
     d.idx = t.idx, d.idx64 = t.idx64, d.n = (int)rows, d.V = (int)h.V, d.k = (int)h.k;
     d.e = ws + p.o_e, d.d = (__bf16*)(ws + p.o_d), d.ld = p.ld, d.plane = rows * p.ld;
     d.part = db ? (float*)(ws + p.o_part) : nullptr;
-    const dim3 dg(ceil_div(p.ld, kDCols), ceil_div(rows, kDRows));
+    d.rw = p.rw;
+    if (h.want_dw && p.pack_x) {
+      d.x = ws + p.o_x + r0 * p.kp * 2;
+      d.xpitch = p.kp * 2, d.xplane = h.n * p.kp * 2, d.planes = p.planes;
+    }
+    const dim3 dg(ceil_div(p.ld, kDCols), ceil_div(rows, 4 * p.rw));
     if (h.f32)
       dscore_kernel<true><<<dg, 256, 0, s>>>(d);
     else
@@ -1334,12 +1368,14 @@ extern "C" void ytk_head_loss(const uintptr_t* ptrs, const long long* lp, double
       }
     }
     if (h.want_dw) {
-      if (h.f32)
-        pack_rows<float>(x + r0 * h.xrs * el, h.xrs, h.xcs, rows, h.d, ws + p.o_xg, p.kp, r.coef, s);
-      else
-        pack_rows<__bf16>(x + r0 * h.xrs * el, h.xrs, h.xcs, rows, h.d, ws + p.o_xg, p.kp, r.coef, s);
       GradArgs g = {};
-      g.a = {ws + p.o_xg, p.kp * 2, rows * p.kp * 2, (int)p.kp};
+      if (p.pack_x) {
+        g.a = rows_from(o.x, r0, rows);
+      } else {
+        pack_rows<__bf16>(x + r0 * h.xrs * el, h.xrs, h.xcs, rows, h.d, ws + p.o_xg, p.kp, r.coef, s);
+        g.a = {ws + p.o_xg, p.kp * 2, 0, 0};
+      }
+      g.a.ext = (int)p.kp;
       g.b = D;
       g.b.ext = (int)p.ld;
       g.ka = g.kb = rows;
