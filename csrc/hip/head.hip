@@ -109,7 +109,8 @@ __global__ __launch_bounds__(256) void pack_kernel(const T* __restrict__ src, lo
 // ------------------------------------------------------------------ scores
 struct ScoreArgs {
   Operand w, x;
-  int K;              // padded d
+  int K;              // d in whole 64s
+  int kw;             // extent of w's rows: K, or d where w is read in place (x is zero from d to K)
   int V, n;
   int nm, nn;         // tiles
   const void* bias;   // element type of the inputs
@@ -164,7 +165,7 @@ __global__ __launch_bounds__(C::kThreads) void scores_kernel(ScoreArgs p) {
   static_assert(C::kFM % 2 == 0, "a wave holds whole groups");
   const int wave = threadIdx.x >> 6, l = threadIdx.x & 63, hi = l >> 5;
   gemm_tiles<C, kKC, kKC, kTerms>(
-      p.w, p.x, p.K, p.K,
+      p.w, p.x, p.kw, p.K,
       [&](int j, int& m0, int& n0, int& kt0, int& nkt) {
         int tm, tn;
         if (!tile_of(j, p.nm, p.nn, tm, tn)) return false;
@@ -262,6 +263,165 @@ __global__ __launch_bounds__(C::kThreads) void scores_kernel(ScoreArgs p) {
           }
         }
       });
+}
+
+// ------------------------------------------------------------------ few fp32 rows
+// Up to 64 fp32 rows: reading w once is the cost, so w goes from memory to registers as it is (the bf16 planes
+// would be another 6 bytes written and read per element) and into the fp32 matrix products, 16 x 16 x 4: lane l holds
+// row l % 16 and k = l / 16. A lane loads 16 bytes, whose four elements are four products' k (the order of k is free as
+// long as both operands agree).
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef f32x4 f32x4u __attribute__((aligned(4)));  // rows of any float alignment
+
+struct FewArgs {
+  const float *w, *x, *bias;
+  long long wrs, xrs;
+  int V, n, d;
+  float inv_t;
+  float2* stats;
+  float* e;        // E or scores [n][ld], or null
+  long long ld;
+};
+
+// 4 floats from column c; zero past the end
+__device__ __forceinline__ f32x4 row4(const float* row, int c, int d) {
+  if (c + 4 <= d) return *(const f32x4u*)(row + c);
+  f32x4 v;
+#pragma unroll
+  for (int u = 0; u < 4; ++u) v[u] = c + u < d ? row[c + u] : 0.0f;
+  return v;
+}
+
+// A wave takes one group of 64 classes against kNT * 16 rows.
+template <int kNT, int kMode>
+__global__ __launch_bounds__(256) void scores_few_kernel(FewArgs p) {
+  const int l = threadIdx.x & 63, r16 = l & 15, g4 = l >> 4;
+  const int vg = (blockIdx.x * 4 + (threadIdx.x >> 6)) * kGroup;
+  if (vg >= p.V) return;
+  const float *w[4], *x[kNT];
+#pragma unroll
+  for (int t = 0; t < 4; ++t) w[t] = p.w + (long long)min(vg + t * 16 + r16, p.V - 1) * p.wrs;
+#pragma unroll
+  for (int t = 0; t < kNT; ++t) x[t] = p.x + (long long)min(t * 16 + r16, p.n - 1) * p.xrs;
+  f32x4 acc[4][kNT] = {};
+  constexpr int kU = kNT > 2 ? 2 : 4;  // steps under way
+  auto mma = [&](const f32x4 (&a)[4], const f32x4 (&b)[kNT]) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+#pragma unroll
+      for (int t = 0; t < 4; ++t)
+#pragma unroll
+        for (int i = 0; i < kNT; ++i) acc[t][i] = __builtin_amdgcn_mfma_f32_16x16x4f32(a[t][j], b[i][j], acc[t][i], 0, 0, 0);
+  };
+  int c = g4 * 4;
+  for (; c - g4 * 4 + 16 * kU <= p.d; c += 16 * kU) {
+    f32x4 a[kU][4], b[kU][kNT];
+#pragma unroll
+    for (int u = 0; u < kU; ++u) {
+#pragma unroll
+      for (int t = 0; t < 4; ++t) a[u][t] = *(const f32x4u*)(w[t] + c + 16 * u);
+#pragma unroll
+      for (int i = 0; i < kNT; ++i) b[u][i] = *(const f32x4u*)(x[i] + c + 16 * u);
+    }
+#pragma unroll
+    for (int u = 0; u < kU; ++u) mma(a[u], b[u]);
+  }
+  for (; c - g4 * 4 < p.d; c += 16) {
+    f32x4 a[4], b[kNT];
+#pragma unroll
+    for (int t = 0; t < 4; ++t) a[t] = row4(w[t], c, p.d);
+#pragma unroll
+    for (int i = 0; i < kNT; ++i) b[i] = row4(x[i], c, p.d);
+    mma(a, b);
+  }
+  // lane: row i = l % 16 (+ 16 per tile), classes vg + 16 t + 4 (l / 16) + r
+#pragma unroll
+  for (int i = 0; i < kNT; ++i) {
+    const int row = i * 16 + r16;
+    float z[4][4], m = -INFINITY;
+#pragma unroll
+    for (int t = 0; t < 4; ++t)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const int v = vg + t * 16 + g4 * 4 + r;
+        const float b = p.bias ? p.bias[min(v, p.V - 1)] : 0.0f;
+        z[t][r] = v < p.V ? (acc[t][i][r] + b) * p.inv_t : -INFINITY;
+        m = fmaxf(m, z[t][r]);
+      }
+    m = fmaxf(m, __shfl_xor(m, 16, 64));
+    m = fmaxf(m, __shfl_xor(m, 32, 64));
+    const float m0 = m == -INFINITY ? 0.0f : m;
+    float s = 0.0f;
+    float* o = p.e + (long long)row * p.ld + vg + g4 * 4;
+#pragma unroll
+    for (int t = 0; t < 4; ++t) {
+      if (kMode == kScores && row < p.n) *(float4*)(o + t * 16) = make_float4(z[t][0], z[t][1], z[t][2], z[t][3]);
+#pragma unroll
+      for (int r = 0; r < 4; ++r) s += z[t][r] = exp_of<true>(z[t][r] - m0);
+      if (kMode == kExpFloat && row < p.n) *(float4*)(o + t * 16) = make_float4(z[t][0], z[t][1], z[t][2], z[t][3]);
+    }
+    s += __shfl_xor(s, 16, 64);
+    s += __shfl_xor(s, 32, 64);
+    if (g4 == 0 && row < p.n) p.stats[(long long)(vg / kGroup) * p.n + row] = make_float2(m, s);
+  }
+}
+
+struct FewGradArgs {
+  const float *w, *D;   // D [n][ld], zero from V to ld
+  long long wrs, ld;
+  int V, n, d, per;     // classes per run, a multiple of 16
+  float* acc;           // [runs][n][d]
+};
+
+// dx = D w: a wave takes 64 columns of one run of classes; lane l holds columns 4 (l % 16) .. + 3 of w's row
+// 4 (l / 16) + j, so that one 16-byte load feeds four products (one per column of the four).
+template <int kNT>
+__global__ __launch_bounds__(256) void dx_few_kernel(FewGradArgs p) {
+  const int l = threadIdx.x & 63, r16 = l & 15, g4 = l >> 4;
+  const int d0 = (blockIdx.x * 4 + (threadIdx.x >> 6)) * 64;
+  if (d0 >= p.d) return;
+  const int v0 = blockIdx.y * p.per, v1 = min(v0 + p.per, p.V), col = d0 + 4 * r16;
+  const float* D[kNT];
+#pragma unroll
+  for (int i = 0; i < kNT; ++i) D[i] = p.D + (long long)min(i * 16 + r16, p.n - 1) * p.ld + g4 * 4;
+  f32x4 acc[4][kNT] = {};
+  constexpr int kU = 2;  // steps of 16 classes under way
+  for (int v = v0; v < v1; v += 16 * kU) {
+    f32x4 a[kU][4], b[kU][kNT];
+#pragma unroll
+    for (int u = 0; u < kU; ++u) {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const int c = v + u * 16 + g4 * 4 + j;
+        // a class past the run: zero, whatever the next row holds
+        a[u][j] = c < v1 ? row4(p.w + (long long)c * p.wrs, col, p.d) : f32x4{0, 0, 0, 0};
+      }
+#pragma unroll
+      for (int i = 0; i < kNT; ++i) b[u][i] = v + u * 16 < p.ld ? *(const f32x4*)(D[i] + v + u * 16) : f32x4{0, 0, 0, 0};
+    }
+#pragma unroll
+    for (int u = 0; u < kU; ++u)
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+#pragma unroll
+          for (int i = 0; i < kNT; ++i) acc[e][i] = __builtin_amdgcn_mfma_f32_16x16x4f32(a[u][j][e], b[u][i][j], acc[e][i], 0, 0, 0);
+  }
+  // product e's row m is column d0 + 4 m + e: lane holds m = 4 (l / 16) + r, so four e make four columns in a row
+#pragma unroll
+  for (int i = 0; i < kNT; ++i) {
+    const int row = i * 16 + r16;
+    if (row >= p.n) continue;
+    float* o = p.acc + ((long long)blockIdx.y * p.n + row) * p.d;
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      const int c = d0 + 16 * g4 + 4 * r;
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        if (c + e < p.d) o[c + e] = acc[e][i][r];
+    }
+  }
 }
 
 // ------------------------------------------------------------------ targets
@@ -499,6 +659,7 @@ struct DArgs {
   long long ld, plane;
   float* part;          // [row blocks][ld] bias gradient partials, or null
   int rw;               // rows per wave
+  int keep32;           // fp32 inputs: D also in fp32, in place of E
   char* x;              // packed x of these rows, or null: rows without a gradient are cleared in it before they meet D
   long long xpitch, xplane;
   int planes;
@@ -587,6 +748,12 @@ __global__ __launch_bounds__(256) void dscore_kernel(DArgs p) {
             split3(d[b][j], x, y, z);
             h[j] = x, mi[j] = y, lo[j] = z;
           }
+          if (p.keep32) {
+            float4* e = (float4*)((float*)p.e + i * p.ld + c);
+            e[0] = make_float4(d[b][0], d[b][1], d[b][2], d[b][3]);
+            e[1] = make_float4(d[b][4], d[b][5], d[b][6], d[b][7]);
+          }
+          if (!p.d) continue;
           __bf16* o = p.d + i * p.ld + c;
           *(bf16x8*)o = h;
           *(bf16x8*)(o + p.plane) = mi;
@@ -1090,8 +1257,8 @@ static HeadIn head_in(const long long* lp) {
 struct HeadPlan {
   int planes, terms;
   long long kp, ld, groups, piece;
-  bool pack_x, pack_w, grads;
-  int splits_dx, splits_dw, tile_dx, tile_dw, rw;
+  bool pack_x, pack_w, grads, few;
+  int splits_dx, splits_dw, tile_dx, tile_dw, rw, few_per;
   bool many;  // more than one piece of rows
   long long o_x, o_w, o_xg, o_e, o_d, o_stats, o_zt, o_q, o_coef, o_norm, o_part, o_dbacc, o_dwacc, o_split, bytes;
 };
@@ -1104,8 +1271,10 @@ static HeadPlan head_plan(const HeadIn& h, bool topk) {
   p.ld = up(h.V, 64);
   p.groups = p.ld / kGroup;
   p.grads = h.want_dx || h.want_dw;
-  p.pack_x = h.f32 || !h.x_al;
-  p.pack_w = h.f32 || !h.w_al;
+  // few fp32 rows (with dense columns): w is read as it is; the planes of x serve dw alone
+  p.few = h.f32 && h.n <= 64 && h.xcs == 1 && h.wcs == 1;
+  p.pack_x = p.few ? h.want_dw && !topk : h.f32 || !h.x_al;
+  p.pack_w = !p.few && (h.f32 || !h.w_al);
   const long long per = topk ? p.ld * 4 : p.grads ? p.ld * (h.f32 ? 10 : 2) : p.groups * 8;
   // (at most 2M rows: the grids of the row passes count rows / 64 in 16 bits and rows * k in 31)
   p.piece = std::min(h.n, std::min(1LL << 21, std::max(256LL, h.piece_bytes / per / 256 * 256)));
@@ -1113,7 +1282,13 @@ static HeadPlan head_plan(const HeadIn& h, bool topk) {
   p.splits_dx = p.splits_dw = 1;
   // partial sums of at most a quarter of the pieces' bytes (64 runs at most); pieces of rows already sum into dw
   auto most = [&](long long rows) { return (int)std::max(1LL, std::min(64LL, h.piece_bytes / 4 / (rows * h.d * 4))); };
-  if (h.want_dx) p.tile_dx = pick_tile(h.d, p.piece, h.V, p.terms, most(p.piece), &p.splits_dx);
+  if (h.want_dx && p.few) {  // runs of classes: about 2048 waves, at least 64 classes each
+    const long long runs = std::max(1LL, std::min<long long>(2048 / ceil_div(h.d, 64), ceil_div(h.V, 64)));
+    p.few_per = (int)up((h.V + runs - 1) / runs, 16);
+    p.splits_dx = ceil_div(h.V, p.few_per);
+  } else if (h.want_dx) {
+    p.tile_dx = pick_tile(h.d, p.piece, h.V, p.terms, most(p.piece), &p.splits_dx);
+  }
   if (h.want_dw) p.tile_dw = pick_tile(h.d, h.V, p.piece, p.terms, p.many ? 1 : most(h.V), &p.splits_dw);
   long long o = 0;
   auto take = [&](bool want, long long bytes) {
@@ -1125,7 +1300,7 @@ static HeadPlan head_plan(const HeadIn& h, bool topk) {
   p.o_w = take(p.pack_w, h.V * p.kp * 2 * p.planes);
   p.o_xg = take(h.want_dw && !p.pack_x, p.piece * p.kp * 2);
   p.o_e = take(p.grads || topk, p.piece * p.ld * (h.f32 || topk ? 4 : 2));
-  p.o_d = take(p.grads && h.f32, p.piece * p.ld * 6);
+  p.o_d = take(h.f32 && (p.few ? h.want_dw : p.grads), p.piece * p.ld * 6);
   p.o_stats = take(true, p.groups * p.piece * 8);
   p.o_zt = take(!topk, p.piece * h.k * 4);
   p.o_q = take(p.grads, p.piece * h.k * 4);
@@ -1138,8 +1313,8 @@ static HeadPlan head_plan(const HeadIn& h, bool topk) {
   p.o_part = take(db, ceil_div(p.piece, 4 * p.rw) * p.ld * 4);
   p.o_dbacc = take(db, h.V * 4);
   p.o_dwacc = take(h.want_dw && p.many, h.V * h.d * 4);
-  p.o_split = take(p.splits_dx > 1 || p.splits_dw > 1,
-                   std::max(p.splits_dx > 1 ? p.splits_dx * p.piece * h.d : 0, p.splits_dw > 1 ? p.splits_dw * h.V * h.d : 0) * 4);
+  p.o_split = take(p.splits_dx > 1 || p.splits_dw > 1 || p.few,
+                   std::max(p.splits_dx > 1 || p.few ? p.splits_dx * p.piece * h.d : 0, p.splits_dw > 1 ? p.splits_dw * h.V * h.d : 0) * 4);
   p.bytes = o;
   return p;
 }
@@ -1219,12 +1394,60 @@ static Operand rows_from(Operand o, long long r0, long long rows) {
   return o;
 }
 
+template <int kNT>
+static void scores_few_n(const FewArgs& a, int mode, hipStream_t s) {
+  const int g = ceil_div(ceil_div(a.V, kGroup), 4);
+  if (mode == kStatsFloat)
+    scores_few_kernel<kNT, kStatsFloat><<<g, 256, 0, s>>>(a);
+  else if (mode == kExpFloat)
+    scores_few_kernel<kNT, kExpFloat><<<g, 256, 0, s>>>(a);
+  else
+    scores_few_kernel<kNT, kScores><<<g, 256, 0, s>>>(a);
+  YTK_LAUNCH_CHECK();
+}
+
+static void scores_few(const HeadIn& h, const HeadPlan& p, const void* x, const void* w, const void* bias, float temp, char* ws, int mode,
+                       hipStream_t s) {
+  FewArgs a = {};
+  a.w = (const float*)w, a.x = (const float*)x, a.bias = (const float*)bias;
+  a.wrs = h.wrs, a.xrs = h.xrs;
+  a.V = (int)h.V, a.n = (int)h.n, a.d = (int)h.d;
+  a.inv_t = 1.0f / temp;
+  a.stats = (float2*)(ws + p.o_stats);
+  a.e = (float*)(ws + p.o_e);
+  a.ld = p.ld;
+  if (h.n <= 16)
+    scores_few_n<1>(a, mode, s);
+  else if (h.n <= 32)
+    scores_few_n<2>(a, mode, s);
+  else
+    scores_few_n<4>(a, mode, s);
+}
+
+static void dx_few(const HeadIn& h, const HeadPlan& p, const void* w, char* ws, void* out, hipStream_t s) {
+  FewGradArgs a = {};
+  a.w = (const float*)w, a.D = (const float*)(ws + p.o_e);
+  a.wrs = h.wrs, a.ld = p.ld;
+  a.V = (int)h.V, a.n = (int)h.n, a.d = (int)h.d, a.per = p.few_per;
+  a.acc = p.splits_dx > 1 ? (float*)(ws + p.o_split) : (float*)out;
+  const dim3 g(ceil_div(ceil_div(h.d, 64), 4), p.splits_dx);
+  if (h.n <= 16)
+    dx_few_kernel<1><<<g, 256, 0, s>>>(a);
+  else if (h.n <= 32)
+    dx_few_kernel<2><<<g, 256, 0, s>>>(a);
+  else
+    dx_few_kernel<4><<<g, 256, 0, s>>>(a);
+  YTK_LAUNCH_CHECK();
+  if (p.splits_dx > 1) split_sum<float>(a.acc, p.splits_dx, h.n, h.d, out, s);
+}
+
 static void scores(const HeadIn& h, const HeadPlan& p, const HeadOps& o, long long r0, long long rows, const void* bias, float temp,
                    char* ws, int mode, hipStream_t s) {
   ScoreArgs a = {};
   a.w = o.w;
   a.x = rows_from(o.x, r0, rows);
   a.K = (int)p.kp;
+  a.kw = (int)(p.pack_w ? p.kp : h.d);
   a.V = (int)h.V;
   a.n = (int)rows;
   a.bias = bias;
@@ -1291,7 +1514,10 @@ extern "C" void ytk_head_loss(const uintptr_t* ptrs, const long long* lp, double
   for (long long r0 = 0; r0 < h.n; r0 += p.piece) {
     const long long rows = std::min(p.piece, h.n - r0);
     const bool first = r0 == 0, last = r0 + rows == h.n;
-    scores(h, p, o, r0, rows, bias, temp, ws, h.f32 ? (p.grads ? kExpFloat : kStatsFloat) : p.grads ? kExpHalf : kStatsOnly, s);
+    if (p.few)
+      scores_few(h, p, x, w, bias, temp, ws, p.grads ? kExpFloat : kStatsFloat, s);
+    else
+      scores(h, p, o, r0, rows, bias, temp, ws, h.f32 ? (p.grads ? kExpFloat : kStatsFloat) : p.grads ? kExpHalf : kStatsOnly, s);
     TargetArgs t = {};
     t.x = x + r0 * h.xrs * el;
     t.w = w;
@@ -1328,6 +1554,8 @@ extern "C" void ytk_head_loss(const uintptr_t* ptrs, const long long* lp, double
     d.e = ws + p.o_e, d.d = (__bf16*)(ws + p.o_d), d.ld = p.ld, d.plane = rows * p.ld;
     d.part = db ? (float*)(ws + p.o_part) : nullptr;
     d.rw = p.rw;
+    d.keep32 = p.few && h.want_dx;
+    if (p.few && !h.want_dw) d.d = nullptr;
     if (h.want_dw && p.pack_x) {
       d.x = ws + p.o_x + r0 * p.kp * 2;
       d.xpitch = p.kp * 2, d.xplane = h.n * p.kp * 2, d.planes = p.planes;
@@ -1348,7 +1576,9 @@ extern "C" void ytk_head_loss(const uintptr_t* ptrs, const long long* lp, double
     }
     // D as an operand: rows = score rows, K contiguous for dx, K strided for dw
     const Operand D = {h.f32 ? ws + p.o_d : ws + p.o_e, p.ld * 2, rows * p.ld * 2, (int)rows};
-    if (h.want_dx) {
+    if (h.want_dx && p.few) {
+      dx_few(h, p, w, ws, (void*)ptrs[10], s);
+    } else if (h.want_dx) {
       GradArgs g = {};
       g.a = o.w;
       g.a.ext = (int)(p.pack_w ? p.kp : h.d);
@@ -1410,7 +1640,10 @@ extern "C" void ytk_head_topk(const uintptr_t* ptrs, const long long* lp, double
   const HeadOps o = head_operands(h, p, x, w, ws, s);
   for (long long r0 = 0; r0 < h.n; r0 += p.piece) {
     const long long rows = std::min(p.piece, h.n - r0);
-    scores(h, p, o, r0, rows, bias, (float)temp_, ws, kScores, s);
+    if (p.few)
+      scores_few(h, p, x, w, bias, (float)temp_, ws, kScores, s);
+    else
+      scores(h, p, o, r0, rows, bias, (float)temp_, ws, kScores, s);
     RowArgs r = {};
     r.stats = (const float2*)(ws + p.o_stats);
     r.groups = (int)p.groups, r.n = (int)rows, r.V = (int)h.V;

@@ -355,9 +355,10 @@ def test_loss_pieces(cuda, dtype, monkeypatch):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("dtype,n,d,V", [(torch.bfloat16, 1100, 512, 16500), (torch.bfloat16, 40, 1024, 20011),
-                                         (torch.float32, 700, 640, 4100), (torch.bfloat16, 4097, 1160, 264)])
+                                         (torch.float32, 700, 640, 4100), (torch.bfloat16, 4097, 1160, 264), (torch.float32, 5, 1000, 20011),
+                                         (torch.float32, 50, 1031, 9000), (torch.float32, 20, 64, 40000), (torch.bfloat16, 300, 1000, 5003)])
 def test_loss_larger(cuda, dtype, n, d, V):
-    """Large and small tiles, K split into runs, every XCD's share of the tile order."""
+    """Large and small tiles, K split into runs, every XCD's share of the tile order, few fp32 rows, rows that end in a step."""
     x, w, y, b = make(n, d, V, dtype, cuda, bias=True)
     r = head.softmax_head_loss(x, w, y, bias=b)
     Ref(x, w, *label_targets(y), bias=b).check(r, db=True)

@@ -16,6 +16,10 @@ gradient D = p - q is rounded to bf16 once before the two gradient products. Eve
 current stream of x's device without a host synchronisation, in a workspace of its own per call (torch's
 allocator), so calls on several streams and captured graphs do not share memory. Results are
 bitwise reproducible.
+
+x of rows that take part, w and bias are finite; a class is switched off by a bias of -inf or the type's lowest value.
+(An infinity or NaN in a row of w reaches that class's scores and, where d is no multiple of 64, may make those of the
+class before it NaN.)
 """
 from __future__ import annotations
 
@@ -63,9 +67,9 @@ def _check(x, w, bias, temperature, **rows):
         raise ValueError("class head: tensors on the GPU or the CPU expected")
 
 
-def _aligned(t):
-    """Whether the products can read the rows in place: 16-byte pieces, whole steps of 64 columns."""
-    return int(t.dtype == torch.bfloat16 and t.stride(1) == 1 and t.shape[1] % 64 == 0 and t.stride(0) % 8 == 0
+def _aligned(t, cols):
+    """Whether the products can read the rows in place: 16-byte pieces, a multiple of ``cols`` columns."""
+    return int(t.dtype == torch.bfloat16 and t.stride(1) == 1 and t.shape[1] % cols == 0 and t.stride(0) % 8 == 0
                and t.stride(0) >= t.shape[1] and t.data_ptr() % 16 == 0 and t.stride(0) <= 1 << 21)
 
 
@@ -77,7 +81,7 @@ def _strided(t):
 def _params(x, w, k, idx64, ignore, base, mode, want_dx, want_dw, bias):
     return [x.shape[0], x.shape[1], w.shape[0], k, int(x.dtype == torch.float32), x.stride(0), x.stride(1), w.stride(0),
             w.stride(1), idx64, ignore, int(base), mode, int(want_dx), int(want_dw), int(bias is not None),
-            PIECE_BYTES, _aligned(x), _aligned(w)]
+            PIECE_BYTES, _aligned(x, 64), _aligned(w, 8)]
 
 
 def _on(dev):
