@@ -114,7 +114,6 @@ struct ScoreArgs {
   int V, n;
   int nm, nn;         // tiles
   const void* bias;   // element type of the inputs
-  int f32;            // inputs (and bias)
   float inv_t;
   float2* stats;      // [groups][n]: m, s
   void* e;            // E [n][ld] (fp16 or fp32) or null
@@ -160,11 +159,11 @@ enum { kStatsOnly = 0, kExpHalf = 1, kExpFloat = 2, kScores = 3, kStatsFloat = 4
 template <int kMode>
 constexpr bool kBase2 = kMode == kStatsOnly || kMode == kExpHalf;
 
-template <class C, int kMode, int kTerms>
+template <class C, int kMode>
 __global__ __launch_bounds__(C::kThreads) void scores_kernel(ScoreArgs p) {
   static_assert(C::kFM % 2 == 0, "a wave holds whole groups");
   const int wave = threadIdx.x >> 6, l = threadIdx.x & 63, hi = l >> 5;
-  gemm_tiles<C, kKC, kKC, kTerms>(
+  gemm_tiles<C, kKC, kKC>(
       p.w, p.x, p.kw, p.K,
       [&](int j, int& m0, int& n0, int& kt0, int& nkt) {
         int tm, tn;
@@ -185,7 +184,7 @@ __global__ __launch_bounds__(C::kThreads) void scores_kernel(ScoreArgs p) {
 #pragma unroll
               for (int r = 0; r < 16; ++r) {
                 const int v = min(vg + h * 32 + 8 * (r >> 2) + 4 * hi + (r & 3), p.V - 1);
-                b[h][r] = kTerms == 6 ? ((const float*)p.bias)[v] : (float)((const __bf16*)p.bias)[v];
+                b[h][r] = C::kPlanes == 3 ? ((const float*)p.bias)[v] : (float)((const __bf16*)p.bias)[v];
               }
 #pragma unroll
             for (int h = 0; h < 2; ++h)
@@ -266,12 +265,14 @@ __global__ __launch_bounds__(C::kThreads) void scores_kernel(ScoreArgs p) {
 }
 
 // ------------------------------------------------------------------ few fp32 rows
-// Up to 64 fp32 rows: reading w once is the cost, so w goes from memory to registers as it is (the bf16 planes
+// Up to 128 fp32 rows: reading w is the cost, so w goes from memory to registers as it is (the bf16 planes
 // would be another 6 bytes written and read per element) and into the fp32 matrix products, 16 x 16 x 4: lane l holds
 // row l % 16 and k = l / 16. A lane loads 16 bytes, whose four elements are four products' k (the order of k is free as
 // long as both operands agree).
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef f32x4 f32x4u __attribute__((aligned(4)));  // rows of any float alignment
+
+constexpr int kFewRows = 128;
 
 struct FewArgs {
   const float *w, *x, *bias;
@@ -292,17 +293,34 @@ __device__ __forceinline__ f32x4 row4(const float* row, int c, int d) {
   return v;
 }
 
-// A wave takes one group of 64 classes against kNT * 16 rows.
+// Sums over the block's four waves through LDS: wave w returns with the sums of row tile i = w (kNT of them take part).
+template <int kNT>
+__device__ __forceinline__ bool few_sum(f32x4 (&acc)[4][kNT], f32x4 (&out)[4]) {
+  __shared__ f32x4 red[4][4][kNT][64];
+  const int l = threadIdx.x & 63, wave = threadIdx.x >> 6;
+#pragma unroll
+  for (int t = 0; t < 4; ++t)
+#pragma unroll
+    for (int i = 0; i < kNT; ++i) red[wave][t][i][l] = acc[t][i];
+  __syncthreads();
+  if (wave >= kNT) return false;
+#pragma unroll
+  for (int t = 0; t < 4; ++t) out[t] = (red[0][t][wave][l] + red[1][t][wave][l]) + (red[2][t][wave][l] + red[3][t][wave][l]);
+  return true;
+}
+
+// A block takes one group of 64 classes against kNT * 16 rows (more rows are further blocks on the same classes), its
+// waves a quarter of the features each: 12 waves a CU at 50000 classes, where a group per wave left one per SIMD.
 template <int kNT, int kMode>
-__global__ __launch_bounds__(256) void scores_few_kernel(FewArgs p) {
-  const int l = threadIdx.x & 63, r16 = l & 15, g4 = l >> 4;
-  const int vg = (blockIdx.x * 4 + (threadIdx.x >> 6)) * kGroup;
-  if (vg >= p.V) return;
+__global__ __launch_bounds__(256, 2) void scores_few_kernel(FewArgs p) {
+  const int l = threadIdx.x & 63, wave = threadIdx.x >> 6, r16 = l & 15, g4 = l >> 4, i0 = blockIdx.y * kNT * 16;
+  const int vg = blockIdx.x * kGroup;
+  const int per = ((p.d + 63) / 64) * 16, d0 = wave * per, d1 = min(d0 + per, p.d);
   const float *w[4], *x[kNT];
 #pragma unroll
   for (int t = 0; t < 4; ++t) w[t] = p.w + (long long)min(vg + t * 16 + r16, p.V - 1) * p.wrs;
 #pragma unroll
-  for (int t = 0; t < kNT; ++t) x[t] = p.x + (long long)min(t * 16 + r16, p.n - 1) * p.xrs;
+  for (int t = 0; t < kNT; ++t) x[t] = p.x + (long long)min(i0 + t * 16 + r16, p.n - 1) * p.xrs;
   f32x4 acc[4][kNT] = {};
   constexpr int kU = kNT > 2 ? 2 : 4;  // steps under way
   auto mma = [&](const f32x4 (&a)[4], const f32x4 (&b)[kNT]) {
@@ -313,113 +331,177 @@ __global__ __launch_bounds__(256) void scores_few_kernel(FewArgs p) {
 #pragma unroll
         for (int i = 0; i < kNT; ++i) acc[t][i] = __builtin_amdgcn_mfma_f32_16x16x4f32(a[t][j], b[i][j], acc[t][i], 0, 0, 0);
   };
-  int c = g4 * 4;
-  for (; c - g4 * 4 + 16 * kU <= p.d; c += 16 * kU) {
+  int c = d0;
+  for (; c + 16 * kU <= d1; c += 16 * kU) {
     f32x4 a[kU][4], b[kU][kNT];
 #pragma unroll
     for (int u = 0; u < kU; ++u) {
 #pragma unroll
-      for (int t = 0; t < 4; ++t) a[u][t] = *(const f32x4u*)(w[t] + c + 16 * u);
+      for (int t = 0; t < 4; ++t) a[u][t] = *(const f32x4u*)(w[t] + c + g4 * 4 + 16 * u);
 #pragma unroll
-      for (int i = 0; i < kNT; ++i) b[u][i] = *(const f32x4u*)(x[i] + c + 16 * u);
+      for (int i = 0; i < kNT; ++i) b[u][i] = *(const f32x4u*)(x[i] + c + g4 * 4 + 16 * u);
     }
 #pragma unroll
     for (int u = 0; u < kU; ++u) mma(a[u], b[u]);
   }
-  for (; c - g4 * 4 < p.d; c += 16) {
+  for (; c < d1; c += 16) {
     f32x4 a[4], b[kNT];
 #pragma unroll
-    for (int t = 0; t < 4; ++t) a[t] = row4(w[t], c, p.d);
+    for (int t = 0; t < 4; ++t) a[t] = row4(w[t], c + g4 * 4, d1);
 #pragma unroll
-    for (int i = 0; i < kNT; ++i) b[i] = row4(x[i], c, p.d);
+    for (int i = 0; i < kNT; ++i) b[i] = row4(x[i], c + g4 * 4, d1);
     mma(a, b);
   }
-  // lane: row i = l % 16 (+ 16 per tile), classes vg + 16 t + 4 (l / 16) + r
+  f32x4 sum[4];
+  if (!few_sum<kNT>(acc, sum)) return;
+  // lane: row l % 16 of the wave's tile, classes vg + 16 t + 4 (l / 16) + r
+  const int row = i0 + wave * 16 + r16;
+  float z[4][4], m = -INFINITY;
 #pragma unroll
-  for (int i = 0; i < kNT; ++i) {
-    const int row = i * 16 + r16;
-    float z[4][4], m = -INFINITY;
+  for (int t = 0; t < 4; ++t)
 #pragma unroll
-    for (int t = 0; t < 4; ++t)
-#pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        const int v = vg + t * 16 + g4 * 4 + r;
-        const float b = p.bias ? p.bias[min(v, p.V - 1)] : 0.0f;
-        z[t][r] = v < p.V ? (acc[t][i][r] + b) * p.inv_t : -INFINITY;
-        m = fmaxf(m, z[t][r]);
-      }
-    m = fmaxf(m, __shfl_xor(m, 16, 64));
-    m = fmaxf(m, __shfl_xor(m, 32, 64));
-    const float m0 = m == -INFINITY ? 0.0f : m;
-    float s = 0.0f;
-    float* o = p.e + (long long)row * p.ld + vg + g4 * 4;
-#pragma unroll
-    for (int t = 0; t < 4; ++t) {
-      if (kMode == kScores && row < p.n) *(float4*)(o + t * 16) = make_float4(z[t][0], z[t][1], z[t][2], z[t][3]);
-#pragma unroll
-      for (int r = 0; r < 4; ++r) s += z[t][r] = exp_of<true>(z[t][r] - m0);
-      if (kMode == kExpFloat && row < p.n) *(float4*)(o + t * 16) = make_float4(z[t][0], z[t][1], z[t][2], z[t][3]);
+    for (int r = 0; r < 4; ++r) {
+      const int v = vg + t * 16 + g4 * 4 + r;
+      const float b = p.bias ? p.bias[min(v, p.V - 1)] : 0.0f;
+      z[t][r] = v < p.V ? (sum[t][r] + b) * p.inv_t : -INFINITY;
+      m = fmaxf(m, z[t][r]);
     }
-    s += __shfl_xor(s, 16, 64);
-    s += __shfl_xor(s, 32, 64);
-    if (g4 == 0 && row < p.n) p.stats[(long long)(vg / kGroup) * p.n + row] = make_float2(m, s);
+  m = fmaxf(m, __shfl_xor(m, 16, 64));
+  m = fmaxf(m, __shfl_xor(m, 32, 64));
+  const float m0 = m == -INFINITY ? 0.0f : m;
+  float s = 0.0f;
+  float* o = p.e + (long long)row * p.ld + vg + g4 * 4;
+#pragma unroll
+  for (int t = 0; t < 4; ++t) {
+    if (kMode == kScores && row < p.n) *(float4*)(o + t * 16) = make_float4(z[t][0], z[t][1], z[t][2], z[t][3]);
+#pragma unroll
+    for (int r = 0; r < 4; ++r) s += z[t][r] = exp_of<true>(z[t][r] - m0);
+    if (kMode == kExpFloat && row < p.n) *(float4*)(o + t * 16) = make_float4(z[t][0], z[t][1], z[t][2], z[t][3]);
   }
+  s += __shfl_xor(s, 16, 64);
+  s += __shfl_xor(s, 32, 64);
+  if (g4 == 0 && row < p.n) p.stats[(long long)(vg / kGroup) * p.n + row] = make_float2(m, s);
 }
 
 struct FewGradArgs {
   const float *w, *D;   // D [n][ld], zero from V to ld
   long long wrs, ld;
-  int V, n, d, per;     // classes per run, a multiple of 16
+  int V, n, d, per;     // classes per run, a multiple of 64: 16 per wave and step
   float* acc;           // [runs][n][d]
 };
 
-// dx = D w: a wave takes 64 columns of one run of classes; lane l holds columns 4 (l % 16) .. + 3 of w's row
-// 4 (l / 16) + j, so that one 16-byte load feeds four products (one per column of the four).
+// dx = D w: a block takes 64 columns of one run of classes, its waves every fourth 16 classes; lane l holds columns
+// 4 (l % 16) .. + 3 of w's row 4 (l / 16) + j, so that one 16-byte load feeds four products (one per column of the four).
 template <int kNT>
-__global__ __launch_bounds__(256) void dx_few_kernel(FewGradArgs p) {
-  const int l = threadIdx.x & 63, r16 = l & 15, g4 = l >> 4;
-  const int d0 = (blockIdx.x * 4 + (threadIdx.x >> 6)) * 64;
-  if (d0 >= p.d) return;
+__global__ __launch_bounds__(256, 2) void dx_few_kernel(FewGradArgs p) {
+  const int l = threadIdx.x & 63, wave = threadIdx.x >> 6, r16 = l & 15, g4 = l >> 4, i0 = blockIdx.z * kNT * 16;
+  const int d0 = blockIdx.x * 64;
   const int v0 = blockIdx.y * p.per, v1 = min(v0 + p.per, p.V), col = d0 + 4 * r16;
   const float* D[kNT];
 #pragma unroll
-  for (int i = 0; i < kNT; ++i) D[i] = p.D + (long long)min(i * 16 + r16, p.n - 1) * p.ld + g4 * 4;
+  for (int i = 0; i < kNT; ++i) D[i] = p.D + (long long)min(i0 + i * 16 + r16, p.n - 1) * p.ld + g4 * 4;
   f32x4 acc[4][kNT] = {};
-  constexpr int kU = 2;  // steps of 16 classes under way
-  for (int v = v0; v < v1; v += 16 * kU) {
-    f32x4 a[kU][4], b[kU][kNT];
+  auto mma = [&](const f32x4 (&a)[4], const f32x4 (&b)[kNT]) {
 #pragma unroll
-    for (int u = 0; u < kU; ++u) {
+    for (int j = 0; j < 4; ++j)
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const int c = v + u * 16 + g4 * 4 + j;
-        // a class past the run: zero, whatever the next row holds
-        a[u][j] = c < v1 ? row4(p.w + (long long)c * p.wrs, col, p.d) : f32x4{0, 0, 0, 0};
+      for (int e = 0; e < 4; ++e)
+#pragma unroll
+        for (int i = 0; i < kNT; ++i) acc[e][i] = __builtin_amdgcn_mfma_f32_16x16x4f32(a[j][e], b[i][j], acc[e][i], 0, 0, 0);
+  };
+  constexpr int kU = 2;  // steps under way
+  int v = v0 + wave * 16;
+  if (d0 + 64 <= p.d || (p.d & 3) == 0) {
+    // whole pieces: lanes past the last column read it again, and their results are not stored
+    const float* w = p.w + (long long)(g4 * 4) * p.wrs + min(col, p.d - 4);
+    for (; v + 64 * (kU - 1) + 16 <= v1; v += 64 * kU) {
+      f32x4 a[kU][4], b[kU][kNT];
+#pragma unroll
+      for (int u = 0; u < kU; ++u) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) a[u][j] = *(const f32x4u*)(w + (long long)(v + 64 * u + j) * p.wrs);
+#pragma unroll
+        for (int i = 0; i < kNT; ++i) b[u][i] = *(const f32x4*)(D[i] + v + 64 * u);
       }
 #pragma unroll
-      for (int i = 0; i < kNT; ++i) b[u][i] = v + u * 16 < p.ld ? *(const f32x4*)(D[i] + v + u * 16) : f32x4{0, 0, 0, 0};
+      for (int u = 0; u < kU; ++u) mma(a[u], b[u]);
+    }
+  }
+  for (; v < v1; v += 64) {
+    f32x4 a[4], b[kNT];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const int c = v + g4 * 4 + j;
+      // a class past the run: zero, whatever the next row holds
+      a[j] = c < v1 ? row4(p.w + (long long)c * p.wrs, col, p.d) : f32x4{0, 0, 0, 0};
     }
 #pragma unroll
-    for (int u = 0; u < kU; ++u)
-#pragma unroll
-      for (int j = 0; j < 4; ++j)
-#pragma unroll
-        for (int e = 0; e < 4; ++e)
-#pragma unroll
-          for (int i = 0; i < kNT; ++i) acc[e][i] = __builtin_amdgcn_mfma_f32_16x16x4f32(a[u][j][e], b[u][i][j], acc[e][i], 0, 0, 0);
+    for (int i = 0; i < kNT; ++i) b[i] = *(const f32x4*)(D[i] + v);
+    mma(a, b);
   }
+  f32x4 sum[4];
+  if (!few_sum<kNT>(acc, sum)) return;
   // product e's row m is column d0 + 4 m + e: lane holds m = 4 (l / 16) + r, so four e make four columns in a row
+  const int row = i0 + wave * 16 + r16;
+  if (row >= p.n) return;
+  float* o = p.acc + ((long long)blockIdx.y * p.n + row) * p.d;
 #pragma unroll
-  for (int i = 0; i < kNT; ++i) {
-    const int row = i * 16 + r16;
-    if (row >= p.n) continue;
-    float* o = p.acc + ((long long)blockIdx.y * p.n + row) * p.d;
+  for (int r = 0; r < 4; ++r) {
+    const int c = d0 + 16 * g4 + 4 * r;
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+      if (c + e < p.d) o[c + e] = sum[e][r];
+  }
+}
+
+struct FewOuterArgs {
+  const float *x, *D, *coef;  // D [n][ld]; rows of x without a gradient (coef 0) count as zero
+  long long xrs, ld;
+  int V, n, d, per;           // classes per block, a multiple of 64
+  float* dw;                  // [V][d]
+};
+
+// dw = D^T x of at most 16 kK rows: a wave keeps its 64 columns of x in registers and walks over classes, 16 at a time;
+// the block's waves are side by side, so that it writes 1 KB pieces of 16 rows (256-byte pieces: 3.0 TB/s of dw).
+template <int kK>
+__global__ __launch_bounds__(256) void dw_few_kernel(FewOuterArgs p) {
+  const int l = threadIdx.x & 63, wave = threadIdx.x >> 6, r16 = l & 15, g4 = l >> 4;
+  const int d0 = (blockIdx.x * 4 + wave) * 64, col = d0 + 4 * r16;
+  const int v0 = blockIdx.y * p.per, v1 = min(v0 + p.per, p.V), steps = (p.n + 3) / 4;
+  if (d0 >= p.d) return;
+  f32x4 a[4 * kK];
+  const float* D[4 * kK];
+#pragma unroll
+  for (int k = 0; k < 4 * kK; ++k) {
+    const int i = k * 4 + g4;
+    a[k] = i < p.n && p.coef[min(i, p.n - 1)] != 0.0f ? row4(p.x + (long long)i * p.xrs, col, p.d) : f32x4{0, 0, 0, 0};
+    D[k] = p.D + (long long)min(i, p.n - 1) * p.ld + r16;
+  }
+  const bool vec = (p.d & 3) == 0;
+  for (int v = v0; v < v1; v += 16) {
+    float b[4 * kK];
+#pragma unroll
+    for (int k = 0; k < 4 * kK; ++k)
+      if (k < steps) b[k] = D[k][v];  // (rows past n: the last one's, against zeros of x)
+    f32x4 acc[4] = {};
+#pragma unroll
+    for (int k = 0; k < 4 * kK; ++k)
+      if (k < steps)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) acc[e] = __builtin_amdgcn_mfma_f32_16x16x4f32(a[k][e], b[k], acc[e], 0, 0, 0);
+    // lane: class v + l % 16, columns d0 + 16 (l / 16) + 4 r + e
+    if (v + r16 >= v1) continue;
+    float* o = p.dw + (long long)(v + r16) * p.d;
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
       const int c = d0 + 16 * g4 + 4 * r;
+      if (vec && c + 4 <= p.d) {
+        *(float4*)(o + c) = make_float4(acc[0][r], acc[1][r], acc[2][r], acc[3][r]);
+      } else {
 #pragma unroll
-      for (int e = 0; e < 4; ++e)
-        if (c + e < p.d) o[c + e] = acc[e][i][r];
+        for (int e = 0; e < 4; ++e)
+          if (c + e < p.d) o[c + e] = acc[e][r];
+      }
     }
   }
 }
@@ -776,14 +858,22 @@ __global__ __launch_bounds__(256) void dscore_kernel(DArgs p) {
   }
 }
 
-// bias gradient: partials summed in block order; `acc` carries pieces of rows (first: overwritten)
+// bias gradient: 64 columns per block, the partials in 16 strips, each in order; `acc` carries pieces of rows (first:
+// overwritten)
 template <typename T>
-__global__ __launch_bounds__(256) void db_kernel(const float* __restrict__ part, int nb, long long ld, int V,
-                                                 float* __restrict__ acc, int first, T* __restrict__ out) {
-  const int v = blockIdx.x * 256 + threadIdx.x;
-  if (v >= V) return;
-  float s = first ? 0.0f : acc[v];
-  for (int b = 0; b < nb; ++b) s += part[b * ld + v];
+__global__ __launch_bounds__(1024) void db_kernel(const float* __restrict__ part, int nb, long long ld, int V,
+                                                  float* __restrict__ acc, int first, T* __restrict__ out) {
+  __shared__ float sh[16][64];
+  const int l = threadIdx.x & 63, strip = threadIdx.x >> 6, v = blockIdx.x * 64 + l;
+  float s = 0.0f;
+#pragma unroll 8
+  for (int b = strip; b < nb; b += 16) s += part[b * ld + v];  // (ld is a multiple of 64)
+  sh[strip][l] = s;
+  __syncthreads();
+  if (strip || v >= V) return;
+  s = first ? 0.0f : acc[v];
+#pragma unroll
+  for (int b = 0; b < 16; ++b) s += sh[b][l];
   if (out)
     Elem<T>::put(out, v, s);
   else
@@ -807,7 +897,7 @@ __global__ __launch_bounds__(C::kThreads) void grad_kernel(GradArgs p) {
   const int wave = threadIdx.x >> 6, l = threadIdx.x & 63, hi = l >> 5;
   // runs of whole 64s; the host leaves none of them empty
   const int per = (p.K + 64 * p.splits - 1) / (64 * p.splits) * 64;
-  gemm_tiles<C, kLA, kLB, sizeof(T) == 4 ? 6 : 1>(
+  gemm_tiles<C, kLA, kLB>(
       p.a, p.b, p.ka, p.kb,
       [&](int j, int& m0, int& n0, int& kt0, int& nkt) {
         int tm, tn;
@@ -1163,18 +1253,19 @@ typedef TileCfg<256, 256, 2, 4, 32, 5> CfgBig;   // 1.39 PFLOP/s; all 160 KB of 
 typedef TileCfg<128, 256, 2, 4, 64, 3> CfgWide;  // 1.25 - 1.35
 typedef TileCfg<128, 128, 2, 2, 32, 4> CfgMid;   // 0.85 - 1.05 (bound by L2 reads), two blocks per CU
 typedef TileCfg<128, 128, 2, 2, 32, 10> CfgDeep; // the same tile where one round of blocks does: nine stages under way
+typedef TileCfg<128, 128, 2, 4, 32, 3, 3> CfgF32; // three planes
 typedef TileCfg<128, 32, 2, 1, 64, 4> CfgSlim;   // few rows: bound by reading w
 
 constexpr unsigned kLdsAll = 160 * 1024;
 
-enum { kBig = 0, kWide = 1, kMid = 2 };
+enum { kBig = 0, kWide = 1, kMid = 2, kF32 = 3 };
 
 // Estimated time of an M x N x K product in units of one CU's multiply-adds: rounds of blocks over the 256 CUs,
 // each paying its tile's products at the tile's rate, and about 4 us (10^7 multiply-adds) to start and finish;
 // K cut into `splits` runs costs the partial sums' traffic.
 static double tile_cost(int cfg, long long m, long long n, long long k, int terms, int splits) {
-  const int bm = cfg == kBig ? 256 : 128, bn = cfg == kMid ? 128 : 256, per_cu = cfg == kMid ? 2 : 1;
-  const double rate = cfg == kBig ? 1.0 : cfg == kWide ? 0.92 : 0.7;
+  const int bm = cfg == kBig ? 256 : 128, bn = cfg >= kMid ? 128 : 256, per_cu = cfg == kMid ? 2 : 1;
+  const double rate = cfg == kMid ? 0.7 : cfg == kWide ? 0.92 : 1.0;
   const long long blocks = (long long)ceil_div(m, bm) * ceil_div(n, bn) * splits;
   const long long rounds = (blocks + 256 * per_cu - 1) / (256 * per_cu);
   const double one = (double)bm * bn * (double)up((k + splits - 1) / splits, 64) * terms / rate * std::min<long long>(per_cu, (blocks + 255) / 256);
@@ -1189,7 +1280,7 @@ static bool use_deep(long long m, long long n, int splits) {
 static int pick_tile(long long m, long long n, long long k, int terms, int max_splits, int* splits) {
   int best = kBig;
   double cost = 1e300;
-  for (int c = kBig; c <= kMid; ++c)
+  for (int c = terms == 1 ? kBig : kF32; c <= (terms == 1 ? kMid : kF32); ++c)
     for (int s = 1; s <= max_splits && (s == 1 || k / s >= 512 / terms); s = s < 4 ? s + 1 : s + s / 4) {
       const double t = tile_cost(c, m, n, k, terms, s);
       if (t < cost) {
@@ -1207,19 +1298,22 @@ void scores_launch(ScoreArgs p, int mode, hipStream_t s) {
   p.nm = ceil_div(p.V, C::kBM);
   p.nn = ceil_div(p.n, C::kBN);
   const int g = grid8((long long)p.nm * p.nn, kLdsAll / C::kLds);
-#define YTK_SC(M, T) scores_kernel<C, M, T><<<g, C::kThreads, C::kLds, s>>>(p)
-  if (mode == kStatsOnly)
-    YTK_SC(kStatsOnly, 1);
-  else if (mode == kExpHalf)
-    YTK_SC(kExpHalf, 1);
-  else if (mode == kExpFloat)
-    YTK_SC(kExpFloat, 6);
-  else if (mode == kStatsFloat)
-    YTK_SC(kStatsFloat, 6);
-  else if (p.f32)
-    YTK_SC(kScores, 6);
-  else
-    YTK_SC(kScores, 1);
+#define YTK_SC(M) scores_kernel<C, M><<<g, C::kThreads, C::kLds, s>>>(p)
+  if constexpr (C::kPlanes == 3) {
+    if (mode == kExpFloat)
+      YTK_SC(kExpFloat);
+    else if (mode == kStatsFloat)
+      YTK_SC(kStatsFloat);
+    else
+      YTK_SC(kScores);
+  } else {
+    if (mode == kStatsOnly)
+      YTK_SC(kStatsOnly);
+    else if (mode == kExpHalf)
+      YTK_SC(kExpHalf);
+    else
+      YTK_SC(kScores);
+  }
 #undef YTK_SC
   YTK_LAUNCH_CHECK();
 }
@@ -1257,7 +1351,7 @@ static HeadIn head_in(const long long* lp) {
 struct HeadPlan {
   int planes, terms;
   long long kp, ld, groups, piece;
-  bool pack_x, pack_w, grads, few;
+  bool pack_x, pack_w, grads, few, few_dw, planes_d;
   int splits_dx, splits_dw, tile_dx, tile_dw, rw, few_per;
   bool many;  // more than one piece of rows
   long long o_x, o_w, o_xg, o_e, o_d, o_stats, o_zt, o_q, o_coef, o_norm, o_part, o_dbacc, o_dwacc, o_split, bytes;
@@ -1271,9 +1365,11 @@ static HeadPlan head_plan(const HeadIn& h, bool topk) {
   p.ld = up(h.V, 64);
   p.groups = p.ld / kGroup;
   p.grads = h.want_dx || h.want_dw;
-  // few fp32 rows (with dense columns): w is read as it is; the planes of x serve dw alone
-  p.few = h.f32 && h.n <= 64 && h.xcs == 1 && h.wcs == 1;
-  p.pack_x = p.few ? h.want_dw && !topk : h.f32 || !h.x_al;
+  // few fp32 rows: w is read as it is; the planes of x serve dw alone
+  p.few = h.f32 && h.n <= kFewRows;
+  if (p.few && (h.xcs != 1 || h.wcs != 1)) throw std::invalid_argument("class head: few fp32 rows need dense columns");
+  p.few_dw = p.few && h.n <= 64;  // (more rows: the planes of x and D)
+  p.pack_x = p.few ? h.want_dw && !topk && !p.few_dw : h.f32 || !h.x_al;
   p.pack_w = !p.few && (h.f32 || !h.w_al);
   const long long per = topk ? p.ld * 4 : p.grads ? p.ld * (h.f32 ? 10 : 2) : p.groups * 8;
   // (at most 2M rows: the grids of the row passes count rows / 64 in 16 bits and rows * k in 31)
@@ -1282,9 +1378,9 @@ static HeadPlan head_plan(const HeadIn& h, bool topk) {
   p.splits_dx = p.splits_dw = 1;
   // partial sums of at most a quarter of the pieces' bytes (64 runs at most); pieces of rows already sum into dw
   auto most = [&](long long rows) { return (int)std::max(1LL, std::min(64LL, h.piece_bytes / 4 / (rows * h.d * 4))); };
-  if (h.want_dx && p.few) {  // runs of classes: about 2048 waves, at least 64 classes each
-    const long long runs = std::max(1LL, std::min<long long>(2048 / ceil_div(h.d, 64), ceil_div(h.V, 64)));
-    p.few_per = (int)up((h.V + runs - 1) / runs, 16);
+  if (h.want_dx && p.few) {  // runs of classes: about 1024 blocks, at least 128 classes each
+    const long long runs = std::max(1LL, std::min<long long>(1024 / (ceil_div(h.d, 64) * ceil_div(h.n, 64)), ceil_div(h.V, 128)));
+    p.few_per = (int)up((h.V + runs - 1) / runs, 64);
     p.splits_dx = ceil_div(h.V, p.few_per);
   } else if (h.want_dx) {
     p.tile_dx = pick_tile(h.d, p.piece, h.V, p.terms, most(p.piece), &p.splits_dx);
@@ -1300,7 +1396,8 @@ static HeadPlan head_plan(const HeadIn& h, bool topk) {
   p.o_w = take(p.pack_w, h.V * p.kp * 2 * p.planes);
   p.o_xg = take(h.want_dw && !p.pack_x, p.piece * p.kp * 2);
   p.o_e = take(p.grads || topk, p.piece * p.ld * (h.f32 || topk ? 4 : 2));
-  p.o_d = take(h.f32 && (p.few ? h.want_dw : p.grads), p.piece * p.ld * 6);
+  p.planes_d = p.grads && h.f32 && (!p.few || (h.want_dw && !p.few_dw));
+  p.o_d = take(p.planes_d, p.piece * p.ld * 6);
   p.o_stats = take(true, p.groups * p.piece * 8);
   p.o_zt = take(!topk, p.piece * h.k * 4);
   p.o_q = take(p.grads, p.piece * h.k * 4);
@@ -1344,14 +1441,18 @@ static void pack_rows(const void* src, long long rs, long long cs, long long row
 
 template <int LA, int LB, typename T>
 static void grad_product(GradArgs g, int tile, hipStream_t s) {
-  if (tile == kBig)
-    grad_launch<CfgBig, LA, LB, T>(g, s);
-  else if (tile == kWide)
-    grad_launch<CfgWide, LA, LB, T>(g, s);
-  else if (use_deep(g.M, g.N, g.splits))
-    grad_launch<CfgDeep, LA, LB, T>(g, s);
-  else
-    grad_launch<CfgMid, LA, LB, T>(g, s);
+  if constexpr (sizeof(T) == 4) {
+    grad_launch<CfgF32, LA, LB, T>(g, s);
+  } else {
+    if (tile == kBig)
+      grad_launch<CfgBig, LA, LB, T>(g, s);
+    else if (tile == kWide)
+      grad_launch<CfgWide, LA, LB, T>(g, s);
+    else if (use_deep(g.M, g.N, g.splits))
+      grad_launch<CfgDeep, LA, LB, T>(g, s);
+    else
+      grad_launch<CfgMid, LA, LB, T>(g, s);
+  }
 }
 
 template <typename T>
@@ -1396,7 +1497,7 @@ static Operand rows_from(Operand o, long long r0, long long rows) {
 
 template <int kNT>
 static void scores_few_n(const FewArgs& a, int mode, hipStream_t s) {
-  const int g = ceil_div(ceil_div(a.V, kGroup), 4);
+  const dim3 g(ceil_div(a.V, kGroup), ceil_div(a.n, kNT * 16));
   if (mode == kStatsFloat)
     scores_few_kernel<kNT, kStatsFloat><<<g, 256, 0, s>>>(a);
   else if (mode == kExpFloat)
@@ -1430,7 +1531,7 @@ static void dx_few(const HeadIn& h, const HeadPlan& p, const void* w, char* ws, 
   a.wrs = h.wrs, a.ld = p.ld;
   a.V = (int)h.V, a.n = (int)h.n, a.d = (int)h.d, a.per = p.few_per;
   a.acc = p.splits_dx > 1 ? (float*)(ws + p.o_split) : (float*)out;
-  const dim3 g(ceil_div(ceil_div(h.d, 64), 4), p.splits_dx);
+  const dim3 g(ceil_div(h.d, 64), p.splits_dx, h.n <= 64 ? 1 : ceil_div(h.n, 64));
   if (h.n <= 16)
     dx_few_kernel<1><<<g, 256, 0, s>>>(a);
   else if (h.n <= 32)
@@ -1439,6 +1540,25 @@ static void dx_few(const HeadIn& h, const HeadPlan& p, const void* w, char* ws, 
     dx_few_kernel<4><<<g, 256, 0, s>>>(a);
   YTK_LAUNCH_CHECK();
   if (p.splits_dx > 1) split_sum<float>(a.acc, p.splits_dx, h.n, h.d, out, s);
+}
+
+static void dw_few(const HeadIn& h, const HeadPlan& p, const void* x, char* ws, void* out, hipStream_t s) {
+  FewOuterArgs a = {};
+  a.x = (const float*)x, a.D = (const float*)(ws + p.o_e), a.coef = (const float*)(ws + p.o_coef);
+  a.xrs = h.xrs, a.ld = p.ld;
+  a.V = (int)h.V, a.n = (int)h.n, a.d = (int)h.d;
+  // about 4096 blocks, each with its x loaded once
+  const long long runs = std::max(1LL, std::min<long long>(4096 / ceil_div(h.d, 256), ceil_div(h.V, 64)));
+  a.per = (int)up((h.V + runs - 1) / runs, 64);
+  a.dw = (float*)out;
+  const dim3 g(ceil_div(h.d, 256), ceil_div(h.V, a.per));
+  if (h.n <= 16)
+    dw_few_kernel<1><<<g, 256, 0, s>>>(a);
+  else if (h.n <= 32)
+    dw_few_kernel<2><<<g, 256, 0, s>>>(a);
+  else
+    dw_few_kernel<4><<<g, 256, 0, s>>>(a);
+  YTK_LAUNCH_CHECK();
 }
 
 static void scores(const HeadIn& h, const HeadPlan& p, const HeadOps& o, long long r0, long long rows, const void* bias, float temp,
@@ -1451,14 +1571,15 @@ static void scores(const HeadIn& h, const HeadPlan& p, const HeadOps& o, long lo
   a.V = (int)h.V;
   a.n = (int)rows;
   a.bias = bias;
-  a.f32 = (int)h.f32;
   a.inv_t = 1.0f / temp;
   a.stats = (float2*)(ws + p.o_stats);
   a.e = ws + p.o_e;
   a.z = (float*)(ws + p.o_e);
   a.ld = p.ld;
   const int tile = pick_tile(h.V, rows, p.kp, p.terms, 1, nullptr);
-  if (rows <= 64)
+  if (h.f32)
+    scores_launch<CfgF32>(a, mode, s);
+  else if (rows <= 64)
     scores_launch<CfgSlim>(a, mode, s);
   else if (tile == kBig)
     scores_launch<CfgBig>(a, mode, s);
@@ -1554,8 +1675,8 @@ extern "C" void ytk_head_loss(const uintptr_t* ptrs, const long long* lp, double
     d.e = ws + p.o_e, d.d = (__bf16*)(ws + p.o_d), d.ld = p.ld, d.plane = rows * p.ld;
     d.part = db ? (float*)(ws + p.o_part) : nullptr;
     d.rw = p.rw;
-    d.keep32 = p.few && h.want_dx;
-    if (p.few && !h.want_dw) d.d = nullptr;
+    d.keep32 = p.few;
+    if (h.f32 && !p.planes_d) d.d = nullptr;
     if (h.want_dw && p.pack_x) {
       d.x = ws + p.o_x + r0 * p.kp * 2;
       d.xpitch = p.kp * 2, d.xplane = h.n * p.kp * 2, d.planes = p.planes;
@@ -1569,9 +1690,9 @@ extern "C" void ytk_head_loss(const uintptr_t* ptrs, const long long* lp, double
     if (db) {
       float* acc = (float*)(ws + p.o_dbacc);
       if (h.f32)
-        db_kernel<float><<<ceil_div(h.V, 256), 256, 0, s>>>(d.part, (int)dg.y, p.ld, (int)h.V, acc, first, last ? (float*)ptrs[12] : nullptr);
+        db_kernel<float><<<ceil_div(h.V, 64), 1024, 0, s>>>(d.part, (int)dg.y, p.ld, (int)h.V, acc, first, last ? (float*)ptrs[12] : nullptr);
       else
-        db_kernel<__bf16><<<ceil_div(h.V, 256), 256, 0, s>>>(d.part, (int)dg.y, p.ld, (int)h.V, acc, first, last ? (__bf16*)ptrs[12] : nullptr);
+        db_kernel<__bf16><<<ceil_div(h.V, 64), 1024, 0, s>>>(d.part, (int)dg.y, p.ld, (int)h.V, acc, first, last ? (__bf16*)ptrs[12] : nullptr);
       YTK_LAUNCH_CHECK();
     }
     // D as an operand: rows = score rows, K contiguous for dx, K strided for dw
@@ -1597,7 +1718,9 @@ extern "C" void ytk_head_loss(const uintptr_t* ptrs, const long long* lp, double
         if (g.splits > 1) split_sum<__bf16>(g.acc, g.splits, rows, h.d, g.out, s);
       }
     }
-    if (h.want_dw) {
+    if (h.want_dw && p.few_dw) {
+      dw_few(h, p, x, ws, (void*)ptrs[11], s);
+    } else if (h.want_dw) {
       GradArgs g = {};
       if (p.pack_x) {
         g.a = rows_from(o.x, r0, rows);

@@ -28,16 +28,10 @@ typedef int i32x4 __attribute__((ext_vector_type(4)));
 
 enum { kKC = 0, kKS = 1 };
 
-// fp32 operands are three bf16 planes (hi, mid, lo: 24 bits); a product takes the six plane pairs whose
-// weight is above 2^-24. Plane of A and B for term t, small terms first so that they are not lost.
-struct TermTable {
-  unsigned a, b;  // 2 bits per term
-};
-__host__ __device__ constexpr unsigned term_pack(int t0, int t1, int t2, int t3, int t4, int t5) {
-  return t0 | t1 << 2 | t2 << 4 | t3 << 6 | t4 << 8 | t5 << 10;
-}
-constexpr unsigned kTermA = term_pack(2, 0, 1, 1, 0, 0);
-constexpr unsigned kTermB = term_pack(0, 2, 1, 0, 1, 0);
+// fp32 operands are three bf16 planes (hi, mid, lo: 24 bits); a product takes the six plane pairs whose weight is
+// above 2^-24, small ones first so that they are not lost. A stage then holds all planes of its K step: each is read once
+// from memory and from LDS for the products it is part of.
+__device__ constexpr int kPairA[6] = {2, 0, 1, 1, 0, 0}, kPairB[6] = {0, 2, 1, 0, 1, 0};
 
 struct Operand {
   const char* p;    // plane 0
@@ -137,8 +131,8 @@ struct Side {
       rem -= step;
     }
   }
-  __device__ __forceinline__ Src src(unsigned pl, bool some) const {
-    const unsigned long long a = (unsigned long long)(base + (pl == 0 ? 0 : pl == 1 ? plane : 2 * plane));
+  __device__ __forceinline__ Src src(int pl, bool some) const {
+    const unsigned long long a = (unsigned long long)(base + pl * plane);
     const unsigned hi = (unsigned)((unsigned long long)rem >> 32), lo = (unsigned)rem;
     Src s;
     s.d[0] = __builtin_amdgcn_readfirstlane((int)(unsigned)a);
@@ -167,12 +161,12 @@ struct Side {
   }
 };
 
-template <int BM, int BN, int WM, int WN, int BK, int S>
+template <int BM, int BN, int WM, int WN, int BK, int S, int P = 1>
 struct TileCfg {
-  static constexpr int kBM = BM, kBN = BN, kWM = WM, kWN = WN, kBK = BK, kStages = S;
+  static constexpr int kPlanes = P, kBM = BM, kBN = BN, kWM = WM, kWN = WN, kBK = BK, kStages = S;
   static constexpr int kNW = WM * WN, kThreads = 64 * kNW;
   static constexpr int kFM = BM / WM / 32, kFN = BN / WN / 32;  // 32x32 blocks per wave
-  static constexpr unsigned kStageBytes = (BM + BN) * BK * 2;
+  static constexpr unsigned kStageBytes = (BM + BN) * BK * 2 * P;
   static constexpr unsigned kLds = S * kStageBytes;
 };
 
@@ -181,8 +175,8 @@ struct TileCfg {
 // the border of two tiles, so only the epilogue's own instructions stand between their products. (Its stores share the
 // counter of the DMA, which counts down in the order of issue.)
 // ka, kb: extent of K in each operand's memory, a multiple of 64 for a KC operand; both reach every step:
-// (kt0 + nkt - 1) * kBK < min(ka, kb). kTerms: plane pairs, 1 or 6.
-template <class C, int kLA, int kLB, int kTerms, class FTile, class FDone>
+// (kt0 + nkt - 1) * kBK < min(ka, kb).
+template <class C, int kLA, int kLB, class FTile, class FDone>
 __device__ __forceinline__ void gemm_tiles(const Operand& A, const Operand& B, long long ka, long long kb, FTile tile,
                                            FDone done) {
   extern __shared__ __align__(1024) char head_smem[];
@@ -195,11 +189,13 @@ __device__ __forceinline__ void gemm_tiles(const Operand& A, const Operand& B, l
   SideA a;
   SideB b;
   a.init(A, wave, wm * C::kFM, lds);
-  b.init(B, wave, wn * C::kFN, lds + SideA::kBytes);
-  constexpr int kLoads = SideA::kLoads + SideB::kLoads;
-  static_assert(kTerms == 1 || kTerms == 6, "");
+  constexpr int P = C::kPlanes, kTerms = P == 1 ? 1 : 6;
+  static_assert(P == 1 || P == 3, "");
+  b.init(B, wave, wn * C::kFN, lds + P * SideA::kBytes);
+  constexpr int kPlaneLoads = SideA::kLoads + SideB::kLoads, kLoads = P * kPlaneLoads;
+
   // the DMA's place in the stream of stages
-  int ij = 0, ikt = 0, iterm = 0, inkt = 0;
+  int ij = 0, ikt = 0, inkt = 0;
   bool some;
   auto begin = [&]() {
     int m0 = 0, n0 = 0, kt0 = 0;
@@ -210,30 +206,31 @@ __device__ __forceinline__ void gemm_tiles(const Operand& A, const Operand& B, l
     } else {
       inkt = 1 << 30;
     }
-    ikt = iterm = 0;
+    ikt = 0;
   };
   begin();
   if (!some) return;
-  typename SideA::Src da;
-  typename SideB::Src db;
+  typename SideA::Src da[P];
+  typename SideB::Src db[P];
   auto next = [&]() {  // (past the last stage: zeros that nothing reads, so that every step issues the same loads)
-    da = a.src(kTerms == 1 ? 0u : (kTermA >> (2 * iterm)) & 3, some);
-    db = b.src(kTerms == 1 ? 0u : (kTermB >> (2 * iterm)) & 3, some);
-    if (kTerms == 1 || ++iterm == kTerms) {
-      iterm = 0;
-      a.advance();
-      b.advance();
-      if (++ikt == inkt) {
-        ++ij;
-        begin();
-      }
+#pragma unroll
+    for (int p = 0; p < P; ++p) {
+      da[p] = a.src(p, some);
+      db[p] = b.src(p, some);
+    }
+    a.advance();
+    b.advance();
+    if (++ikt == inkt) {
+      ++ij;
+      begin();
     }
   };
   auto piece = [&](int i, unsigned so) {
-    if (i < SideA::kLoads)
-      a.issue(i, da, so);
+    const int p = i / kPlaneLoads, u = i % kPlaneLoads;
+    if (u < SideA::kLoads)
+      a.issue(u, da[p], so + p * SideA::kBytes);
     else
-      b.issue(i - SideA::kLoads, db, so);
+      b.issue(u - SideA::kLoads, db[p], so + p * SideB::kBytes);
   };
   constexpr int S = C::kStages;
   static_assert(S >= 3, "");
@@ -246,17 +243,18 @@ __device__ __forceinline__ void gemm_tiles(const Operand& A, const Operand& B, l
   wait_vm<(S - 2) * kLoads>();
   __builtin_amdgcn_s_barrier();
 
-  bf16x8 fa[2][C::kFM], fb[2][C::kFN];
-  auto read = [&](int r, int p, int q, unsigned so) {
-    if (r < C::kFN)
-      fb[p][r] = b.frag(r, q, so);
+  bf16x8 fa[2][P][C::kFM], fb[2][P][C::kFN];
+  auto read = [&](int r, int set, int q, unsigned so) {
+    const int p = r % P, f = r / P;
+    if (f < C::kFN)
+      fb[set][p][f] = b.frag(f, q, so + p * SideB::kBytes);
     else
-      fa[p][r - C::kFN] = a.frag(r - C::kFN, q, so);
+      fa[set][p][f - C::kFN] = a.frag(f - C::kFN, q, so + p * SideA::kBytes);
   };
   // kQ quarters per K step, each kFM rows of products. The next quarter's kR fragments are read during the first
   // half of a quarter (they have returned by its end), the DMA is issued in the second half: in one
   // burst, the loads stall every wave at the memory unit (1.20 -> 1.34 PFLOP/s at 32768 x 8192 x 4096).
-  constexpr int kQ = C::kBK / 16, kR = C::kFM + C::kFN, kHalf = C::kFM / 2, kSlots = kQ * (C::kFM - kHalf);
+  constexpr int kQ = C::kBK / 16, kR = P * (C::kFM + C::kFN), kHalf = C::kFM / 2, kSlots = kQ * (C::kFM - kHalf);
   // DMA instructions that may still be under way when the next stage has landed
   constexpr int kAhead = (S - 3) * kLoads + (kQ - 1) * (C::kFM - kHalf) * kLoads / kSlots;
   unsigned so = 0, fill = (S - 1) * C::kStageBytes;  // stage being read, stage being filled
@@ -265,7 +263,7 @@ __device__ __forceinline__ void gemm_tiles(const Operand& A, const Operand& B, l
   int m0, n0, kt0, nkt;
   for (int j = 0; tile(j, m0, n0, kt0, nkt); ++j) {
     f32x16 acc[C::kFM][C::kFN] = {};
-    for (int left = nkt * kTerms; left > 0; --left) {
+    for (int left = nkt; left > 0; --left) {
       const unsigned after = so + C::kStageBytes == C::kLds ? 0u : so + C::kStageBytes;
 #pragma unroll
       for (int q = 0; q < kQ; ++q) {
@@ -279,8 +277,11 @@ __device__ __forceinline__ void gemm_tiles(const Operand& A, const Operand& B, l
 #pragma unroll
         for (int i = 0; i < C::kFM; ++i) {
 #pragma unroll
-          for (int j = 0; j < C::kFN; ++j)
-            acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(fa[q & 1][i], fb[q & 1][j], acc[i][j], 0, 0, 0);
+          for (int t = 0; t < kTerms; ++t)
+#pragma unroll
+            for (int j = 0; j < C::kFN; ++j)
+              acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(fa[q & 1][P == 1 ? 0 : kPairA[t]][i],
+                                                                  fb[q & 1][P == 1 ? 0 : kPairB[t]][j], acc[i][j], 0, 0, 0);
           if (q == 0 && i == 0) next();  // scalar work, while the first products run
           if (i < kHalf) {
             // (the next step's are the next tile's after a tile's last step)

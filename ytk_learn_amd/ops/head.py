@@ -32,6 +32,7 @@ from ._ext import hip, ptr, stream
 
 # bytes of exponentials (or scores, head_topk) that live at a time; rows beyond are taken in further pieces
 PIECE_BYTES = 2 << 30
+FEW_ROWS = 128           # == kFewRows (head.hip)
 MAX_LIST = 256           # entries of a teacher's list, and k of head_topk
 MAX_DIM = 1 << 21         # classes, features
 _TYPES = (torch.float32, torch.bfloat16)
@@ -73,9 +74,16 @@ def _aligned(t, cols):
                and t.stride(0) >= t.shape[1] and t.data_ptr() % 16 == 0 and t.stride(0) <= 1 << 21)
 
 
-def _strided(t):
-    """Tensors that repeat memory or run backwards are copied; every other stride is read as it is."""
-    return t.contiguous() if (t.stride(0) <= 0 and t.shape[0] > 1) or (t.stride(1) <= 0 and t.shape[1] > 1) else t
+def _operands(x, w):
+    """Tensors that repeat memory or run backwards are copied, and those of few float32 rows whose columns are not dense;
+    every other stride is read as it is."""
+    few = x.dtype == torch.float32 and x.shape[0] <= FEW_ROWS
+
+    def one(t):
+        odd = (t.stride(0) <= 0 and t.shape[0] > 1) or (t.stride(1) <= 0 and t.shape[1] > 1)
+        return t.contiguous() if odd or (few and t.stride(1) != 1) else t
+
+    return one(x), one(w)
 
 
 def _params(x, w, k, idx64, ignore, base, mode, want_dx, want_dw, bias):
@@ -97,7 +105,7 @@ def _loss(x, w, idx, tl, tlse, bias, weight, temperature, ignore, base, mode, wa
         return HeadLoss(loss, lse, torch.zeros_like(x) if want_dx else None,
                         torch.zeros(w.shape, dtype=w.dtype, device=dev) if want_dw else None,
                         torch.zeros(V, dtype=w.dtype, device=dev) if want_dw and bias is not None else None)
-    x, w = _strided(x), _strided(w)
+    x, w = _operands(x, w)
     idx = idx.contiguous()
     bias, weight, tl, tlse = (None if t is None else t.contiguous() for t in (bias, weight, tl, tlse))
     dx = torch.empty(x.shape, dtype=x.dtype, device=dev) if want_dx else None
@@ -180,7 +188,7 @@ def head_topk(x: torch.Tensor, w: torch.Tensor, k: int, bias: Optional[torch.Ten
     lse = torch.empty(n, dtype=torch.float32, device=dev)
     if n == 0:
         return values, classes, lse
-    x, w = _strided(x), _strided(w)
+    x, w = _operands(x, w)
     bias = None if bias is None else bias.contiguous()
     lp = _params(x, w, k, 1, -1, False, 0, False, False, bias)
     h = hip()
