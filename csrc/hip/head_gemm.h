@@ -29,7 +29,7 @@ typedef int i32x4 __attribute__((ext_vector_type(4)));
 enum { kKC = 0, kKS = 1 };
 
 // fp32 operands are three bf16 planes (hi, mid, lo: 24 bits); a product takes the six plane pairs whose weight is
-// above 2^-24, small ones first so that they are not lost. A stage then holds all planes of its K step: each is read once
+// above 2^-24. A stage then holds all planes of its K step: each is read once
 // from memory and from LDS for the products it is part of.
 __device__ constexpr int kPairA[6] = {2, 0, 1, 1, 0, 0}, kPairB[6] = {0, 2, 1, 0, 1, 0};
 
@@ -262,7 +262,9 @@ __device__ __forceinline__ void gemm_tiles(const Operand& A, const Operand& B, l
   for (int r = 0; r < kR; ++r) read(r, 0, 0, 0);
   int m0, n0, kt0, nkt;
   for (int j = 0; tile(j, m0, n0, kt0, nkt); ++j) {
-    f32x16 acc[C::kFM][C::kFN] = {};
+    // three planes: the five small pairs have sums of their own and the large one has two, so that these are rounded
+    // less often and at a smaller size
+    f32x16 acc[C::kFM][C::kFN] = {}, odd[C::kFM][C::kFN] = {}, low[C::kFM][C::kFN] = {};
     for (int left = nkt; left > 0; --left) {
       const unsigned after = so + C::kStageBytes == C::kLds ? 0u : so + C::kStageBytes;
 #pragma unroll
@@ -279,9 +281,11 @@ __device__ __forceinline__ void gemm_tiles(const Operand& A, const Operand& B, l
 #pragma unroll
           for (int t = 0; t < kTerms; ++t)
 #pragma unroll
-            for (int j = 0; j < C::kFN; ++j)
-              acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(fa[q & 1][P == 1 ? 0 : kPairA[t]][i],
-                                                                  fb[q & 1][P == 1 ? 0 : kPairB[t]][j], acc[i][j], 0, 0, 0);
+            for (int j = 0; j < C::kFN; ++j) {
+              f32x16& to = P == 1 ? acc[i][j] : t < 5 ? low[i][j] : q & 1 ? odd[i][j] : acc[i][j];
+              to = __builtin_amdgcn_mfma_f32_32x32x16_bf16(fa[q & 1][P == 1 ? 0 : kPairA[t]][i], fb[q & 1][P == 1 ? 0 : kPairB[t]][j],
+                                                           to, 0, 0, 0);
+            }
           if (q == 0 && i == 0) next();  // scalar work, while the first products run
           if (i < kHalf) {
             // (the next step's are the next tile's after a tile's last step)
@@ -299,6 +303,11 @@ __device__ __forceinline__ void gemm_tiles(const Operand& A, const Operand& B, l
       so = after;
       fill = fill + C::kStageBytes == C::kLds ? 0u : fill + C::kStageBytes;
     }
+    if (P == 3)
+#pragma unroll
+      for (int i = 0; i < C::kFM; ++i)
+#pragma unroll
+        for (int j = 0; j < C::kFN; ++j) acc[i][j] += odd[i][j] + low[i][j];
     done(j, m0, n0, acc);
   }
   wait_vm<0>();  // no DMA outlives the block
