@@ -537,3 +537,93 @@ def test_graph(cuda, dtype):
         torch.cuda.synchronize()
         for a, c in zip(out, want):
             assert torch.equal(a, c)
+
+
+# ------------------------------------------------------------------ the multiclass linear model on dense rows
+def _train_dense(tmp, dev, K, dense, **kw):
+    import os
+
+    import numpy as np
+    from ytk_learn_amd.config.hocon import parse_file
+    from ytk_learn_amd.parallel.comm import Comm
+    from ytk_learn_amd.train import train
+
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    rng = np.random.default_rng(7)
+    W = rng.normal(size=(12, K))
+    os.makedirs(tmp, exist_ok=True)
+    for name, n in (("tr", 400), ("te", 90)):
+        x = rng.random((n, 12)).round(4)
+        y = (x @ W).argmax(1)
+        with open(f"{tmp}/{name}.txt", "w") as f:
+            for i in range(n):
+                keep = [j for j in range(12) if (i + j) % 5]  # absent features are zeros
+                f.write("%g###%d###%s\n" % (1 + i % 3, y[i], ",".join(f"{j}:{x[i, j]:.4f}" for j in keep)))
+    ov = {"data.train.data_path": f"{tmp}/tr.txt", "data.test.data_path": f"{tmp}/te.txt", "model.data_path": f"{tmp}/m", "k": K,
+          "loss.evaluate_metric": [], "optimization.line_search.lbfgs.convergence.max_iter": 6, "dense_head": dense}
+    ov.update(kw)
+    c = parse_file(os.path.join(root, "config", "model", "multiclass_linear.conf")).with_overrides(ov)
+    return train("multiclass_linear", c, comm=Comm.local(dev))
+
+
+def _dense_gradient(dev, K):
+    """The model's loss and gradient on rows with absent and repeated features."""
+    from types import SimpleNamespace
+
+    from ytk_learn_amd.models.continuous.multiclass import MulticlassLinearModel, class_ids, dense_rows
+    from ytk_learn_amd.ops.sparse import SparseMatrix
+
+    g = torch.Generator().manual_seed(K)
+    n, F = 150, 12
+    count = torch.randint(0, 6, (n,), generator=g)
+    indptr = torch.cat([torch.zeros(1, dtype=torch.int64), count.cumsum(0)])
+    cols = torch.randint(0, F, (int(indptr[-1]),), generator=g, dtype=torch.int32)
+    vals = torch.rand(int(indptr[-1]), generator=g)
+    y = torch.randint(0, K, (n,), generator=g)
+    X = SparseMatrix(indptr.to(dev), cols.to(dev), vals.to(dev), F)
+    x = torch.zeros(n, F, dtype=torch.float64)
+    x.index_put_((torch.repeat_interleave(torch.arange(n), count), cols.long()), vals.double(), accumulate=True)
+    onehot = torch.nn.functional.one_hot(y, K).float().to(dev)
+    W = torch.randn(F, K - 1, generator=g).to(dev)
+    wt = torch.rand(n, generator=g).to(dev)
+    m = MulticlassLinearModel.__new__(MulticlassLinearModel)
+    m.F, m.S, m.dense = F, K - 1, {"train": (dense_rows(X), class_ids(onehot))}
+    # a repeated feature's values are summed in fp32: exact operands for the reference are the rows the model holds
+    near(m.dense["train"][0], x, 8 * U * x.abs(), "rows")
+    out = torch.empty(F * (K - 1), device=dev)
+    loss, pred = m._forward(X, SimpleNamespace(weight=wt), W.view(-1), out, "train")
+    ref = Ref(m.dense["train"][0], W.t(), *label_targets(y), weight=wt, base=True)
+    assert pred is None and abs(loss - float(ref.loss.sum())) <= float(ref.eloss.sum())
+    near(out.view(F, K - 1).t(), ref.dw, ref.edw, "gradient")
+    loss2, _ = m._forward(X, SimpleNamespace(weight=wt), W.view(-1), None, "train")
+    assert loss2 == loss
+
+
+@pytest.mark.parametrize("K", [2, 70])
+def test_dense_head_gradient_cpu(K):
+    _dense_gradient("cpu", K)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("K", [2, 70, 300])
+def test_dense_head_gradient_gpu(cuda, K):
+    _dense_gradient(cuda, K)
+
+
+def test_dense_head_trains_cpu(tmp_path):
+    r = _train_dense(str(tmp_path / "a"), "cpu", 70, True)
+    assert r.loss > 0 and r.test_loss > 0
+
+
+def test_dense_head_refusals(tmp_path):
+    from ytk_learn_amd.utils.errors import YtkLearnError
+    for kw in ({"loss.loss_function": "multiclass_hinge"}, {"loss.evaluate_metric": ["confusion_matrix"]}):
+        with pytest.raises(YtkLearnError):
+            _train_dense(str(tmp_path / "r"), "cpu", 5, True, **kw)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("K", [3, 300])
+def test_dense_head_trains_gpu(cuda, tmp_path, K):
+    r = _train_dense(str(tmp_path / "b"), cuda, K, True)
+    assert r.loss > 0 and r.test_loss > 0

@@ -346,7 +346,7 @@ class CommonParams:
                       "hyper.grid.l2 length must be 3 * loss.regularization.l2 length")
         for key in ("k", "bias_need_latent_factor", "instance_sample_rate", "feature_sample_rate",
                     "uniform_base_prediction", "sample_dependent_base_prediction", "tree_num",
-                    "learning_rate", "type", "leaf_random_init_range"):
+                    "learning_rate", "type", "leaf_random_init_range", "dense_head"):
             if c.has(key):
                 p.extra[key] = c.get(key)
         return p

@@ -8,6 +8,9 @@ class id or a K-vector summing to 1; dump ``name,w_0,...,w_{K-2}`` with Float.to
 Device path: S = X W and G = X^T D as the segmented SpMM kernel (J = K-1 columns); the
 per-row loss / prediction / D epilogue is one fused HIP pass (``ops.blas.multiclass_row_loss``,
 every multiclass loss, K <= 64) and fp64 torch otherwise.
+``dense_head = true`` (extension, softmax with one class per row): dense rows X [n, F] against the
+F x (K-1) weights through ``ops.head.softmax_head_loss``, for many classes: no n x K scores,
+probabilities or score gradients are held.
 Note: y_sampling keys on the first label value (a class id line); K-vector label lines are
 not sampled by class.
 """
@@ -19,7 +22,23 @@ import numpy as np
 import torch
 
 from ...ops.blas import multiclass_row_loss
+from ...ops.head import softmax_head_loss
+from ...utils.errors import YtkLearnError
 from .base import ContinuousModelBase, jfloat
+
+
+def dense_rows(X) -> torch.Tensor:
+    """The rows of a SparseMatrix as a dense fp32 [n, ncols] matrix."""
+    out = torch.zeros(X.n * X.ncols, dtype=torch.float32, device=X.device)
+    out.index_add_(0, X.rows_of_nnz.long() * X.ncols + X.indices.long(), X.values)
+    return out.view(X.n, X.ncols)
+
+
+def class_ids(y: torch.Tensor) -> torch.Tensor:
+    """Class of every one-hot label row."""
+    if not bool(((y == 1.0).sum(1) == 1).all() & ((y != 0.0).sum(1) == 1).all()):
+        raise YtkLearnError("dense_head needs one class per row (one-hot labels)")
+    return y.argmax(1)
 
 
 class MulticlassLinearModel(ContinuousModelBase):
@@ -33,6 +52,15 @@ class MulticlassLinearModel(ContinuousModelBase):
         if not self.loss.multi:
             raise ValueError(f"multiclass_linear needs a multi-class loss, got {self.loss.name}")
         self.S = self.K - 1
+        self.dense = {}  # "train" / "test": (dense rows, class ids)
+        if params.extra.get("dense_head", False):
+            if self.loss.name != "softmax":
+                raise YtkLearnError(f"dense_head needs the softmax loss, got {self.loss.name}")
+            if params.loss.evaluate_metric:
+                raise YtkLearnError("dense_head holds no predictions: loss.evaluate_metric must be empty")
+            for part, X, d in (("train", self.X, data.train), ("test", self.Xt, data.test)):
+                if X is not None:
+                    self.dense[part] = (dense_rows(X), class_ids(d.y))
         self.dim = self.F * self.S
         self.w = torch.zeros(self.dim, dtype=torch.float32, device=self.device)
         rows = self.load_model_rows()
@@ -50,8 +78,14 @@ class MulticlassLinearModel(ContinuousModelBase):
     def _eval_info(self):
         return (self.K, True)
 
-    def _forward(self, X, d, w, g):
+    def _forward(self, X, d, w, g, part):
         W = w.view(self.F, self.S)
+        if part in self.dense:
+            x, ids = self.dense[part]
+            r = softmax_head_loss(x, W.t(), ids, weight=d.weight.float(), base_class=True, want_dx=False, want_dw=g is not None)
+            if g is not None:
+                g.view(self.F, self.S).copy_(r.dw.t())
+            return float(r.loss.double().sum()), None
         s32 = X.matmul(W)
         fused = multiclass_row_loss(self.loss, s32, d.y, d.weight, want_grad=g is not None)
         if fused is not None:  # one fused row pass on the GPU
@@ -70,7 +104,7 @@ class MulticlassLinearModel(ContinuousModelBase):
         return float((wt * lv).sum()), pred.float()
 
     def pure_loss_grad(self, w, g):
-        loss, self.pred = self._forward(self.X, self.data.train, w, g)
+        loss, self.pred = self._forward(self.X, self.data.train, w, g, "train")
         return loss
 
     def test_pure_loss_grad(self, w, g):
@@ -78,7 +112,7 @@ class MulticlassLinearModel(ContinuousModelBase):
             return 0.0
         if g is not None and self.Xt._csc is None:
             self.Xt._build_csc()
-        loss, self.pred_test = self._forward(self.Xt, self.data.test, w, g)
+        loss, self.pred_test = self._forward(self.Xt, self.data.test, w, g, "test")
         return loss
 
     def dump(self, w, precision):
