@@ -166,8 +166,10 @@ __global__ __launch_bounds__(C::kThreads) void scores_kernel(ScoreArgs p) {
   gemm_tiles<C, kKC, kKC>(
       p.w, p.x, p.kw, p.K,
       [&](int j, int& m0, int& n0, int& kt0, int& nkt) {
+        const int id = item_of(j, p.nm * p.nn);
+        if (id < 0) return false;
         int tm, tn;
-        if (!tile_of(j, p.nm, p.nn, tm, tn)) return false;
+        order_of(id, p.nm, p.nn, tm, tn);
         m0 = tm * C::kBM, n0 = tn * C::kBN, kt0 = 0, nkt = p.K / C::kBK;
         return true;
       },
@@ -884,34 +886,63 @@ __global__ __launch_bounds__(1024) void db_kernel(const float* __restrict__ part
 struct GradArgs {
   Operand a, b;
   long long ka, kb;        // extent of K in each operand's memory
-  int K, splits;           // products run over K (at most ka, kb), cut into `splits` runs of whole 64s
+  int K;                   // products run over K (at most ka, kb)
   int M, N, nm, nn;        // result [N][M], M contiguous
+  // tiles taken whole; each of the rest is cut along K into ts runs of `per` (a multiple of 64). With runs, whole is
+  // a multiple of the grid and the runs are at most one per block.
+  int whole, ts, per, grid;
   void* out;               // T [N][ldo]
   long long ldo;
-  float* acc;              // [splits][N][M] fp32
-  int mode;                // 0: out = C  1: acc[split] = C  2: acc += C  3: out = acc + C
+  float* part;             // the runs' sums, a tile each: [tile - whole][ts][kBN][kBM]
+  float* acc;              // pieces of rows: [N][M] fp32
+  int mode;                // 0: out = C  1: acc = C  2: acc += C  3: out = acc + C
 };
+
+// Item of the block's j-th turn: whole tiles first, in full rounds of the grid, then one round of runs.
+__device__ __forceinline__ bool grad_item(const GradArgs& p, int j, int& id, int& run) {
+  const int rounds = p.ts > 1 ? p.whole / (int)gridDim.x : 1 << 30;
+  run = -1;
+  if (j < rounds) {
+    id = item_of(j, p.whole);
+    return id >= 0;
+  }
+  const int item = j == rounds ? item_of(0, (p.nm * p.nn - p.whole) * p.ts) : -1;
+  if (item < 0) return false;
+  id = p.whole + item / p.ts;
+  run = item % p.ts;
+  return true;
+}
 
 template <class C, int kLA, int kLB, typename T>
 __global__ __launch_bounds__(C::kThreads) void grad_kernel(GradArgs p) {
   const int wave = threadIdx.x >> 6, l = threadIdx.x & 63, hi = l >> 5;
-  // runs of whole 64s; the host leaves none of them empty
-  const int per = (p.K + 64 * p.splits - 1) / (64 * p.splits) * 64;
   gemm_tiles<C, kLA, kLB>(
       p.a, p.b, p.ka, p.kb,
       [&](int j, int& m0, int& n0, int& kt0, int& nkt) {
-        int tm, tn;
-        if (!tile_of(j, p.nm, p.nn * p.splits, tm, tn)) return false;
-        const int k0 = tn / p.nn * per;
-        m0 = tm * C::kBM, n0 = tn % p.nn * C::kBN;
-        kt0 = k0 / C::kBK, nkt = (min(per, p.K - k0) + C::kBK - 1) / C::kBK;
+        int id, run, tm, tn;
+        if (!grad_item(p, j, id, run)) return false;
+        order_of(id, p.nm, p.nn, tm, tn);
+        const int k0 = run < 0 ? 0 : run * p.per, k1 = run < 0 ? p.K : min(k0 + p.per, p.K);
+        m0 = tm * C::kBM, n0 = tn * C::kBN;
+        kt0 = k0 / C::kBK, nkt = (k1 - k0 + C::kBK - 1) / C::kBK;
         return true;
       },
       [&](int j, int m0, int n0, f32x16(&acc)[C::kFM][C::kFN]) {
-        int tm, tn;
-        tile_of(j, p.nm, p.nn * p.splits, tm, tn);
-        const int split = tn / p.nn;
+        int id, run;
+        grad_item(p, j, id, run);
         const int mw = m0 + (wave / C::kWN) * C::kFM * 32, nw = n0 + (wave % C::kWN) * C::kFN * 32;
+        if (run >= 0) {
+          float* t = p.part + ((long long)(id - p.whole) * p.ts + run) * (C::kBM * C::kBN);
+#pragma unroll
+          for (int j = 0; j < C::kFN; ++j)
+#pragma unroll
+            for (int i = 0; i < C::kFM; ++i)
+#pragma unroll
+              for (int q = 0; q < 4; ++q)
+                *(float4*)(t + (nw - n0 + j * 32 + (l & 31)) * C::kBM + mw - m0 + i * 32 + 8 * q + 4 * hi) =
+                    make_float4(acc[i][j][4 * q], acc[i][j][4 * q + 1], acc[i][j][4 * q + 2], acc[i][j][4 * q + 3]);
+          return;
+        }
         const bool vec = (p.ldo & 7) == 0 && ((uintptr_t)p.out & 15) == 0, avec = (p.M & 3) == 0;
 #pragma unroll
         for (int j = 0; j < C::kFN; ++j) {
@@ -925,7 +956,7 @@ __global__ __launch_bounds__(C::kThreads) void grad_kernel(GradArgs p) {
               if (m >= p.M) continue;
               float v[4] = {acc[i][j][4 * q], acc[i][j][4 * q + 1], acc[i][j][4 * q + 2], acc[i][j][4 * q + 3]};
               if (p.mode) {
-                float* a = p.acc + ((long long)split * p.N + n) * p.M + m;
+                float* a = p.acc + (long long)n * p.M + m;
                 if (avec) {
                   if (p.mode != 1) {
                     const float4 o = *(const float4*)a;
@@ -955,6 +986,32 @@ __global__ __launch_bounds__(C::kThreads) void grad_kernel(GradArgs p) {
             }
         }
       });
+}
+
+// out tile = sum of its runs, in order: 32 result rows of one tile per block
+template <int BM, int BN, typename T>
+__global__ __launch_bounds__(256) void run_sum_kernel(GradArgs p) {
+  int tm, tn;
+  order_of(p.whole + (int)blockIdx.x, p.nm, p.nn, tm, tn);
+  constexpr int kPer = BM / 4;  // threads per row
+  const int m = tm * BM + (int)(threadIdx.x % kPer) * 4;
+  if (m >= p.M) return;
+  for (int r = threadIdx.x / kPer; r < 32; r += 256 / kPer) {
+    const int nl = blockIdx.y * 32 + r, n = tn * BN + nl;
+    if (n >= p.N) return;
+    const float* t = p.part + (long long)blockIdx.x * p.ts * (BM * BN) + nl * BM + (m - tm * BM);
+    float4 s = make_float4(0, 0, 0, 0);
+#pragma unroll 4
+    for (int k = 0; k < p.ts; ++k) {
+      const float4 v = *(const float4*)(t + (long long)k * (BM * BN));
+      s.x += v.x, s.y += v.y, s.z += v.z, s.w += v.w;
+    }
+    const float v[4] = {s.x, s.y, s.z, s.w};
+    T* o = (T*)p.out + (long long)n * p.ldo + m;
+#pragma unroll
+    for (int u = 0; u < 4; ++u)
+      if (m + u < p.M) Elem<T>::put(o, u, v[u]);
+  }
 }
 
 // out = sum over splits, in split order
@@ -1260,38 +1317,49 @@ constexpr unsigned kLdsAll = 160 * 1024;
 
 enum { kBig = 0, kWide = 1, kMid = 2, kF32 = 3 };
 
-// Estimated time of an M x N x K product in units of one CU's multiply-adds: rounds of blocks over the 256 CUs,
-// each paying its tile's products at the tile's rate, and about 4 us (10^7 multiply-adds) to start and finish;
-// K cut into `splits` runs costs the partial sums' traffic.
-static double tile_cost(int cfg, long long m, long long n, long long k, int terms, int splits) {
-  const int bm = cfg == kBig ? 256 : 128, bn = cfg >= kMid ? 128 : 256, per_cu = cfg == kMid ? 2 : 1;
+// How a product is laid over the card, and its estimated time in units of one CU's multiply-adds (2.7e12 a second):
+// full rounds of blocks over the 256 CUs at the tile's rate, and about 4 us (10^7) each to start and finish; the
+// tiles left over are cut along K into `ts` runs, at most one per block, whose sums are written and read again (4.6
+// per value at the card's copy rate).
+struct Layout {
+  int cfg, whole, ts, per, grid;
+  double cost;
+};
+
+static Layout layout_of(int cfg, long long m, long long n, long long k, int terms, bool runs) {
+  const int bm = cfg == kBig ? 256 : 128, bn = cfg >= kMid ? 128 : 256;
   const double rate = cfg == kMid ? 0.7 : cfg == kWide ? 0.92 : 1.0;
-  const long long blocks = (long long)ceil_div(m, bm) * ceil_div(n, bn) * splits;
-  const long long rounds = (blocks + 256 * per_cu - 1) / (256 * per_cu);
-  const double one = (double)bm * bn * (double)up((k + splits - 1) / splits, 64) * terms / rate * std::min<long long>(per_cu, (blocks + 255) / 256);
-  return rounds * (one + 1e7) + (splits > 1 ? 5e6 + (double)m * n * splits * 5.0 : 0.0);
+  const long long tiles = (long long)ceil_div(m, bm) * ceil_div(n, bn), grid = cfg == kMid && tiles > 256 ? 512 : 256;
+  const long long rounds = tiles / grid, tail = tiles % grid;
+  auto one = [&](long long kk, long long blocks) {
+    return (double)bm * bn * (double)up(kk, 64) * terms / rate * (double)std::min(grid / 256, (blocks + 255) / 256) + 1e7;
+  };
+  Layout best = {cfg, (int)tiles, 1, 0, (int)grid, 1e300};
+  for (long long ts = 1; ts <= (runs && tail ? std::max(1LL, std::min(grid / tail, k * terms / 512)) : 1); ++ts) {
+    const long long per = up((k + ts - 1) / ts, 64);
+    if (ceil_div(k, per) != ts) continue;  // an empty run
+    const double c = rounds * one(k, grid) + (tail ? one(per, tail * ts) : 0.0) + (ts > 1 ? 8e6 + 4.6 * (double)(tail * ts) * bm * bn : 0.0);
+    if (c < best.cost) best = {cfg, (int)(ts > 1 ? tiles - tail : tiles), (int)ts, (int)per, (int)grid, c};
+  }
+  return best;
+}
+
+static Layout pick_layout(long long m, long long n, long long k, int terms, bool runs) {
+  Layout best = layout_of(terms == 1 ? kBig : kF32, m, n, k, terms, runs);
+  for (int c = kWide; terms == 1 && c <= kMid; ++c) {
+    const Layout l = layout_of(c, m, n, k, terms, runs);
+    if (l.cost < best.cost) best = l;
+  }
+  return best;
+}
+
+static long long run_bytes(const Layout& l, long long m, long long n) {
+  const int bm = l.cfg == kBig ? 256 : 128, bn = l.cfg >= kMid ? 128 : 256;
+  return l.ts == 1 ? 0 : ((long long)ceil_div(m, bm) * ceil_div(n, bn) - l.whole) * l.ts * bm * bn * 4;
 }
 
 // one round of Mid tiles: a block alone on its CU, so the latency of its K steps counts
-static bool use_deep(long long m, long long n, int splits) {
-  return (long long)ceil_div(m, CfgMid::kBM) * ceil_div(n, CfgMid::kBN) * splits <= 256;
-}
-
-static int pick_tile(long long m, long long n, long long k, int terms, int max_splits, int* splits) {
-  int best = kBig;
-  double cost = 1e300;
-  for (int c = terms == 1 ? kBig : kF32; c <= (terms == 1 ? kMid : kF32); ++c)
-    for (int s = 1; s <= max_splits && (s == 1 || k / s >= 512 / terms); s = s < 4 ? s + 1 : s + s / 4) {
-      const double t = tile_cost(c, m, n, k, terms, s);
-      if (t < cost) {
-        cost = t;
-        best = c;
-        // no empty run: as many as whole 64s of this length need
-        if (splits) *splits = ceil_div(k, up((k + s - 1) / s, 64));
-      }
-    }
-  return best;
-}
+static bool use_deep(long long tiles) { return tiles <= 256; }
 
 template <class C>
 void scores_launch(ScoreArgs p, int mode, hipStream_t s) {
@@ -1320,10 +1388,14 @@ void scores_launch(ScoreArgs p, int mode, hipStream_t s) {
 
 template <class C, int LA, int LB, typename T>
 void grad_launch(GradArgs p, hipStream_t s) {
-  p.nm = ceil_div(p.M, C::kBM);
-  p.nn = ceil_div(p.N, C::kBN);
-  grad_kernel<C, LA, LB, T><<<grid8((long long)p.nm * p.nn * p.splits, kLdsAll / C::kLds), C::kThreads, C::kLds, s>>>(p);
+  const long long tiles = (long long)p.nm * p.nn;
+  const int g = p.ts > 1 ? p.grid : grid8(tiles, kLdsAll / C::kLds);
+  grad_kernel<C, LA, LB, T><<<g, C::kThreads, C::kLds, s>>>(p);
   YTK_LAUNCH_CHECK();
+  if (p.ts > 1) {
+    run_sum_kernel<C::kBM, C::kBN, T><<<dim3((unsigned)(tiles - p.whole), C::kBN / 32), 256, 0, s>>>(p);
+    YTK_LAUNCH_CHECK();
+  }
 }
 
 }  // namespace ytk
@@ -1352,7 +1424,7 @@ struct HeadPlan {
   int planes, terms;
   long long kp, ld, groups, piece;
   bool pack_x, pack_w, grads, few, few_dw, planes_d;
-  int splits_dx, splits_dw, tile_dx, tile_dw, rw, few_per;
+  int rw, few_per, few_runs;
   bool many;  // more than one piece of rows
   long long o_x, o_w, o_xg, o_e, o_d, o_stats, o_zt, o_q, o_coef, o_norm, o_part, o_dbacc, o_dwacc, o_split, bytes;
 };
@@ -1375,17 +1447,17 @@ static HeadPlan head_plan(const HeadIn& h, bool topk) {
   // (at most 2M rows: the grids of the row passes count rows / 64 in 16 bits and rows * k in 31)
   p.piece = std::min(h.n, std::min(1LL << 21, std::max(256LL, h.piece_bytes / per / 256 * 256)));
   p.many = p.piece < h.n;
-  p.splits_dx = p.splits_dw = 1;
-  // partial sums of at most a quarter of the pieces' bytes (64 runs at most); pieces of rows already sum into dw
-  auto most = [&](long long rows) { return (int)std::max(1LL, std::min(64LL, h.piece_bytes / 4 / (rows * h.d * 4))); };
+  long long part = 0;
   if (h.want_dx && p.few) {  // runs of classes: about 1024 blocks, at least 128 classes each
     const long long runs = std::max(1LL, std::min<long long>(1024 / (ceil_div(h.d, 64) * ceil_div(h.n, 64)), ceil_div(h.V, 128)));
     p.few_per = (int)up((h.V + runs - 1) / runs, 64);
-    p.splits_dx = ceil_div(h.V, p.few_per);
+    p.few_runs = ceil_div(h.V, p.few_per);
+    part = p.few_runs > 1 ? p.few_runs * h.n * h.d * 4 : 0;
   } else if (h.want_dx) {
-    p.tile_dx = pick_tile(h.d, p.piece, h.V, p.terms, most(p.piece), &p.splits_dx);
+    for (const long long rows : {p.piece, (h.n - 1) % p.piece + 1})
+      part = std::max(part, run_bytes(pick_layout(h.d, rows, h.V, p.terms, true), h.d, rows));
   }
-  if (h.want_dw) p.tile_dw = pick_tile(h.d, h.V, p.piece, p.terms, p.many ? 1 : most(h.V), &p.splits_dw);
+  if (h.want_dw && !p.many && !p.few_dw) part = std::max(part, run_bytes(pick_layout(h.d, h.V, h.n, p.terms, true), h.d, h.V));
   long long o = 0;
   auto take = [&](bool want, long long bytes) {
     const long long at = o;
@@ -1410,8 +1482,7 @@ static HeadPlan head_plan(const HeadIn& h, bool topk) {
   p.o_part = take(db, ceil_div(p.piece, 4 * p.rw) * p.ld * 4);
   p.o_dbacc = take(db, h.V * 4);
   p.o_dwacc = take(h.want_dw && p.many, h.V * h.d * 4);
-  p.o_split = take(p.splits_dx > 1 || p.splits_dw > 1 || p.few,
-                   std::max(p.splits_dx > 1 || p.few ? p.splits_dx * p.piece * h.d : 0, p.splits_dw > 1 ? p.splits_dw * h.V * h.d : 0) * 4);
+  p.o_split = take(part > 0, part);
   p.bytes = o;
   return p;
 }
@@ -1439,16 +1510,21 @@ static void pack_rows(const void* src, long long rs, long long cs, long long row
   }
 }
 
+// C = A B^T of g.M x g.N x g.K; `part` has room for the runs of this layout
 template <int LA, int LB, typename T>
-static void grad_product(GradArgs g, int tile, hipStream_t s) {
+static void grad_product(GradArgs g, bool runs, hipStream_t s) {
+  const Layout l = pick_layout(g.M, g.N, g.K, sizeof(T) == 4 ? 6 : 1, runs);
+  g.whole = l.whole, g.ts = l.ts, g.per = l.per, g.grid = l.grid;
+  g.nm = ceil_div(g.M, l.cfg == kBig ? 256 : 128);
+  g.nn = ceil_div(g.N, l.cfg >= kMid ? 128 : 256);
   if constexpr (sizeof(T) == 4) {
     grad_launch<CfgF32, LA, LB, T>(g, s);
   } else {
-    if (tile == kBig)
+    if (l.cfg == kBig)
       grad_launch<CfgBig, LA, LB, T>(g, s);
-    else if (tile == kWide)
+    else if (l.cfg == kWide)
       grad_launch<CfgWide, LA, LB, T>(g, s);
-    else if (use_deep(g.M, g.N, g.splits))
+    else if (use_deep((long long)g.nm * g.nn))
       grad_launch<CfgDeep, LA, LB, T>(g, s);
     else
       grad_launch<CfgMid, LA, LB, T>(g, s);
@@ -1530,8 +1606,8 @@ static void dx_few(const HeadIn& h, const HeadPlan& p, const void* w, char* ws, 
   a.w = (const float*)w, a.D = (const float*)(ws + p.o_e);
   a.wrs = h.wrs, a.ld = p.ld;
   a.V = (int)h.V, a.n = (int)h.n, a.d = (int)h.d, a.per = p.few_per;
-  a.acc = p.splits_dx > 1 ? (float*)(ws + p.o_split) : (float*)out;
-  const dim3 g(ceil_div(h.d, 64), p.splits_dx, h.n <= 64 ? 1 : ceil_div(h.n, 64));
+  a.acc = p.few_runs > 1 ? (float*)(ws + p.o_split) : (float*)out;
+  const dim3 g(ceil_div(h.d, 64), p.few_runs, h.n <= 64 ? 1 : ceil_div(h.n, 64));
   if (h.n <= 16)
     dx_few_kernel<1><<<g, 256, 0, s>>>(a);
   else if (h.n <= 32)
@@ -1539,7 +1615,7 @@ static void dx_few(const HeadIn& h, const HeadPlan& p, const void* w, char* ws, 
   else
     dx_few_kernel<4><<<g, 256, 0, s>>>(a);
   YTK_LAUNCH_CHECK();
-  if (p.splits_dx > 1) split_sum<float>(a.acc, p.splits_dx, h.n, h.d, out, s);
+  if (p.few_runs > 1) split_sum<float>(a.acc, p.few_runs, h.n, h.d, out, s);
 }
 
 static void dw_few(const HeadIn& h, const HeadPlan& p, const void* x, char* ws, void* out, hipStream_t s) {
@@ -1576,7 +1652,7 @@ static void scores(const HeadIn& h, const HeadPlan& p, const HeadOps& o, long lo
   a.e = ws + p.o_e;
   a.z = (float*)(ws + p.o_e);
   a.ld = p.ld;
-  const int tile = pick_tile(h.V, rows, p.kp, p.terms, 1, nullptr);
+  const int tile = pick_layout(h.V, rows, p.kp, p.terms, false).cfg;
   if (h.f32)
     scores_launch<CfgF32>(a, mode, s);
   else if (rows <= 64)
@@ -1585,7 +1661,7 @@ static void scores(const HeadIn& h, const HeadPlan& p, const HeadOps& o, long lo
     scores_launch<CfgBig>(a, mode, s);
   else if (tile == kWide)
     scores_launch<CfgWide>(a, mode, s);
-  else if (use_deep(h.V, rows, 1))
+  else if (use_deep((long long)ceil_div(h.V, 128) * ceil_div(rows, 128)))
     scores_launch<CfgDeep>(a, mode, s);
   else
     scores_launch<CfgMid>(a, mode, s);
@@ -1705,18 +1781,14 @@ extern "C" void ytk_head_loss(const uintptr_t* ptrs, const long long* lp, double
       g.a.ext = (int)(p.pack_w ? p.kp : h.d);
       g.b = D;
       g.ka = h.V, g.kb = p.ld;
-      g.K = (int)h.V, g.splits = p.splits_dx;
+      g.K = (int)h.V;
       g.M = (int)h.d, g.N = (int)rows;
       g.out = (char*)ptrs[10] + r0 * h.d * el, g.ldo = h.d;
-      g.acc = (float*)(ws + p.o_split);
-      g.mode = g.splits > 1 ? 1 : 0;
-      if (h.f32) {
-        grad_product<kKS, kKC, float>(g, p.tile_dx, s);
-        if (g.splits > 1) split_sum<float>(g.acc, g.splits, rows, h.d, g.out, s);
-      } else {
-        grad_product<kKS, kKC, __bf16>(g, p.tile_dx, s);
-        if (g.splits > 1) split_sum<__bf16>(g.acc, g.splits, rows, h.d, g.out, s);
-      }
+      g.part = (float*)(ws + p.o_split);
+      if (h.f32)
+        grad_product<kKS, kKC, float>(g, true, s);
+      else
+        grad_product<kKS, kKC, __bf16>(g, true, s);
     }
     if (h.want_dw && p.few_dw) {
       dw_few(h, p, x, ws, (void*)ptrs[11], s);
@@ -1732,18 +1804,16 @@ extern "C" void ytk_head_loss(const uintptr_t* ptrs, const long long* lp, double
       g.b = D;
       g.b.ext = (int)p.ld;
       g.ka = g.kb = rows;
-      g.K = (int)rows, g.splits = p.splits_dw;
+      g.K = (int)rows;
       g.M = (int)h.d, g.N = (int)h.V;
       g.out = (void*)ptrs[11], g.ldo = h.d;
-      g.acc = (float*)(ws + (p.many ? p.o_dwacc : p.o_split));
-      g.mode = g.splits > 1 ? 1 : !p.many ? 0 : first ? 1 : last ? 3 : 2;
-      if (h.f32) {
-        grad_product<kKS, kKS, float>(g, p.tile_dw, s);
-        if (g.splits > 1) split_sum<float>(g.acc, g.splits, h.V, h.d, g.out, s);
-      } else {
-        grad_product<kKS, kKS, __bf16>(g, p.tile_dw, s);
-        if (g.splits > 1) split_sum<__bf16>(g.acc, g.splits, h.V, h.d, g.out, s);
-      }
+      g.part = (float*)(ws + p.o_split);
+      g.acc = (float*)(ws + p.o_dwacc);
+      g.mode = !p.many ? 0 : first ? 1 : last ? 3 : 2;
+      if (h.f32)
+        grad_product<kKS, kKS, float>(g, !p.many, s);
+      else
+        grad_product<kKS, kKS, __bf16>(g, !p.many, s);
     }
   }
 }

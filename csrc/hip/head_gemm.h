@@ -313,17 +313,19 @@ __device__ __forceinline__ void gemm_tiles(const Operand& A, const Operand& B, l
   wait_vm<0>();  // no DMA outlives the block
 }
 
-// j-th tile of this block: each XCD (blocks go to them round robin) works through a contiguous run of the tile
-// order, its blocks side by side, and the order walks 8 m tiles before the next n tile, so the 32 CUs behind one
-// L2 share their panels. The grid is a multiple of 8.
-__device__ __forceinline__ bool tile_of(int j, int nm, int nn, int& tm, int& tn) {
-  const int T = nm * nn, chunk = (T + 7) / 8;
-  const int at = (int)(blockIdx.x >> 3) + j * (int)(gridDim.x >> 3), id = (int)(blockIdx.x & 7) * chunk + at;
-  if (at >= chunk || id >= T) return false;
+// Tile order: 8 m tiles before the next n tile, so that tiles next to each other share their panels.
+__device__ __forceinline__ void order_of(int id, int nm, int nn, int& tm, int& tn) {
   const int gsz = 8 * nn, g = id / gsz, r = id % gsz, gm = nm - g * 8 < 8 ? nm - g * 8 : 8;
   tm = g * 8 + r % gm;
   tn = r / gm;
-  return true;
+}
+
+// j-th of the `count` items of this block: each XCD (blocks go to them round robin) works through a contiguous run of
+// them, its blocks side by side, so the 32 CUs behind one L2 share what they read. The grid is a multiple of 8. -1: no more.
+__device__ __forceinline__ int item_of(int j, int count) {
+  const int chunk = (count + 7) / 8, at = (int)(blockIdx.x >> 3) + j * (int)(gridDim.x >> 3);
+  const int id = (int)(blockIdx.x & 7) * chunk + at;
+  return at < chunk && id < count ? id : -1;
 }
 
 }  // namespace ytk
