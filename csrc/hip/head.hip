@@ -944,6 +944,24 @@ __global__ __launch_bounds__(C::kThreads) void grad_kernel(GradArgs p) {
           return;
         }
         const bool vec = (p.ldo & 7) == 0 && ((uintptr_t)p.out & 15) == 0, avec = (p.M & 3) == 0;
+        if (sizeof(T) == 2 && p.mode == 0 && vec && (p.M & 7) == 0) {  // 16-byte stores: a lane's 8 values of m
+#pragma unroll
+          for (int j = 0; j < C::kFN; ++j) {
+            const int n = nw + j * 32 + (l & 31);
+#pragma unroll
+            for (int i = 0; i < C::kFM; ++i)
+#pragma unroll
+              for (int q = 0; q < 4; q += 2) {
+                const f32x16& t = acc[i][j];
+                unsigned a0 = pack_b2(t[4 * q], t[4 * q + 1]), a1 = pack_b2(t[4 * q + 2], t[4 * q + 3]);
+                unsigned b0 = pack_b2(t[4 * q + 4], t[4 * q + 5]), b1 = pack_b2(t[4 * q + 6], t[4 * q + 7]);
+                swap_quads(a0, a1, b0, b1);
+                const int m = mw + i * 32 + 8 * q + 8 * hi;
+                if (n < p.N && m < p.M) *(uint4*)((T*)p.out + (long long)n * p.ldo + m) = make_uint4(a0, a1, b0, b1);
+              }
+          }
+          return;
+        }
 #pragma unroll
         for (int j = 0; j < C::kFN; ++j) {
           const int n = nw + j * 32 + (l & 31);
