@@ -129,6 +129,21 @@ __device__ __forceinline__ void swap_quads(unsigned& a0, unsigned& a1, unsigned&
   a0 = p[0], a1 = q[0], b0 = p[1], b1 = q[1];
 }
 
+__device__ __forceinline__ uint4 bits4(float a, float b, float c, float d) {
+  return make_uint4(__builtin_bit_cast(unsigned, a), __builtin_bit_cast(unsigned, b), __builtin_bit_cast(unsigned, c),
+                    __builtin_bit_cast(unsigned, d));
+}
+// the 32 turned rows of 128 bytes to rows of `pitch` bytes, as many as there are
+__device__ __forceinline__ void store_rows(const Turn& turn, char* to, long long pitch, int rows) {
+  const int l = threadIdx.x & 63, c = l & 7;
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    const int r = k * 8 + (l >> 3);
+    const uint4 v = turn.take(r, c);
+    if (r < rows) *(uint4*)(to + r * pitch + c * 16) = v;
+  }
+}
+
 __device__ __forceinline__ unsigned pack_h2(float a, float b) {
   typedef _Float16 h2 __attribute__((ext_vector_type(2)));
   h2 v = {(_Float16)a, (_Float16)b};
@@ -163,7 +178,7 @@ template <class C, int kMode>
 __global__ __launch_bounds__(C::kThreads) void scores_kernel(ScoreArgs p) {
   static_assert(C::kFM % 2 == 0, "a wave holds whole groups");
   const int wave = threadIdx.x >> 6, l = threadIdx.x & 63, hi = l >> 5;
-  gemm_tiles<C, kKC, kKC>(
+  gemm_tiles<C, kKC, kKC, kMode == kExpHalf || kMode == kExpFloat || kMode == kScores>(
       p.w, p.x, p.kw, p.K,
       [&](int j, int& m0, int& n0, int& kt0, int& nkt) {
         const int id = item_of(j, p.nm * p.nn);
@@ -173,7 +188,7 @@ __global__ __launch_bounds__(C::kThreads) void scores_kernel(ScoreArgs p) {
         m0 = tm * C::kBM, n0 = tn * C::kBN, kt0 = 0, nkt = p.K / C::kBK;
         return true;
       },
-      [&](int, int m0, int n0, f32x16(&acc)[C::kFM][C::kFN]) {
+      [&](int, int m0, int n0, f32x16(&acc)[C::kFM][C::kFN], const Turn& turn) {
         const int v0 = m0 + (wave / C::kWN) * C::kFM * 32, i0 = n0 + (wave % C::kWN) * C::kFN * 32;
 #pragma unroll
         for (int g = 0; g < C::kFM / 2; ++g) {
@@ -216,16 +231,14 @@ __global__ __launch_bounds__(C::kThreads) void scores_kernel(ScoreArgs p) {
               for (int r = 0; r < 16; ++r) mx = fmaxf(mx, acc[2 * g + h][j][r]);
             const float m = fmaxf(mx, __shfl_xor(mx, 32, 64)) * c;
             const float m0 = m == -INFINITY ? 0.0f : m;
-            if (kMode == kScores && i < p.n) {
-              float* o = p.z + (long long)i * p.ld + vg + 4 * hi;
+            if (kMode == kScores)
 #pragma unroll
-              for (int h = 0; h < 2; ++h)
+              for (int h = 0; h < 2; ++h) {
+                const f32x16& t = acc[2 * g + h][j];
 #pragma unroll
-                for (int q = 0; q < 4; ++q) {
-                  const f32x16& t = acc[2 * g + h][j];
-                  *(float4*)(o + h * 32 + 8 * q) = make_float4(t[4 * q] * c, t[4 * q + 1] * c, t[4 * q + 2] * c, t[4 * q + 3] * c);
-                }
-            }
+                for (int q = 0; q < 4; ++q) turn.put(l & 31, 2 * q + hi, bits4(t[4 * q] * c, t[4 * q + 1] * c, t[4 * q + 2] * c, t[4 * q + 3] * c));
+                store_rows(turn, (char*)p.z + (i0 + j * 32) * p.ld * 4 + (vg + h * 32) * 4LL, p.ld * 4, p.n - i0 - j * 32);
+              }
             float s = 0.0f, e[2][16];
             const float off = kMode == kExpHalf ? 15.0f - m0 : -m0;  // E is scaled by 2^15
 #pragma unroll
@@ -241,16 +254,14 @@ __global__ __launch_bounds__(C::kThreads) void scores_kernel(ScoreArgs p) {
             s += __shfl_xor(s, 32, 64);
             if (kMode == kExpHalf) s *= 1.0f / 32768.0f;
             if (hi == 0 && i < p.n) p.stats[(long long)(vg / kGroup) * p.n + i] = make_float2(m, s);
-            if (kMode == kExpFloat && i < p.n) {
-              float* o = (float*)p.e + (long long)i * p.ld + vg + 4 * hi;
+            if (kMode == kExpFloat)
 #pragma unroll
-              for (int h = 0; h < 2; ++h)
+              for (int h = 0; h < 2; ++h) {
 #pragma unroll
-                for (int q = 0; q < 4; ++q)
-                  *(float4*)(o + h * 32 + 8 * q) = make_float4(e[h][4 * q], e[h][4 * q + 1], e[h][4 * q + 2], e[h][4 * q + 3]);
-            }
+                for (int q = 0; q < 4; ++q) turn.put(l & 31, 2 * q + hi, bits4(e[h][4 * q], e[h][4 * q + 1], e[h][4 * q + 2], e[h][4 * q + 3]));
+                store_rows(turn, (char*)p.e + (i0 + j * 32) * p.ld * 4 + (vg + h * 32) * 4LL, p.ld * 4, p.n - i0 - j * 32);
+              }
             if (kMode == kExpHalf) {
-              unsigned short* o = (unsigned short*)p.e + (long long)i * p.ld + vg + 8 * hi;
 #pragma unroll
               for (int h = 0; h < 2; ++h)
 #pragma unroll
@@ -258,8 +269,9 @@ __global__ __launch_bounds__(C::kThreads) void scores_kernel(ScoreArgs p) {
                   unsigned a0 = pack_h2(e[h][4 * q], e[h][4 * q + 1]), a1 = pack_h2(e[h][4 * q + 2], e[h][4 * q + 3]);
                   unsigned b0 = pack_h2(e[h][4 * q + 4], e[h][4 * q + 5]), b1 = pack_h2(e[h][4 * q + 6], e[h][4 * q + 7]);
                   swap_quads(a0, a1, b0, b1);
-                  if (i < p.n) *(uint4*)(o + h * 32 + 8 * q) = make_uint4(a0, a1, b0, b1);
+                  turn.put(l & 31, h * 4 + q + hi, make_uint4(a0, a1, b0, b1));
                 }
+              store_rows(turn, (char*)p.e + (i0 + j * 32) * p.ld * 2 + vg * 2LL, p.ld * 2, p.n - i0 - j * 32);
             }
           }
         }
@@ -916,7 +928,7 @@ __device__ __forceinline__ bool grad_item(const GradArgs& p, int j, int& id, int
 template <class C, int kLA, int kLB, typename T>
 __global__ __launch_bounds__(C::kThreads) void grad_kernel(GradArgs p) {
   const int wave = threadIdx.x >> 6, l = threadIdx.x & 63, hi = l >> 5;
-  gemm_tiles<C, kLA, kLB>(
+  gemm_tiles<C, kLA, kLB, false>(
       p.a, p.b, p.ka, p.kb,
       [&](int j, int& m0, int& n0, int& kt0, int& nkt) {
         int id, run, tm, tn;
@@ -927,7 +939,7 @@ __global__ __launch_bounds__(C::kThreads) void grad_kernel(GradArgs p) {
         kt0 = k0 / C::kBK, nkt = (k1 - k0 + C::kBK - 1) / C::kBK;
         return true;
       },
-      [&](int j, int m0, int n0, f32x16(&acc)[C::kFM][C::kFN]) {
+      [&](int j, int m0, int n0, f32x16(&acc)[C::kFM][C::kFN], const Turn&) {
         int id, run;
         grad_item(p, j, id, run);
         const int mw = m0 + (wave / C::kWN) * C::kFM * 32, nw = n0 + (wave % C::kWN) * C::kFN * 32;

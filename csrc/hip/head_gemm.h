@@ -170,13 +170,31 @@ struct TileCfg {
   static constexpr unsigned kLds = S * kStageBytes;
 };
 
+// A wave's 4 KB of LDS to turn 32 rows of 128 bytes: lanes put 16-byte chunk c of their row, then take whole rows, eight
+// per step, so that a store instruction covers full 128-byte lines. Against 32-byte pieces straight from the accumulators:
+// fp32 scores of 4096 x 65536 at K = 1024 735 -> 668 us, E of 8192 x 131072 at K = 4096 -0.8 %; the gradients' bf16 stores
+// did not gain (dw of 131072 x 4096 7.03 -> 7.17 ms) and stay direct.
+struct Turn {
+  typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
+  typedef __attribute__((address_space(3))) u32x4 l16;
+  unsigned at;
+  __device__ __forceinline__ void put(int row, int c, uint4 v) const {
+    *(l16*)(uintptr_t)(at + row * 128 + ((c ^ (row & 7)) << 4)) = u32x4{v.x, v.y, v.z, v.w};
+  }
+  __device__ __forceinline__ uint4 take(int row, int c) const {
+    const u32x4 v = *(const l16*)(uintptr_t)(at + row * 128 + ((c ^ (row & 7)) << 4));
+    return make_uint4(v.x, v.y, v.z, v.w);
+  }
+};
+
 // One block's tiles, one after the other: tile(j, m0, n0, kt0, nkt) tells its j-th (false: no more; nkt >= 1 steps
-// of kBK from step kt0), done(j, m0, n0, acc) takes the accumulators. The DMA runs S - 1 stages ahead across
+// of kBK from step kt0), done(j, m0, n0, acc, turn) takes the accumulators, with a free stage to turn them in
+// where kTurn. The DMA runs S - 1 stages ahead across
 // the border of two tiles, so only the epilogue's own instructions stand between their products. (Its stores share the
 // counter of the DMA, which counts down in the order of issue.)
 // ka, kb: extent of K in each operand's memory, a multiple of 64 for a KC operand; both reach every step:
 // (kt0 + nkt - 1) * kBK < min(ka, kb).
-template <class C, int kLA, int kLB, class FTile, class FDone>
+template <class C, int kLA, int kLB, bool kTurn, class FTile, class FDone>
 __device__ __forceinline__ void gemm_tiles(const Operand& A, const Operand& B, long long ka, long long kb, FTile tile,
                                            FDone done) {
   extern __shared__ __align__(1024) char head_smem[];
@@ -308,7 +326,13 @@ __device__ __forceinline__ void gemm_tiles(const Operand& A, const Operand& B, l
       for (int i = 0; i < C::kFM; ++i)
 #pragma unroll
         for (int j = 0; j < C::kFN; ++j) acc[i][j] += odd[i][j] + low[i][j];
-    done(j, m0, n0, acc);
+    // the stage to be filled next is free: every wave has read it (last barrier), and none fills it before the next one
+    static_assert(C::kStageBytes >= 4096u * C::kNW, "");
+    done(j, m0, n0, acc, Turn{lds + fill + wave * 4096u});
+    if (kTurn) {
+      wait_lgkm();
+      __builtin_amdgcn_s_barrier();
+    }
   }
   wait_vm<0>();  // no DMA outlives the block
 }
