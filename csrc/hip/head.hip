@@ -109,8 +109,7 @@ __global__ __launch_bounds__(256) void pack_kernel(const T* __restrict__ src, lo
 // ------------------------------------------------------------------ scores
 struct ScoreArgs {
   Operand w, x;
-  int K;              // d in whole 64s
-  int kw;             // extent of w's rows: K, or d where w is read in place (x is zero from d to K)
+  int kw, kx;         // columns of w and x: K of packed ones, d of those read in place
   int V, n;
   int nm, nn;         // tiles
   const void* bias;   // element type of the inputs
@@ -179,13 +178,13 @@ __global__ __launch_bounds__(C::kThreads) void scores_kernel(ScoreArgs p) {
   static_assert(C::kFM % 2 == 0, "a wave holds whole groups");
   const int wave = threadIdx.x >> 6, l = threadIdx.x & 63, hi = l >> 5;
   gemm_tiles<C, kKC, kKC, kMode == kExpHalf || kMode == kExpFloat || kMode == kScores>(
-      p.w, p.x, p.kw, p.K,
+      p.w, p.x, p.kw, p.kx,
       [&](int j, int& m0, int& n0, int& kt0, int& nkt) {
         const int id = item_of(j, p.nm * p.nn);
         if (id < 0) return false;
         int tm, tn;
         order_of(id, p.nm, p.nn, tm, tn);
-        m0 = tm * C::kBM, n0 = tn * C::kBN, kt0 = 0, nkt = p.K / C::kBK;
+        m0 = tm * C::kBM, n0 = tn * C::kBN, kt0 = 0, nkt = (min(p.kw, p.kx) + C::kBK - 1) / C::kBK;
         return true;
       },
       [&](int, int m0, int n0, f32x16(&acc)[C::kFM][C::kFN], const Turn& turn) {
@@ -1672,8 +1671,8 @@ static void scores(const HeadIn& h, const HeadPlan& p, const HeadOps& o, long lo
   ScoreArgs a = {};
   a.w = o.w;
   a.x = rows_from(o.x, r0, rows);
-  a.K = (int)p.kp;
   a.kw = (int)(p.pack_w ? p.kp : h.d);
+  a.kx = (int)(p.pack_x ? p.kp : h.d);
   a.V = (int)h.V;
   a.n = (int)rows;
   a.bias = bias;

@@ -69,14 +69,20 @@ struct Side {
   const char* base;
   long long rem;                // bytes to the operand's end
   unsigned koff;                // KC: bytes along K
+  unsigned tail;                // KC: what puts this lane's piece of the last K step out of bounds if it lies past K
   long long step, plane;
 
   static __device__ __forceinline__ int swz(int row) { return ((row & 3) | (((row >> 3) & 1) << 2)) & (kUnits - 1); }
 
   // lane constants
-  __device__ __forceinline__ void init(const Operand& o, int wave, int frag0, unsigned lds) {
+  __device__ __forceinline__ void init(const Operand& o, long long K, int wave, int frag0, unsigned lds) {
     const int l = threadIdx.x & 63;
+    tail = 0;
     if (kL == kKC) {
+      // (the chunk a lane takes of its row is the same in all its loads: their rows differ by multiples of 16)
+      static_assert((kNW * kRpi) % 16 == 0, "");
+      const int last = (int)(K % kBK), c = (l & (kCh - 1)) ^ swc(wave * kRpi + l / kCh);
+      if (last && c * 8 >= last) tail = 0x80000000u;
 #pragma unroll
       for (int i = 0; i < kLoads; ++i) {
         const int row = (i * kNW + wave) * kRpi + l / kCh;
@@ -120,7 +126,7 @@ struct Side {
   // the host), so K is the scalar offset; a KS operand may be longer than 2^32 bytes, so K moves the base.
   struct Src {
     i32x4 d;
-    unsigned soff;
+    unsigned soff, past;
   };
   // the next K step
   __device__ __forceinline__ void advance() {
@@ -131,7 +137,7 @@ struct Side {
       rem -= step;
     }
   }
-  __device__ __forceinline__ Src src(int pl, bool some) const {
+  __device__ __forceinline__ Src src(int pl, bool some, bool last) const {
     const unsigned long long a = (unsigned long long)(base + pl * plane);
     const unsigned hi = (unsigned)((unsigned long long)rem >> 32), lo = (unsigned)rem;
     Src s;
@@ -141,11 +147,12 @@ struct Side {
     s.d[2] = __builtin_amdgcn_readfirstlane(!some || (int)hi < 0 ? 0 : hi || lo > 0x7fffffffu ? 0x7fffffff : (int)lo);
     s.d[3] = 0x00020000;
     s.soff = kL == kKC ? __builtin_amdgcn_readfirstlane(koff) : 0u;
+    s.past = last ? tail : 0u;
     return s;
   }
   // this wave's i-th piece of the stage at LDS offset `so`
   __device__ __forceinline__ void issue(int i, const Src& s, unsigned so) const {
-    dma16(voff[i], s.d, s.soff, __builtin_amdgcn_readfirstlane(lds0 + so + i * kNW * 1024));
+    dma16(kL == kKC ? voff[i] + s.past : voff[i], s.d, s.soff, __builtin_amdgcn_readfirstlane(lds0 + so + i * kNW * 1024));
   }
 
   __device__ __forceinline__ bf16x8 frag(int b, int s, unsigned so) const {
@@ -192,8 +199,9 @@ struct Turn {
 // where kTurn. The DMA runs S - 1 stages ahead across
 // the border of two tiles, so only the epilogue's own instructions stand between their products. (Its stores share the
 // counter of the DMA, which counts down in the order of issue.)
-// ka, kb: extent of K in each operand's memory, a multiple of 64 for a KC operand; both reach every step:
-// (kt0 + nkt - 1) * kBK < min(ka, kb).
+// ka, kb: extent of K in each operand's memory, a multiple of 8 for a KC operand; both reach every step:
+// (kt0 + nkt - 1) * kBK < min(ka, kb). Past it an operand counts as zero, whatever its memory holds there (a KC operand
+// whose K is no multiple of kBK: in the last step of every tile, so its tiles all run to the end of K).
 template <class C, int kLA, int kLB, bool kTurn, class FTile, class FDone>
 __device__ __forceinline__ void gemm_tiles(const Operand& A, const Operand& B, long long ka, long long kb, FTile tile,
                                            FDone done) {
@@ -206,10 +214,10 @@ __device__ __forceinline__ void gemm_tiles(const Operand& A, const Operand& B, l
   typedef Side<kLB, C::kBN, C::kNW, C::kFN, C::kBK> SideB;
   SideA a;
   SideB b;
-  a.init(A, wave, wm * C::kFM, lds);
+  a.init(A, ka, wave, wm * C::kFM, lds);
   constexpr int P = C::kPlanes, kTerms = P == 1 ? 1 : 6;
   static_assert(P == 1 || P == 3, "");
-  b.init(B, wave, wn * C::kFN, lds + P * SideA::kBytes);
+  b.init(B, kb, wave, wn * C::kFN, lds + P * SideA::kBytes);
   constexpr int kPlaneLoads = SideA::kLoads + SideB::kLoads, kLoads = P * kPlaneLoads;
 
   // the DMA's place in the stream of stages
@@ -233,8 +241,8 @@ __device__ __forceinline__ void gemm_tiles(const Operand& A, const Operand& B, l
   auto next = [&]() {  // (past the last stage: zeros that nothing reads, so that every step issues the same loads)
 #pragma unroll
     for (int p = 0; p < P; ++p) {
-      da[p] = a.src(p, some);
-      db[p] = b.src(p, some);
+      da[p] = a.src(p, some, ikt + 1 == inkt);
+      db[p] = b.src(p, some, ikt + 1 == inkt);
     }
     a.advance();
     b.advance();

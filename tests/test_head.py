@@ -205,7 +205,7 @@ def _refusals(dev):
         (ValueError, lambda: di(x, w, idx[:3], tl[:3])), (ValueError, lambda: di(x, w, idx, tl[:, :2])),
         (ValueError, lambda: di(x, w, idx[:, :0], tl[:, :0])), (ValueError, lambda: di(x, w, idx, tl.bfloat16())),
         (TypeError, lambda: di(x, w, idx.float(), tl)), (ValueError, lambda: di(x, w, idx, tl, temperature=0.0)),
-        (ValueError, lambda: di(x, w, idx, tl, temperature=float("nan"))), (ValueError, lambda: di(x, w, idx, tl, top_lse=tl)),
+        (ValueError, lambda: di(x, w, idx, tl, temperature=float("nan"))), (ValueError, lambda: di(x, w, idx, tl, temperature=1e-30)), (ValueError, lambda: di(x, w, idx, tl, top_lse=tl)),
         (ValueError, lambda: di(x, w, idx.repeat(1, 100), tl.repeat(1, 100))),
         (ValueError, lambda: tk(x, w, 0)), (ValueError, lambda: tk(x, w, 7)), (ValueError, lambda: tk(x, w.repeat(100, 1), 257)),
         (ValueError, lambda: tk(x, w, 2, temperature=-1.0)),
@@ -277,6 +277,66 @@ def test_loss_strides(cuda, dtype):
     one = x[:1].expand(70, 64)
     r = head.softmax_head_loss(one, w, y)
     Ref(one, w, *label_targets(y)).check(r)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", BOTH)
+@pytest.mark.parametrize("n", [5, 150, 300])
+@pytest.mark.parametrize("d", [8, 72, 200])
+def test_loss_rows_inside_a_wider_buffer(cuda, dtype, n, d):
+    """What stands between the rows (NaN) stays out, also where a row ends inside a step of the product."""
+    x, w, y, b = make(n, d, 333, dtype, cuda, bias=True)
+    bx = torch.full((n + 1, d + 24), float("nan"), dtype=dtype, device=cuda)
+    bw = torch.full((334, d + 8), float("nan"), dtype=dtype, device=cuda)
+    bx[:n, :d], bw[:333, :d] = x, w
+    for x2, w2 in ((bx[:n, :d], bw[:333, :d]), (x, bw[:333, :d]), (bx[:n, :d], w)):
+        r = head.softmax_head_loss(x2, w2, y, bias=b)
+        Ref(x, w, *label_targets(y), bias=b).check(r, db=True)
+        v, c, _ = head.head_topk(x2, w2, 4, bias=b)
+        assert torch.equal(c, topk_ref(x, w, b, 1.0, 4)[1])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", BOTH)
+def test_no_rows(cuda, dtype):
+    x, w, y, b = make(3, 8, 5, dtype, cuda, bias=True)
+    r = head.softmax_head_loss(x[:0], w, y[:0], bias=b)
+    assert r.loss.shape == r.lse.shape == (0,) and r.dx.shape == (0, 8) and bool((r.dw == 0).all()) and bool((r.db == 0).all())
+    r = head.distill_head_loss(x[:0], w, y[:0, None], torch.zeros(0, 1, device=cuda))
+    assert r.dw.shape == (5, 8) and bool((r.dw == 0).all())
+    v, c, l = head.head_topk(x[:0], w, 2)
+    assert v.shape == c.shape == (0, 2) and l.shape == (0,)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype,V", [(torch.bfloat16, 300001), (torch.float32, 150001)])
+def test_weights_beyond_32_bit_offsets(cuda, dtype, V):
+    """w of more than 2^32 bytes: every class's score and gradient, in 64 bits in pieces on the GPU."""
+    d, n = 8192, 3
+    g = torch.Generator(device=cuda).manual_seed(3)
+    w = torch.empty(V, d, dtype=dtype, device=cuda)
+    for a in range(0, V, 50000):
+        w[a:a + 50000] = (torch.randn(min(50000, V - a), d, generator=g, device=cuda) * (2.0 / d ** 0.5)).to(dtype)
+    x = torch.randn(n, d, generator=g, device=cuda).to(dtype)
+    y = torch.tensor([V - 1, 7, V // 2], device=cuda)
+    r = head.softmax_head_loss(x, w, y)
+    v, c, l = head.head_topk(x, w, 5)
+    z = torch.cat([x.double() @ w[a:a + 20000].double().t() for a in range(0, V, 20000)], 1)
+    lse = torch.logsumexp(z, 1)
+    rv, rc = z.sort(dim=1, descending=True, stable=True)
+    assert torch.equal(c, rc[:, :5])
+    # |x||w| sums to at most ~ 2 d 2 / sqrt(d) = 362: scores off by (6 d + 32) 2^-24 * 362 at worst, in practice far less
+    near(r.lse, lse.cpu(), torch.full((n,), 1e-3, dtype=torch.float64), "lse")
+    near(r.loss, (lse - z.gather(1, y[:, None])[:, 0]).cpu(), torch.full((n,), 2e-3, dtype=torch.float64), "loss")
+    D = (z - lse[:, None]).exp()
+    D[torch.arange(n, device=cuda), y] -= 1
+    step = 2 * (H if dtype == torch.bfloat16 else 2e-3)  # D's rounding, or the scores' bound
+    dx = sum(D[:, a:a + 20000] @ w[a:a + 20000].double() for a in range(0, V, 20000))
+    bound = sum(D[:, a:a + 20000].abs() @ w[a:a + 20000].double().abs() for a in range(0, V, 20000)) * step
+    near(r.dx, dx.cpu(), bound.cpu(), "dx")
+    for a in (0, 65500, 131040, V - 70):
+        dw = D[:, a:a + 70].t() @ x.double()
+        near(r.dw[a:a + 70], dw.cpu(), (step * (D[:, a:a + 70].abs().t() @ x.double().abs()) + 2 * H * dw.abs() + 1e-12).cpu(), "dw")
 
 
 @pytest.mark.gpu
@@ -427,7 +487,8 @@ def topk_ref(x, w, bias, T, k):
 @pytest.mark.gpu
 @pytest.mark.parametrize("dtype", BOTH)
 @pytest.mark.parametrize("n,d,V,k", [(1, 1, 1, 1), (1, 64, 70, 70), (2, 33, 129, 1), (7, 333, 2003, 5), (33, 64, 640, 9), (65, 128, 5000, 64),
-                                     (3, 64, 30000, 256), (130, 200, 300, 256), (1, 512, 40001, 16)])
+                                     (3, 64, 30000, 256), (130, 200, 300, 256), (1, 512, 40001, 16), (5, 64, 1500, 256),
+                                     (260, 64, 150001, 7), (2, 16, 600000, 30)])
 def test_topk_sizes(cuda, dtype, n, d, V, k):
     x, w, _, b = make(n, d, V, dtype, cuda, bias=k % 2 == 1)
     T = 1.5 if n % 2 else 1.0

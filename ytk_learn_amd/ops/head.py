@@ -17,9 +17,8 @@ current stream of x's device without a host synchronisation, in a workspace of i
 allocator), so calls on several streams and captured graphs do not share memory. Results are
 bitwise reproducible.
 
-x of rows that take part, w and bias are finite; a class is switched off by a bias of -inf or the type's lowest value.
-(An infinity or NaN in a row of w reaches that class's scores and, where d is no multiple of 64, may make those of the
-class before it NaN.)
+x of rows that take part and w are finite; a class is switched off by a bias of -inf or the type's lowest value, and at
+least one class is on.
 """
 from __future__ import annotations
 
@@ -59,8 +58,8 @@ def _check(x, w, bias, temperature, **rows):
         raise ValueError(f"class head: 1 to {MAX_DIM} features and classes expected, got d = {d}, V = {V}")
     if bias is not None and (tuple(bias.shape) != (V,) or bias.dtype != w.dtype):
         raise ValueError(f"class head: bias [{V}] of type {w.dtype} expected")
-    if not (temperature > 0.0 and temperature < float("inf")):
-        raise ValueError("class head: the temperature is a positive number")
+    if not 1e-6 <= temperature <= 1e6:
+        raise ValueError("class head: a temperature from 1e-6 to 1e6 expected")
     for name, t in dict(w=w, bias=bias, **rows).items():
         if t is not None and t.device != x.device:
             raise ValueError(f"class head: {name} is on {t.device}, x on {x.device}")
@@ -68,9 +67,9 @@ def _check(x, w, bias, temperature, **rows):
         raise ValueError("class head: tensors on the GPU or the CPU expected")
 
 
-def _aligned(t, cols):
-    """Whether the products can read the rows in place: 16-byte pieces, a multiple of ``cols`` columns."""
-    return int(t.dtype == torch.bfloat16 and t.stride(1) == 1 and t.shape[1] % cols == 0 and t.stride(0) % 8 == 0
+def _aligned(t):
+    """Whether the products can read the rows in place: whole, aligned 16-byte pieces."""
+    return int(t.dtype == torch.bfloat16 and t.stride(1) == 1 and t.shape[1] % 8 == 0 and t.stride(0) % 8 == 0
                and t.stride(0) >= t.shape[1] and t.data_ptr() % 16 == 0 and t.stride(0) <= 1 << 21)
 
 
@@ -89,7 +88,7 @@ def _operands(x, w):
 def _params(x, w, k, idx64, ignore, base, mode, want_dx, want_dw, bias):
     return [x.shape[0], x.shape[1], w.shape[0], k, int(x.dtype == torch.float32), x.stride(0), x.stride(1), w.stride(0),
             w.stride(1), idx64, ignore, int(base), mode, int(want_dx), int(want_dw), int(bias is not None),
-            PIECE_BYTES, _aligned(x, 64), _aligned(w, 8)]
+            PIECE_BYTES, _aligned(x), _aligned(w)]
 
 
 def _on(dev):
