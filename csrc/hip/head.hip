@@ -1,5 +1,5 @@
 // Softmax class head over many classes (gfx950): z = (x w^T + b) / T for rows x [n, d] and classes w [V, d],
-// without ever holding n x V scores.
+// in pieces of rows that bound what is held of the n x V scores.
 //
 //   loss:    per-row targets q_j on classes v_j (one label, or a teacher's k best), lse = log sum_v e^z,
 //            loss = g T^2 sum_j q_j (log q_j + lse - z_j);  D = g T (s p - q), s = sum_j q_j, p = e^(z - lse);
@@ -14,8 +14,8 @@
 //   3. row_kernel      lse from the groups, loss, and the row's coefficients
 //   4. dscore_kernel   E -> D in place (fp32: three bf16 planes), bias gradient partials
 //   5. grad kernels    dx = D w, dw = D^T x
-// The scores are computed once: 6 n d V operations for a step, against 8 n d V where the scores are computed
-// again for the gradient.
+// The scores are computed once: 6 n d V operations for a step, against 8 n d V where pieces of the classes compute
+// them again for the gradient. (8192 x 4096 x 131072: the D pass over 2 GiB takes 0.88 ms, a fourth product 7.0.)
 #include "head_gemm.h"
 
 #include <algorithm>

@@ -9,8 +9,8 @@ Device path: S = X W and G = X^T D as the segmented SpMM kernel (J = K-1 columns
 per-row loss / prediction / D epilogue is one fused HIP pass (``ops.blas.multiclass_row_loss``,
 every multiclass loss, K <= 64) and fp64 torch otherwise.
 ``dense_head = true`` (extension, softmax with one class per row): dense rows X [n, F] against the
-F x (K-1) weights through ``ops.head.softmax_head_loss``, for many classes: no n x K scores,
-probabilities or score gradients are held.
+F x (K-1) weights through ``ops.head.softmax_head_loss``, for many classes: a bounded piece
+of the n x K exponentials is held at a time, no probabilities.
 Note: y_sampling keys on the first label value (a class id line); K-vector label lines are
 not sampled by class.
 """

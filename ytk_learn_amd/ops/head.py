@@ -1,6 +1,7 @@
 """Softmax class head over many classes (``csrc/hip/head.hip``) + torch CPU path.
 
-Scores z = (x w^T + bias) / T of rows ``x`` [n, d] against classes ``w`` [V, d]; the n x V scores are never held.
+Scores z = (x w^T + bias) / T of rows ``x`` [n, d] against classes ``w`` [V, d]. Rows are taken in pieces: at most
+``PIECE_BYTES`` of exponentials (or scores, head_topk) live at a time, however many rows and classes there are.
 
 * :func:`softmax_head_loss`: per-row softmax cross entropy with the gradients of x, w and bias. With
   ``base_class`` one more class has score 0 and no weights (index V): the multiclass linear model's convention
@@ -15,7 +16,7 @@ float32 or bfloat16 (x, w and bias alike); any strides. float32 products run as 
 gradient D = p - q is rounded to bf16 once before the two gradient products. Everything runs on the
 current stream of x's device without a host synchronisation, in a workspace of its own per call (torch's
 allocator), so calls on several streams and captured graphs do not share memory. Results are
-bitwise reproducible.
+bitwise reproducible. Gradients are returned; nothing is recorded for autograd.
 
 x of rows that take part and w are finite; a class is switched off by a bias of -inf or the type's lowest value, and at
 least one class is on.
@@ -198,6 +199,7 @@ def head_topk(x: torch.Tensor, w: torch.Tensor, k: int, bias: Optional[torch.Ten
 
 
 # ------------------------------------------------------------------ CPU path (64 bits, rounded once)
+@torch.no_grad()
 def _cpu_loss(x, w, idx, tl, tlse, bias, weight, T, ignore, base, mode, want_dx, want_dw):
     n, V = x.shape[0], w.shape[0]
     xd, wd, idx = x.double(), w.double(), idx.long()
@@ -237,6 +239,7 @@ def _cpu_loss(x, w, idx, tl, tlse, bias, weight, T, ignore, base, mode, want_dx,
     return HeadLoss(loss.float(), lse.float(), dx, dw, db)
 
 
+@torch.no_grad()
 def _cpu_topk(x, w, k, bias, T):
     z = x.double() @ w.double().t()
     if bias is not None:
