@@ -118,7 +118,18 @@ struct ScoreArgs {
   void* e;            // E [n][ld] (fp16 or fp32) or null
   float* z;           // scores [n][ld] or null
   long long ld;
+  const void* label;  // [n] or null: each row's label's score, less its group's m, goes to zt in the unit of the stats
+  int idx64;
+  float* zt;
 };
+
+__device__ __forceinline__ long long index_at(const void* p, int is64, long long i) {
+  return is64 ? ((const long long*)p)[i] : (long long)((const int*)p)[i];
+}
+__device__ __forceinline__ int class_at(const void* p, int is64, long long i, int V) {
+  const long long v = index_at(p, is64, i);
+  return v >= 0 && v < V ? (int)v : -1;
+}
 
 // lanes l and l + 32 hold rows 8q .. 8q+3 and 8q+4 .. 8q+7 of a 32-row block: exchange halves so that lane l has
 // all 8 values of quad pair 2p and lane l + 32 all 8 of 2p + 1 (16-byte stores of 16-bit values)
@@ -189,6 +200,12 @@ __global__ __launch_bounds__(C::kThreads) void scores_kernel(ScoreArgs p) {
       },
       [&](int, int m0, int n0, f32x16(&acc)[C::kFM][C::kFN], const Turn& turn) {
         const int v0 = m0 + (wave / C::kWN) * C::kFM * 32, i0 = n0 + (wave % C::kWN) * C::kFN * 32;
+        int label[C::kFN];
+#pragma unroll
+        for (int j = 0; j < C::kFN; ++j) {
+          const int i = i0 + j * 32 + (l & 31);
+          label[j] = kMode != kScores && p.label && i < p.n ? class_at(p.label, p.idx64, i, p.V) : -1;
+        }
 #pragma unroll
         for (int g = 0; g < C::kFM / 2; ++g) {
           const int vg = v0 + g * kGroup;
@@ -230,6 +247,18 @@ __global__ __launch_bounds__(C::kThreads) void scores_kernel(ScoreArgs p) {
               for (int r = 0; r < 16; ++r) mx = fmaxf(mx, acc[2 * g + h][j][r]);
             const float m = fmaxf(mx, __shfl_xor(mx, 32, 64)) * c;
             const float m0 = m == -INFINITY ? 0.0f : m;
+            if (kMode != kScores && __any(label[j] >= vg && label[j] < vg + kGroup)) {
+              // the very score that is part of lse: a confident row's loss is the difference of the two
+              const int at = label[j] - vg - 4 * hi;
+              float zl = 0.0f;
+              bool mine = false;
+#pragma unroll
+              for (int h = 0; h < 2; ++h)
+#pragma unroll
+                for (int r = 0; r < 16; ++r)
+                  if (at == h * 32 + 8 * (r >> 2) + (r & 3)) zl = acc[2 * g + h][j][r], mine = true;
+              if (mine) p.zt[i] = fmaf(zl, c, -m0);
+            }
             if (kMode == kScores)
 #pragma unroll
               for (int h = 0; h < 2; ++h) {
@@ -295,6 +324,9 @@ struct FewArgs {
   float2* stats;
   float* e;        // E or scores [n][ld], or null
   long long ld;
+  const void* label;
+  int idx64;
+  float* zt;
 };
 
 // 4 floats from column c; zero past the end
@@ -369,6 +401,7 @@ __global__ __launch_bounds__(256, 2) void scores_few_kernel(FewArgs p) {
   if (!few_sum<kNT>(acc, sum)) return;
   // lane: row l % 16 of the wave's tile, classes vg + 16 t + 4 (l / 16) + r
   const int row = i0 + wave * 16 + r16;
+  const int label = kMode != kScores && p.label && row < p.n ? class_at(p.label, p.idx64, row, p.V) : -1;
   float z[4][4], m = -INFINITY;
 #pragma unroll
   for (int t = 0; t < 4; ++t)
@@ -388,7 +421,11 @@ __global__ __launch_bounds__(256, 2) void scores_few_kernel(FewArgs p) {
   for (int t = 0; t < 4; ++t) {
     if (kMode == kScores && row < p.n) *(float4*)(o + t * 16) = make_float4(z[t][0], z[t][1], z[t][2], z[t][3]);
 #pragma unroll
-    for (int r = 0; r < 4; ++r) s += z[t][r] = exp_of<true>(z[t][r] - m0);
+    for (int r = 0; r < 4; ++r) {
+      z[t][r] -= m0;
+      if (kMode != kScores && vg + t * 16 + g4 * 4 + r == label) p.zt[row] = z[t][r];
+      s += z[t][r] = exp_of<true>(z[t][r]);
+    }
     if (kMode == kExpFloat && row < p.n) *(float4*)(o + t * 16) = make_float4(z[t][0], z[t][1], z[t][2], z[t][3]);
   }
   s += __shfl_xor(s, 16, 64);
@@ -526,13 +563,9 @@ struct TargetArgs {
   long long xrs, xcs, wrs, wcs;
   const void* idx;     // [n][k], int64 or int32
   int idx64, k, n, d, V, vec;
-  float inv_t;
+  float unit;          // 1 / T in the unit of the stats
   float* zt;           // [n][k]
 };
-
-__device__ __forceinline__ long long index_at(const void* p, int is64, long long i) {
-  return is64 ? ((const long long*)p)[i] : (long long)((const int*)p)[i];
-}
 
 // 16 bytes of a row as fp32
 __device__ __forceinline__ void unpack16(const uint4& u, float (&v)[4]) {
@@ -621,7 +654,7 @@ __global__ __launch_bounds__(256) void target_kernel(TargetArgs p) {
   if (l == 0) {
 #pragma unroll
     for (int i = 0; i < kW; ++i)
-      if (i < m) p.zt[first + i] = v[i] < 0 ? 0.0f : (s[i] + (p.bias ? Elem<T>::get((const T*)p.bias, v[i]) : 0.0f)) * p.inv_t;
+      if (i < m) p.zt[first + i] = v[i] < 0 ? 0.0f : (s[i] + (p.bias ? Elem<T>::get((const T*)p.bias, v[i]) : 0.0f)) * p.unit;
   }
 }
 
@@ -633,7 +666,8 @@ struct RowArgs {
   const void* idx;
   int idx64;
   long long ignore;
-  const float *tl, *tlse, *weight, *zt;
+  const float *tl, *tlse, *weight;
+  float* zt;
   float temp;
   float *lse, *loss;    // outputs
   float* coef;          // [n] g T s  (0: the row has no gradient)
@@ -687,8 +721,8 @@ __global__ __launch_bounds__(256) void row_kernel(RowArgs p) {
   }
   if (t < p.rb && row < p.n) {
     if (p.norm) p.norm[row] = make_float2(sm[t], 1.0f / ss[t]);
-    sm[t] = (kB2 ? sm[t] * 0.6931471805599453f : sm[t]) + logf(ss[t]);
-    p.lse[row] = sm[t];
+    ss[t] = logf(ss[t]);
+    p.lse[row] = (kB2 ? sm[t] * 0.6931471805599453f : sm[t]) + ss[t];
   }
   __syncthreads();
   if (!p.loss) return;
@@ -697,7 +731,7 @@ __global__ __launch_bounds__(256) void row_kernel(RowArgs p) {
   for (int r = wave; r < p.rb; r += 4) {
     const long long i = (long long)blockIdx.x * p.rb + r;
     if (i >= p.n) break;
-    const float lse = sm[r], g = p.weight ? p.weight[i] : 1.0f;
+    const float mx_row = sm[r], log_s = ss[r], g = p.weight ? p.weight[i] : 1.0f;
     float norm = 0.0f;
     if (p.mode == 1) {  // renormalise the list: log sum e^(t/T) over its entries
       float mx = -INFINITY;
@@ -725,7 +759,17 @@ __global__ __launch_bounds__(256) void row_kernel(RowArgs p) {
         } else {
           const float lq = p.mode == 0 ? 0.0f : p.tl[i * p.k + j] / p.temp - norm;
           q = p.mode == 0 ? 1.0f : expf(lq);
-          if (q > 0.0f || q != q) term = q * (lq + lse - p.zt[i * p.k + j]);
+          if (q > 0.0f || q != q) {
+            // log q + lse - z, the maximum's part first: it cancels exactly where z is the maximum. A label's score is
+            // kept relative to its group's maximum as its exponential in s is, and from here on to the row's.
+            float up = mx_row - (v < p.V ? p.zt[i * p.k + j] : 0.0f);
+            if (p.mode == 0 && v < p.V) {
+              const float mg = p.stats[v / kGroup * p.n + i].x, rel = p.zt[i] + ((mg == -INFINITY ? 0.0f : mg) - mx_row);
+              p.zt[i] = rel;
+              up = -rel;
+            }
+            term = q * (lq + ((kB2 ? up * 0.6931471805599453f : up) + log_s));
+          }
         }
       }
       if (p.q) p.q[i * p.k + j] = q * g * p.temp;
@@ -754,6 +798,7 @@ struct DArgs {
   long long ld, plane;
   float* part;          // [row blocks][ld] bias gradient partials, or null
   int rw;               // rows per wave
+  int zt_rel;           // zt is relative to the row's maximum (labels)
   int keep32;           // fp32 inputs: D also in fp32, in place of E
   char* x;              // packed x of these rows, or null: rows without a gradient are cleared in it before they meet D
   long long xpitch, xplane;
@@ -817,7 +862,8 @@ __global__ __launch_bounds__(256) void dscore_kernel(DArgs p) {
             for (unsigned long long h = __ballot(at >= 0); h; h &= h - 1) {
               const int bit = __builtin_ctzll(h), vb = __builtin_amdgcn_readlane(at, bit);
               const long long e = i * p.k + j0 + bit;
-              const float x = pass != 0 ? p.q[e] : co * (kF32 ? exp_of<true>(p.zt[e] - nr[b].x) : __builtin_amdgcn_exp2f(p.zt[e] * kLog2e - nr[b].x));
+              const float rel = p.zt_rel ? p.zt[e] : p.zt[e] - nr[b].x;
+              const float x = pass != 0 ? p.q[e] : co * (kF32 ? exp_of<true>(rel) : __builtin_amdgcn_exp2f(rel));
 #pragma unroll
               for (int u = 0; u < 8; ++u)
                 if (vb == l * 8 + u) d[b][u] = pass == 0 ? x : d[b][u] - x;
@@ -1613,8 +1659,9 @@ static void scores_few_n(const FewArgs& a, int mode, hipStream_t s) {
 }
 
 static void scores_few(const HeadIn& h, const HeadPlan& p, const void* x, const void* w, const void* bias, float temp, char* ws, int mode,
-                       hipStream_t s) {
+                       const void* label, hipStream_t s) {
   FewArgs a = {};
+  a.label = label, a.idx64 = (int)h.idx64, a.zt = (float*)(ws + p.o_zt);
   a.w = (const float*)w, a.x = (const float*)x, a.bias = (const float*)bias;
   a.wrs = h.wrs, a.xrs = h.xrs;
   a.V = (int)h.V, a.n = (int)h.n, a.d = (int)h.d;
@@ -1667,8 +1714,9 @@ static void dw_few(const HeadIn& h, const HeadPlan& p, const void* x, char* ws, 
 }
 
 static void scores(const HeadIn& h, const HeadPlan& p, const HeadOps& o, long long r0, long long rows, const void* bias, float temp,
-                   char* ws, int mode, hipStream_t s) {
+                   char* ws, int mode, const void* label, hipStream_t s) {
   ScoreArgs a = {};
+  a.label = label, a.idx64 = (int)h.idx64, a.zt = (float*)(ws + p.o_zt);
   a.w = o.w;
   a.x = rows_from(o.x, r0, rows);
   a.kw = (int)(p.pack_w ? p.kp : h.d);
@@ -1740,10 +1788,6 @@ extern "C" void ytk_head_loss(const uintptr_t* ptrs, const long long* lp, double
   for (long long r0 = 0; r0 < h.n; r0 += p.piece) {
     const long long rows = std::min(p.piece, h.n - r0);
     const bool first = r0 == 0, last = r0 + rows == h.n;
-    if (p.few)
-      scores_few(h, p, x, w, bias, temp, ws, p.grads ? kExpFloat : kStatsFloat, s);
-    else
-      scores(h, p, o, r0, rows, bias, temp, ws, h.f32 ? (p.grads ? kExpFloat : kStatsFloat) : p.grads ? kExpHalf : kStatsOnly, s);
     TargetArgs t = {};
     t.x = x + r0 * h.xrs * el;
     t.w = w;
@@ -1752,12 +1796,19 @@ extern "C" void ytk_head_loss(const uintptr_t* ptrs, const long long* lp, double
     t.idx = idx + r0 * h.k * (h.idx64 ? 8 : 4);
     t.idx64 = (int)h.idx64;
     t.k = (int)h.k, t.n = (int)rows, t.d = (int)h.d, t.V = (int)h.V, t.vec = dots_vec(h, x, w);
-    t.inv_t = 1.0f / temp;
+    t.unit = h.f32 ? 1.0f / temp : 1.0f / temp * kLog2e;
     t.zt = (float*)(ws + p.o_zt);
-    if (h.f32)
-      targets<float>(t, s);
+    const void* label = h.mode == 0 ? t.idx : nullptr;
+    if (p.few)
+      scores_few(h, p, x, w, bias, temp, ws, p.grads ? kExpFloat : kStatsFloat, label, s);
     else
-      targets<__bf16>(t, s);
+      scores(h, p, o, r0, rows, bias, temp, ws, h.f32 ? (p.grads ? kExpFloat : kStatsFloat) : p.grads ? kExpHalf : kStatsOnly, label, s);
+    if (h.mode != 0) {  // (a label's score comes from the products)
+      if (h.f32)
+        targets<float>(t, s);
+      else
+        targets<__bf16>(t, s);
+    }
     RowArgs r = {};
     r.stats = (const float2*)(ws + p.o_stats);
     r.groups = (int)p.groups, r.n = (int)rows, r.base = (int)h.base;
@@ -1780,6 +1831,7 @@ extern "C" void ytk_head_loss(const uintptr_t* ptrs, const long long* lp, double
     d.e = ws + p.o_e, d.d = (__bf16*)(ws + p.o_d), d.ld = p.ld, d.plane = rows * p.ld;
     d.part = db ? (float*)(ws + p.o_part) : nullptr;
     d.rw = p.rw;
+    d.zt_rel = h.mode == 0;
     d.keep32 = p.few;
     if (h.f32 && !p.planes_d) d.d = nullptr;
     if (h.want_dw && p.pack_x) {
@@ -1863,9 +1915,9 @@ extern "C" void ytk_head_topk(const uintptr_t* ptrs, const long long* lp, double
   for (long long r0 = 0; r0 < h.n; r0 += p.piece) {
     const long long rows = std::min(p.piece, h.n - r0);
     if (p.few)
-      scores_few(h, p, x, w, bias, (float)temp_, ws, kScores, s);
+      scores_few(h, p, x, w, bias, (float)temp_, ws, kScores, nullptr, s);
     else
-      scores(h, p, o, r0, rows, bias, (float)temp_, ws, kScores, s);
+      scores(h, p, o, r0, rows, bias, (float)temp_, ws, kScores, nullptr, s);
     RowArgs r = {};
     r.stats = (const float2*)(ws + p.o_stats);
     r.groups = (int)p.groups, r.n = (int)rows, r.V = (int)h.V;

@@ -429,6 +429,22 @@ def test_loss_larger(cuda, dtype, n, d, V):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("dtype", BOTH)
+@pytest.mark.parametrize("n", [1, 40, 300])
+def test_loss_confident_rows(cuda, dtype, n):
+    """Rows sure of their label: lse and the label's score share their error, so the loss is near 0 without the scores'
+    rounding: |dloss| <= 2 (1 - p_y) max |dz| + the rounding of the sum (1 + small: 8 u) and of the log."""
+    x, w, y, _ = make(n, 520, 700, dtype, cuda)
+    x = (x.float() + 2.5 * w[y].float()).to(dtype)
+    r = head.softmax_head_loss(x, w, y, want_dx=False, want_dw=n == 40)
+    z = x.double() @ w.double().t()
+    ref = torch.logsumexp(z, 1) - z.gather(1, y[:, None])[:, 0]
+    ez = ((6 * 520 + 20 if dtype == torch.float32 else 520 + 12) * U * (x.double().abs() @ w.double().abs().t())).amax(1)
+    assert float(ref.median()) < 0.05
+    near(r.loss, ref.cpu(), (2 * (1 - (-ref).exp()) * ez + 8 * U + 16 * U * ref).cpu(), "loss")
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", BOTH)
 def test_loss_many_rows(cuda, dtype):
     """More rows than one piece holds at most, few classes."""
     n = (1 << 21) + 777
