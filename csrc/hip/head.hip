@@ -118,7 +118,7 @@ struct ScoreArgs {
   void* e;            // E [n][ld] (fp16 or fp32) or null
   float* z;           // scores [n][ld] or null
   long long ld;
-  const void* label;  // [n] or null: each row's label's score, less its group's m, goes to zt in the unit of the stats
+  const void* label;  // [n] or null: a row's label is left out of its group; its score less the group's m (0 for -inf) goes to zt
   int idx64;
   float* zt;
 };
@@ -240,6 +240,18 @@ __global__ __launch_bounds__(C::kThreads) void scores_kernel(ScoreArgs p) {
 #pragma unroll
           for (int j = 0; j < C::kFN; ++j) {
             const int i = i0 + j * 32 + (l & 31);
+            // a row's label is taken out of its group's m and s (row_kernel adds it: a confident row's loss is the log of
+            // 1 + what the others sum to, which a sum with the label's 1 in it would round away)
+            float zl = 0.0f;
+            bool mine = false;
+            if (kMode != kScores && __any(label[j] >= vg && label[j] < vg + kGroup)) {
+              const int at = label[j] - vg - 4 * hi;
+#pragma unroll
+              for (int h = 0; h < 2; ++h)
+#pragma unroll
+                for (int r = 0; r < 16; ++r)
+                  if (at == h * 32 + 8 * (r >> 2) + (r & 3)) zl = acc[2 * g + h][j][r], acc[2 * g + h][j][r] = -INFINITY, mine = true;
+            }
             float mx = -INFINITY;
 #pragma unroll
             for (int h = 0; h < 2; ++h)
@@ -247,18 +259,7 @@ __global__ __launch_bounds__(C::kThreads) void scores_kernel(ScoreArgs p) {
               for (int r = 0; r < 16; ++r) mx = fmaxf(mx, acc[2 * g + h][j][r]);
             const float m = fmaxf(mx, __shfl_xor(mx, 32, 64)) * c;
             const float m0 = m == -INFINITY ? 0.0f : m;
-            if (kMode != kScores && __any(label[j] >= vg && label[j] < vg + kGroup)) {
-              // the very score that is part of lse: a confident row's loss is the difference of the two
-              const int at = label[j] - vg - 4 * hi;
-              float zl = 0.0f;
-              bool mine = false;
-#pragma unroll
-              for (int h = 0; h < 2; ++h)
-#pragma unroll
-                for (int r = 0; r < 16; ++r)
-                  if (at == h * 32 + 8 * (r >> 2) + (r & 3)) zl = acc[2 * g + h][j][r], mine = true;
-              if (mine) p.zt[i] = fmaf(zl, c, -m0);
-            }
+            if (kMode != kScores && mine) p.zt[i] = fmaf(zl, c, -m0);
             if (kMode == kScores)
 #pragma unroll
               for (int h = 0; h < 2; ++h) {
@@ -402,7 +403,8 @@ __global__ __launch_bounds__(256, 2) void scores_few_kernel(FewArgs p) {
   // lane: row l % 16 of the wave's tile, classes vg + 16 t + 4 (l / 16) + r
   const int row = i0 + wave * 16 + r16;
   const int label = kMode != kScores && p.label && row < p.n ? class_at(p.label, p.idx64, row, p.V) : -1;
-  float z[4][4], m = -INFINITY;
+  float z[4][4], m = -INFINITY, zl = 0.0f;
+  bool mine = false;
 #pragma unroll
   for (int t = 0; t < 4; ++t)
 #pragma unroll
@@ -410,22 +412,20 @@ __global__ __launch_bounds__(256, 2) void scores_few_kernel(FewArgs p) {
       const int v = vg + t * 16 + g4 * 4 + r;
       const float b = p.bias ? p.bias[min(v, p.V - 1)] : 0.0f;
       z[t][r] = v < p.V ? (sum[t][r] + b) * p.inv_t : -INFINITY;
+      if (v == label) zl = z[t][r], z[t][r] = -INFINITY, mine = true;  // as in scores_kernel
       m = fmaxf(m, z[t][r]);
     }
   m = fmaxf(m, __shfl_xor(m, 16, 64));
   m = fmaxf(m, __shfl_xor(m, 32, 64));
   const float m0 = m == -INFINITY ? 0.0f : m;
+  if (mine) p.zt[row] = zl - m0;
   float s = 0.0f;
   float* o = p.e + (long long)row * p.ld + vg + g4 * 4;
 #pragma unroll
   for (int t = 0; t < 4; ++t) {
     if (kMode == kScores && row < p.n) *(float4*)(o + t * 16) = make_float4(z[t][0], z[t][1], z[t][2], z[t][3]);
 #pragma unroll
-    for (int r = 0; r < 4; ++r) {
-      z[t][r] -= m0;
-      if (kMode != kScores && vg + t * 16 + g4 * 4 + r == label) p.zt[row] = z[t][r];
-      s += z[t][r] = exp_of<true>(z[t][r]);
-    }
+    for (int r = 0; r < 4; ++r) s += z[t][r] = exp_of<true>(z[t][r] - m0);
     if (kMode == kExpFloat && row < p.n) *(float4*)(o + t * 16) = make_float4(z[t][0], z[t][1], z[t][2], z[t][3]);
   }
   s += __shfl_xor(s, 16, 64);
@@ -666,20 +666,19 @@ struct RowArgs {
   const void* idx;
   int idx64;
   long long ignore;
-  const float *tl, *tlse, *weight;
-  float* zt;
+  const float *tl, *tlse, *weight, *zt;
   float temp;
   float *lse, *loss;    // outputs
   float* coef;          // [n] g T s  (0: the row has no gradient)
   float2* norm;         // [n] maximum and 1 / sum: p = e^(z - max) / sum, without the rounding of lse
-  float* q;             // [n][k] g T q_j
+  float* q;             // [n][k] g T q_j; of a label g (1 - p), all of its D
   int rb;               // rows per block (a power of two, <= 16)
 };
 
 // kB2: the maxima are in log2 units
 template <bool kB2>
 __global__ __launch_bounds__(256) void row_kernel(RowArgs p) {
-  __shared__ float sm[256], ss[256];
+  __shared__ float sm[256], ss[256], sl[16], sg[16];  // sl, sg: loss and -D of a label
   auto ex = [](float v) { return kB2 ? __builtin_amdgcn_exp2f(v) : exp_of<true>(v); };
   const int t = threadIdx.x, rl = t & (p.rb - 1), strip = t / p.rb, strips = 256 / p.rb;
   const long long row = (long long)blockIdx.x * p.rb + rl;
@@ -702,7 +701,7 @@ __global__ __launch_bounds__(256) void row_kernel(RowArgs p) {
       for (int u = 0; u < 4; ++u) s += a[u].y * (a[u].x == -INFINITY ? 1.0f : ex(a[u].x - n0));
       m = nm;
     }
-    if (p.base && strip == 0) {
+    if (p.base && strip == 0 && !(p.mode == 0 && p.loss && index_at(p.idx, p.idx64, row) == p.V)) {
       const float nm = fmaxf(m, 0.0f);
       s = (m == -INFINITY ? 0.0f : s * ex(m - nm)) + ex(-nm);
       m = nm;
@@ -720,9 +719,38 @@ __global__ __launch_bounds__(256) void row_kernel(RowArgs p) {
     __syncthreads();
   }
   if (t < p.rb && row < p.n) {
-    if (p.norm) p.norm[row] = make_float2(sm[t], 1.0f / ss[t]);
-    ss[t] = logf(ss[t]);
-    p.lse[row] = (kB2 ? sm[t] * 0.6931471805599453f : sm[t]) + ss[t];
+    const float m = sm[t];
+    float s = ss[t];
+    const long long v = p.mode == 0 && p.loss ? index_at(p.idx, p.idx64, row) : -1;
+    if (v >= 0 && v < p.V + p.base) {
+      // the label's own term: rel = z - m. loss = log(1 + s e^-rel), D = -s / (s + e^rel) without cancellation
+      const float mg = v < p.V ? p.stats[v / kGroup * p.n + row].x : 0.0f;
+      const float z = v < p.V ? p.zt[row] : 0.0f, rel = z + ((mg == -INFINITY ? 0.0f : mg) - m);
+      const float nat = kB2 ? rel * 0.6931471805599453f : rel;
+      if (m == -INFINITY) {  // nothing else
+        const float abs = z + (mg == -INFINITY ? 0.0f : mg);
+        sl[t] = s;  // 0, or NaN
+        sg[t] = s;
+        p.lse[row] = (kB2 ? abs * 0.6931471805599453f : abs) + s;
+        if (p.norm) p.norm[row] = make_float2(abs, 1.0f);
+      } else if (nat > 60.0f) {  // e^rel does not fit: relative to the label
+        const float w = s * ex(-rel);
+        sl[t] = log1pf(w);
+        sg[t] = w / (1.0f + w);
+        p.lse[row] = (kB2 ? (m + rel) * 0.6931471805599453f : m + rel) + sl[t];
+        if (p.norm) p.norm[row] = make_float2(m + rel, 1.0f / (1.0f + w));
+      } else {
+        const float e = ex(rel), all = s + e;
+        sl[t] = nat > 0.0f ? log1pf(s * ex(-rel)) : logf(all) - nat;
+        sg[t] = s / all;
+        p.lse[row] = (kB2 ? m * 0.6931471805599453f : m) + logf(all);
+        if (p.norm) p.norm[row] = make_float2(m, 1.0f / all);
+      }
+    } else {
+      if (p.norm) p.norm[row] = make_float2(m, 1.0f / s);
+      ss[t] = logf(s);
+      p.lse[row] = (kB2 ? m * 0.6931471805599453f : m) + ss[t];
+    }
   }
   __syncthreads();
   if (!p.loss) return;
@@ -732,7 +760,7 @@ __global__ __launch_bounds__(256) void row_kernel(RowArgs p) {
     const long long i = (long long)blockIdx.x * p.rb + r;
     if (i >= p.n) break;
     const float mx_row = sm[r], log_s = ss[r], g = p.weight ? p.weight[i] : 1.0f;
-    float norm = 0.0f;
+    float norm = 0.0f, log_e = 0.0f, inv_e = 1.0f;  // q = e^(t - norm) inv_e
     if (p.mode == 1) {  // renormalise the list: log sum e^(t/T) over its entries
       float mx = -INFINITY;
       for (int j = l; j < p.k; j += 64)
@@ -744,7 +772,8 @@ __global__ __launch_bounds__(256) void row_kernel(RowArgs p) {
       for (int j = l; j < p.k; j += 64)
         if (index_at(p.idx, p.idx64, i * p.k + j) >= 0) e += expf(p.tl[i * p.k + j] / p.temp - mx);
       e = wave_sumf(e);
-      norm = e == 0.0f ? 0.0f : mx + logf(e);  // nothing but -inf: every q_j is 0
+      norm = mx;
+      if (e != 0.0f) log_e = logf(e), inv_e = 1.0f / e;  // otherwise nothing but -inf: every q_j is 0
     } else if (p.mode == 2) {
       norm = p.tlse[i];
     }
@@ -757,22 +786,18 @@ __global__ __launch_bounds__(256) void row_kernel(RowArgs p) {
         if (v < 0 || v >= p.V + p.base) {
           term = NAN;  // a class that does not exist
         } else {
-          const float lq = p.mode == 0 ? 0.0f : p.tl[i * p.k + j] / p.temp - norm;
-          q = p.mode == 0 ? 1.0f : expf(lq);
-          if (q > 0.0f || q != q) {
-            // log q + lse - z, the maximum's part first: it cancels exactly where z is the maximum. A label's score is
-            // kept relative to its group's maximum as its exponential in s is, and from here on to the row's.
-            float up = mx_row - (v < p.V ? p.zt[i * p.k + j] : 0.0f);
-            if (p.mode == 0 && v < p.V) {
-              const float mg = p.stats[v / kGroup * p.n + i].x, rel = p.zt[i] + ((mg == -INFINITY ? 0.0f : mg) - mx_row);
-              p.zt[i] = rel;
-              up = -rel;
-            }
+          const float t = p.mode == 0 ? 0.0f : p.tl[i * p.k + j] / p.temp - norm, lq = t - log_e;
+          q = p.mode == 0 ? 1.0f : expf(t) * inv_e;
+          if (p.mode == 0) {
+            term = sl[r];
+          } else if (q > 0.0f || q != q) {
+            // log q + lse - z, the maximum's part first: it cancels where z is near the maximum
+            const float up = mx_row - p.zt[i * p.k + j];
             term = q * (lq + ((kB2 ? up * 0.6931471805599453f : up) + log_s));
           }
         }
       }
-      if (p.q) p.q[i * p.k + j] = q * g * p.temp;
+      if (p.q) p.q[i * p.k + j] = (p.mode == 0 ? q * sg[r] : q) * g * p.temp;
       sq += q;
       ls += term;
     }
@@ -798,7 +823,7 @@ struct DArgs {
   long long ld, plane;
   float* part;          // [row blocks][ld] bias gradient partials, or null
   int rw;               // rows per wave
-  int zt_rel;           // zt is relative to the row's maximum (labels)
+  int label;            // targets are labels: q is all of D there
   int keep32;           // fp32 inputs: D also in fp32, in place of E
   char* x;              // packed x of these rows, or null: rows without a gradient are cleared in it before they meet D
   long long xpitch, xplane;
@@ -862,8 +887,8 @@ __global__ __launch_bounds__(256) void dscore_kernel(DArgs p) {
             for (unsigned long long h = __ballot(at >= 0); h; h &= h - 1) {
               const int bit = __builtin_ctzll(h), vb = __builtin_amdgcn_readlane(at, bit);
               const long long e = i * p.k + j0 + bit;
-              const float rel = p.zt_rel ? p.zt[e] : p.zt[e] - nr[b].x;
-              const float x = pass != 0 ? p.q[e] : co * (kF32 ? exp_of<true>(rel) : __builtin_amdgcn_exp2f(rel));
+              const float rel = p.zt[e] - nr[b].x;
+              const float x = pass != 0 ? p.q[e] : p.label ? 0.0f : co * (kF32 ? exp_of<true>(rel) : __builtin_amdgcn_exp2f(rel));
 #pragma unroll
               for (int u = 0; u < 8; ++u)
                 if (vb == l * 8 + u) d[b][u] = pass == 0 ? x : d[b][u] - x;
@@ -1831,7 +1856,7 @@ extern "C" void ytk_head_loss(const uintptr_t* ptrs, const long long* lp, double
     d.e = ws + p.o_e, d.d = (__bf16*)(ws + p.o_d), d.ld = p.ld, d.plane = rows * p.ld;
     d.part = db ? (float*)(ws + p.o_part) : nullptr;
     d.rw = p.rw;
-    d.zt_rel = h.mode == 0;
+    d.label = h.mode == 0;
     d.keep32 = p.few;
     if (h.f32 && !p.planes_d) d.d = nullptr;
     if (h.want_dw && p.pack_x) {
