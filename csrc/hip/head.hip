@@ -877,23 +877,25 @@ __global__ __launch_bounds__(256) void dscore_kernel(DArgs p) {
         const float f = co * (kF32 ? exp_of<true>(mg) : __builtin_amdgcn_exp2f(mg - 15.0f));
 #pragma unroll
         for (int j = 0; j < 8; ++j) d[b][j] *= f;
-        // target classes: p is taken from the fp32 score, and every entry of the list on that class is subtracted
-        // (first all probabilities, then all targets: a class named twice is counted twice)
+        // target classes: every entry of the list on that class is subtracted from p. bf16 lists take p from the fp32
+        // score first (E's 11 bits would show where p is near q); fp32 E agrees with the row's sum to the last bit,
+        // which the score summed in another order does not, and a label's E is 0
 #pragma unroll
-        for (int pass = 0; pass < 2; ++pass)
+        for (int pass = 0; pass < 2; ++pass) {
+          if (pass == 0 && (kF32 || p.label)) continue;
           for (int j0 = 0; j0 < p.k; j0 += 64) {
             const long long vv = j0 == 0 ? v[b] : j0 + l < p.k ? index_at(p.idx, p.idx64, i * p.k + j0 + l) : -1;
             const int at = vv >= c0 && vv < c0 + kDCols && vv < p.V ? (int)(vv - c0) : -1;
             for (unsigned long long h = __ballot(at >= 0); h; h &= h - 1) {
               const int bit = __builtin_ctzll(h), vb = __builtin_amdgcn_readlane(at, bit);
               const long long e = i * p.k + j0 + bit;
-              const float rel = p.zt[e] - nr[b].x;
-              const float x = pass != 0 ? p.q[e] : p.label ? 0.0f : co * (kF32 ? exp_of<true>(rel) : __builtin_amdgcn_exp2f(rel));
+              const float x = pass != 0 ? p.q[e] : co * __builtin_amdgcn_exp2f(p.zt[e] - nr[b].x);
 #pragma unroll
               for (int u = 0; u < 8; ++u)
                 if (vb == l * 8 + u) d[b][u] = pass == 0 ? x : d[b][u] - x;
             }
           }
+        }
       } else {
 #pragma unroll
         for (int j = 0; j < 8; ++j) d[b][j] = 0.0f;
