@@ -1546,8 +1546,10 @@ static HeadPlan head_plan(const HeadIn& h, bool topk) {
   p.pack_x = p.few ? h.want_dw && !topk && !p.few_dw : h.f32 || !h.x_al;
   p.pack_w = !p.few && (h.f32 || !h.w_al);
   const long long per = topk ? p.ld * 4 : p.grads ? p.ld * (h.f32 ? 10 : 2) : p.groups * 8;
-  // (at most 2M rows: the grids of the row passes count rows / 64 in 16 bits and rows * k in 31)
-  p.piece = std::min(h.n, std::min(1LL << 21, std::max(256LL, h.piece_bytes / per / 256 * 256)));
+  // (at most 2M rows, fewer of long lists: the grids of the row passes count rows / 64 in 16 bits, and the targets' threads,
+  // 16 per list entry, in 32)
+  const long long most = topk ? 1LL << 21 : std::min(1LL << 21, (1LL << 25) / ceil_div(h.k, 4) / 256 * 256);
+  p.piece = std::min(h.n, std::min(most, std::max(256LL, h.piece_bytes / per / 256 * 256)));
   p.many = p.piece < h.n;
   long long part = 0;
   if (h.want_dx && p.few) {  // runs of classes: about 1024 blocks, at least 128 classes each

@@ -490,6 +490,24 @@ def test_distill_edges(cuda):
     near(r.loss[2:3], one.loss.double().cpu() + (q * q.log()).sum(), ref.eloss[1:2] * 2, "split entry")
 
 
+@pytest.mark.gpu
+def test_distill_many_rows_with_long_lists(cuda):
+    """As many list entries as one launch's threads: the rows go in pieces. Only the first and last rows have a weight."""
+    n, k, V, T = (1 << 20) + 777, 256, 40, 1.5
+    x, w, _, b = make(n, 3, V, torch.float32, cuda, bias=True)
+    at = torch.cat([torch.arange(150), torch.arange(n - 150, n)])
+    g = torch.zeros(n, device=cuda)
+    g[at.to(cuda)] = 1.0
+    idx = torch.full((n, k), -1, dtype=torch.int32, device=cuda)
+    tl = torch.zeros((n, k), device=cuda)
+    i, t = lists(len(at), V, k)
+    idx[at.to(cuda)], tl[at.to(cuda)] = i.int().to(cuda), t.to(cuda)
+    r = head.distill_head_loss(x, w, idx, tl, bias=b, weight=g, temperature=T)
+    assert int((r.loss != 0).sum()) <= len(at) and int((r.dx != 0).any(1).sum()) <= len(at)
+    at = at.to(cuda)
+    Ref(x[at], w, i, list_targets(i, t, T), bias=b, T=T).check(head.HeadLoss(r.loss[at], r.lse[at], r.dx[at], r.dw, r.db), db=True)
+
+
 # ------------------------------------------------------------------ top k
 def topk_ref(x, w, bias, T, k):
     z = x.double() @ w.double().t()
