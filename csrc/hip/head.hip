@@ -804,7 +804,7 @@ __global__ __launch_bounds__(256) void row_kernel(RowArgs p) {
     sq = wave_sumf(sq);
     ls = wave_sumf(ls);
     if (l == 0) {
-      const float c = g * p.temp * sq;
+      const float c = g == 0.0f ? 0.0f : g * p.temp * sq;  // (a row without weight: whatever its list holds)
       p.loss[i] = (g == 0.0f || (sq == 0.0f && ls == ls)) ? 0.0f : g * p.temp * p.temp * ls;
       if (p.coef) p.coef[i] = c;
     }

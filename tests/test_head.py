@@ -490,6 +490,32 @@ def test_distill_edges(cuda):
     near(r.loss[2:3], one.loss.double().cpu() + (q * q.log()).sum(), ref.eloss[1:2] * 2, "split entry")
 
 
+def _weightless(dev):
+    """A weight of 0 takes a row out of every gradient, whatever its list and x hold; so does an entry -1 its logit."""
+    nan, inf = float("nan"), float("inf")
+    x, w, _, _ = make(5, 64, 100, torch.float32, dev)
+    x[1], x[3] = nan, inf
+    idx = torch.tensor([[1, 2, -1], [3, 4, 5], [6, -1, 7], [8, 9, 10], [11, 12, 13]])
+    tl = torch.tensor([[1.0, 2.0, nan], [nan, 1.0, 2.0], [0.5, inf, 1.0], [inf, inf, 0.0], [nan, nan, nan]])
+    g = torch.tensor([1.0, 0.0, 2.0, 0.0, 0.0])
+    tlse = torch.tensor([3.0, nan, 3.0, inf, nan])
+    ok = [0, 2]
+    for t in (None, tlse):
+        r = head.distill_head_loss(x, w, idx.to(dev), tl.to(dev), weight=g.to(dev), top_lse=None if t is None else t.to(dev))
+        assert bool((r.loss[[1, 3, 4]] == 0).all()) and bool((r.dx[[1, 3, 4]] == 0).all())
+        ref = Ref(x[ok], w, idx[ok], list_targets(idx[ok], tl[ok], 1.0, None if t is None else t[ok]), weight=g[ok])
+        ref.check(head.HeadLoss(r.loss[ok], r.lse[ok], r.dx[ok], r.dw, None))
+
+
+def test_distill_weightless_rows_cpu():
+    _weightless("cpu")
+
+
+@pytest.mark.gpu
+def test_distill_weightless_rows_gpu(cuda):
+    _weightless(cuda)
+
+
 @pytest.mark.gpu
 def test_distill_many_rows_with_long_lists(cuda):
     """As many list entries as one launch's threads: the rows go in pieces. Only the first and last rows have a weight."""
