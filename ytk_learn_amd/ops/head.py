@@ -80,6 +80,8 @@ def _operands(x, w):
     few = x.dtype == torch.float32 and x.shape[0] <= FEW_ROWS
 
     def one(t):
+        if t.shape[1] == 1:  # one column may carry any stride, and contiguous() leaves it
+            t = t.as_strided(t.shape, (t.stride(0), 1))
         odd = (t.stride(0) <= 0 and t.shape[0] > 1) or (t.stride(1) <= 0 and t.shape[1] > 1)
         return t.contiguous() if odd or (few and t.stride(1) != 1) else t
 
