@@ -12,9 +12,8 @@
 //
 // Tiles go from global memory straight into LDS (buffer_load ... lds, 16 B a lane). The buffer descriptor ends at
 // the operand's last byte, so rows past the end (of M, N or K) read as zero and need no branch.
-// The DMA writes LDS linearly, so the bank swizzle is applied to the SOURCE address: a KC row is 128 B = eight
-// 16-B chunks, chunk c of row r sits at c ^ (r & 7); a KS row is cut into 64-B units, unit u of
-// row k sits at u ^ f(k). KC fragments are ds_read_b128; KS fragments are read transposed
+// The DMA writes LDS linearly, so the bank swizzle is applied to the SOURCE address: a KC row is eight or four 16-B
+// chunks, chunk c of row r sits at c ^ swc(r); a KS row is cut into 64-B units, unit u of row k sits at u ^ swz(k). KC fragments are ds_read_b128; KS fragments are read transposed
 // (ds_read_b64_tr_b16: 16 lanes exchange a 4 x 16 block).
 #pragma once
 #include "common.h"
