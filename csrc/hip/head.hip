@@ -10,12 +10,12 @@
 //   1. scores_kernel   z by MFMA; per row and group of 64 classes the maximum m and sum s of e^(z - m); with
 //                      gradients also E = e^(z - m) (bf16 inputs: as fp16 scaled by 2^15, 11 bits, so that
 //                      the one rounding that matters is D's own to bf16; fp32 inputs: fp32)
-//   2. target_kernel   z of the target classes as plain fp32 dot products
+//   2. target_kernel   (lists) z of the target classes as plain fp32 dot products
 //   3. row_kernel      lse from the groups, loss, and the row's coefficients
 //   4. dscore_kernel   E -> D in place (fp32: three bf16 planes), bias gradient partials
 //   5. grad kernels    dx = D w, dw = D^T x
 // The scores are computed once: 6 n d V operations for a step, against 8 n d V where pieces of the classes compute
-// them again for the gradient. (8192 x 4096 x 131072: the D pass over 2 GiB takes 0.88 ms, a fourth product 7.0.)
+// them again for the gradient. (8192 x 4096 x 131072: the D pass over 2 GiB takes 0.86 ms, a fourth product 7.0.)
 #include "head_gemm.h"
 
 #include <algorithm>
