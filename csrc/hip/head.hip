@@ -872,8 +872,9 @@ __global__ __launch_bounds__(256) void dscore_kernel(DArgs p) {
       const long long i = r0 + rb + b;
       const float co = cw[b] * nr[b].y;
       if (cw[b] != 0.0f) {
-        // E is e^(z - m) with m = 0 for a group that has only -inf
-        const float mg = (m[b] == -INFINITY ? 0.0f : m[b]) - nr[b].x;
+        // (a group that has only -inf, or nothing but the label: E is 0, and m = -inf makes f 0 too. With 0 for its m, f would be
+        // e^-max, infinite for a row of low scores, and 0 f NaN)
+        const float mg = m[b] - nr[b].x;
         const float f = co * (kF32 ? exp_of<true>(mg) : __builtin_amdgcn_exp2f(mg - 15.0f));
 #pragma unroll
         for (int j = 0; j < 8; ++j) d[b][j] *= f;
