@@ -10,6 +10,9 @@
 //   1. scores_kernel   z by MFMA; per row and group of 64 classes the maximum m and sum s of e^(z - m); with
 //                      gradients also E = e^(z - m) (bf16 inputs: as fp16 scaled by 2^15, 11 bits, so that
 //                      the one rounding that matters is D's own to bf16; fp32 inputs: fp32)
+//                      Maxima, and scores that are kept, are those before the division by T. A difference is taken before
+//                      it is scaled: the maximum's own exponent is exactly 0 and no other is above it, however large
+//                      the scores are (z / T - m / T in one fma keeps the rounding of m / T, 2^-24 of it: unbounded).
 //   2. target_kernel   (lists) z of the target classes as plain fp32 dot products
 //   3. row_kernel      lse from the groups, loss, and the row's coefficients
 //   4. dscore_kernel   E -> D in place (fp32: three bf16 planes), bias gradient partials
@@ -116,9 +119,9 @@ struct ScoreArgs {
   float inv_t;
   float2* stats;      // [groups][n]: m, s
   void* e;            // E [n][ld] (fp16 or fp32) or null
-  float* z;           // scores [n][ld] or null
+  float* z;           // scores before the division by T [n][ld], or null
   long long ld;
-  const void* label;  // [n] or null: a row's label is left out of its group; its score less the group's m (0 for -inf) goes to zt
+  const void* label;  // [n] or null: a row's label is left out of its group; its score (before the division) goes to zt
   int idx64;
   float* zt;
 };
@@ -179,8 +182,7 @@ __device__ __forceinline__ float exp_of(float v) {
 // what a call keeps of its scores: nothing (bf16, fp32 inputs), E (bf16, fp32), the scores
 enum { kStatsOnly = 0, kExpHalf = 1, kExpFloat = 2, kScores = 3, kStatsFloat = 4 };
 
-// Maxima are in the unit of the stats: log2 units for bf16 inputs with a loss (the exponential is one fma and
-// one exp2 from the accumulator), natural ones otherwise (fp32: a finer exponential; top k: the stored scores' own).
+// bf16 inputs with a loss: the exponential is a difference, an fma and an exp2 from the accumulator (fp32: a finer one)
 template <int kMode>
 constexpr bool kBase2 = kMode == kStatsOnly || kMode == kExpHalf;
 
@@ -257,27 +259,27 @@ __global__ __launch_bounds__(C::kThreads) void scores_kernel(ScoreArgs p) {
             for (int h = 0; h < 2; ++h)
 #pragma unroll
               for (int r = 0; r < 16; ++r) mx = fmaxf(mx, acc[2 * g + h][j][r]);
-            const float m = fmaxf(mx, __shfl_xor(mx, 32, 64)) * c;
+            const float m = fmaxf(mx, __shfl_xor(mx, 32, 64));
             const float m0 = m == -INFINITY ? 0.0f : m;
-            if (kMode != kScores && mine) p.zt[i] = fmaf(zl, c, -m0);
+            if (kMode != kScores && mine) p.zt[i] = zl;
             if (kMode == kScores)
 #pragma unroll
               for (int h = 0; h < 2; ++h) {
                 const f32x16& t = acc[2 * g + h][j];
 #pragma unroll
-                for (int q = 0; q < 4; ++q) turn.put(l & 31, 2 * q + hi, bits4(t[4 * q] * c, t[4 * q + 1] * c, t[4 * q + 2] * c, t[4 * q + 3] * c));
+                for (int q = 0; q < 4; ++q) turn.put(l & 31, 2 * q + hi, bits4(t[4 * q], t[4 * q + 1], t[4 * q + 2], t[4 * q + 3]));
                 store_rows(turn, (char*)p.z + (i0 + j * 32) * p.ld * 4 + (vg + h * 32) * 4LL, p.ld * 4, p.n - i0 - j * 32);
               }
             float s = 0.0f, e[2][16];
-            const float off = kMode == kExpHalf ? 15.0f - m0 : -m0;  // E is scaled by 2^15
+            const float off = kMode == kExpHalf ? 15.0f : 0.0f;  // E is scaled by 2^15
 #pragma unroll
             for (int h = 0; h < 2; ++h)
 #pragma unroll
               for (int r = 0; r < 16; ++r) {
                 if (kBase2<kMode>)
-                  e[h][r] = __builtin_amdgcn_exp2f(fmaf(acc[2 * g + h][j][r], c, off));
+                  e[h][r] = __builtin_amdgcn_exp2f(fmaf(acc[2 * g + h][j][r] - m0, c, off));
                 else
-                  e[h][r] = exp_of<kMode == kExpFloat || kMode == kStatsFloat>(acc[2 * g + h][j][r] * c - m0);
+                  e[h][r] = exp_of<kMode == kExpFloat || kMode == kStatsFloat>((acc[2 * g + h][j][r] - m0) * c);
                 s += e[h][r];
               }
             s += __shfl_xor(s, 32, 64);
@@ -411,21 +413,21 @@ __global__ __launch_bounds__(256, 2) void scores_few_kernel(FewArgs p) {
     for (int r = 0; r < 4; ++r) {
       const int v = vg + t * 16 + g4 * 4 + r;
       const float b = p.bias ? p.bias[min(v, p.V - 1)] : 0.0f;
-      z[t][r] = v < p.V ? (sum[t][r] + b) * p.inv_t : -INFINITY;
+      z[t][r] = v < p.V ? sum[t][r] + b : -INFINITY;
       if (v == label) zl = z[t][r], z[t][r] = -INFINITY, mine = true;  // as in scores_kernel
       m = fmaxf(m, z[t][r]);
     }
   m = fmaxf(m, __shfl_xor(m, 16, 64));
   m = fmaxf(m, __shfl_xor(m, 32, 64));
   const float m0 = m == -INFINITY ? 0.0f : m;
-  if (mine) p.zt[row] = zl - m0;
+  if (mine) p.zt[row] = zl;
   float s = 0.0f;
   float* o = p.e + (long long)row * p.ld + vg + g4 * 4;
 #pragma unroll
   for (int t = 0; t < 4; ++t) {
     if (kMode == kScores && row < p.n) *(float4*)(o + t * 16) = make_float4(z[t][0], z[t][1], z[t][2], z[t][3]);
 #pragma unroll
-    for (int r = 0; r < 4; ++r) s += z[t][r] = exp_of<true>(z[t][r] - m0);
+    for (int r = 0; r < 4; ++r) s += z[t][r] = exp_of<true>((z[t][r] - m0) * p.inv_t);
     if (kMode == kExpFloat && row < p.n) *(float4*)(o + t * 16) = make_float4(z[t][0], z[t][1], z[t][2], z[t][3]);
   }
   s += __shfl_xor(s, 16, 64);
@@ -557,13 +559,12 @@ __global__ __launch_bounds__(256) void dw_few_kernel(FewOuterArgs p) {
 }
 
 // ------------------------------------------------------------------ targets
-// z of each row's target classes by plain fp32 dot products.
+// Scores (before the division by T) of each row's target classes by plain fp32 dot products.
 struct TargetArgs {
   const void *x, *w, *bias;
   long long xrs, xcs, wrs, wcs;
   const void* idx;     // [n][k], int64 or int32
   int idx64, k, n, d, V, vec;
-  float unit;          // 1 / T in the unit of the stats
   float* zt;           // [n][k]
 };
 
@@ -654,7 +655,7 @@ __global__ __launch_bounds__(256) void target_kernel(TargetArgs p) {
   if (l == 0) {
 #pragma unroll
     for (int i = 0; i < kW; ++i)
-      if (i < m) p.zt[first + i] = v[i] < 0 ? 0.0f : (s[i] + (p.bias ? Elem<T>::get((const T*)p.bias, v[i]) : 0.0f)) * p.unit;
+      if (i < m) p.zt[first + i] = v[i] < 0 ? 0.0f : s[i] + (p.bias ? Elem<T>::get((const T*)p.bias, v[i]) : 0.0f);
   }
 }
 
@@ -667,19 +668,20 @@ struct RowArgs {
   int idx64;
   long long ignore;
   const float *tl, *tlse, *weight, *zt;
-  float temp;
+  float temp, inv_t;
   float *lse, *loss;    // outputs
   float* coef;          // [n] g T s  (0: the row has no gradient)
-  float2* norm;         // [n] maximum and 1 / sum: p = e^(z - max) / sum, without the rounding of lse
+  float2* norm;         // [n] maximum (before the division by T) and 1 / sum: p = e^((z - max) / T) / sum, without the rounding of lse
   float* q;             // [n][k] g T q_j; of a label g (1 - p), all of its D
   int rb;               // rows per block (a power of two, <= 16)
 };
 
-// kB2: the maxima are in log2 units
+// Scores and maxima are those before the division by T. kB2: bf16 inputs, whose exponentials are exp2 alone
 template <bool kB2>
 __global__ __launch_bounds__(256) void row_kernel(RowArgs p) {
   __shared__ float sm[256], ss[256], sl[16], sg[16];  // sl, sg: loss and -D of a label
-  auto ex = [](float v) { return kB2 ? __builtin_amdgcn_exp2f(v) : exp_of<true>(v); };
+  const float unit = kB2 ? p.inv_t * kLog2e : p.inv_t;
+  auto ex = [&](float v) { return kB2 ? __builtin_amdgcn_exp2f(v * unit) : exp_of<true>(v * unit); };  // e^(v / T)
   const int t = threadIdx.x, rl = t & (p.rb - 1), strip = t / p.rb, strips = 256 / p.rb;
   const long long row = (long long)blockIdx.x * p.rb + rl;
   // running maximum and sum over this thread's groups
@@ -724,32 +726,29 @@ __global__ __launch_bounds__(256) void row_kernel(RowArgs p) {
     const long long v = p.mode == 0 && p.loss ? index_at(p.idx, p.idx64, row) : -1;
     if (v >= 0 && v < p.V + p.base) {
       // the label's own term: rel = z - m. loss = log(1 + s e^-rel), D = -s / (s + e^rel) without cancellation
-      const float mg = v < p.V ? p.stats[v / kGroup * p.n + row].x : 0.0f;
-      const float z = v < p.V ? p.zt[row] : 0.0f, rel = z + ((mg == -INFINITY ? 0.0f : mg) - m);
-      const float nat = kB2 ? rel * 0.6931471805599453f : rel;
+      const float z = v < p.V ? p.zt[row] : 0.0f, rel = z - m, nat = rel * p.inv_t;
       if (m == -INFINITY) {  // nothing else
-        const float abs = z + (mg == -INFINITY ? 0.0f : mg);
         sl[t] = s;  // 0, or NaN
         sg[t] = s;
-        p.lse[row] = (kB2 ? abs * 0.6931471805599453f : abs) + s;
-        if (p.norm) p.norm[row] = make_float2(abs, 1.0f);
+        p.lse[row] = z * p.inv_t + s;
+        if (p.norm) p.norm[row] = make_float2(z, 1.0f);
       } else if (nat > 60.0f) {  // e^rel does not fit: relative to the label
         const float w = s * ex(-rel);
         sl[t] = log1pf(w);
         sg[t] = w / (1.0f + w);
-        p.lse[row] = (kB2 ? (m + rel) * 0.6931471805599453f : m + rel) + sl[t];
-        if (p.norm) p.norm[row] = make_float2(m + rel, 1.0f / (1.0f + w));
+        p.lse[row] = z * p.inv_t + sl[t];
+        if (p.norm) p.norm[row] = make_float2(z, 1.0f / (1.0f + w));
       } else {
         const float e = ex(rel), all = s + e;
         sl[t] = nat > 0.0f ? log1pf(s * ex(-rel)) : logf(all) - nat;
         sg[t] = s / all;
-        p.lse[row] = (kB2 ? m * 0.6931471805599453f : m) + logf(all);
+        p.lse[row] = m * p.inv_t + logf(all);
         if (p.norm) p.norm[row] = make_float2(m, 1.0f / all);
       }
     } else {
       if (p.norm) p.norm[row] = make_float2(m, 1.0f / s);
       ss[t] = logf(s);
-      p.lse[row] = (kB2 ? m * 0.6931471805599453f : m) + ss[t];
+      p.lse[row] = m * p.inv_t + ss[t];
     }
   }
   __syncthreads();
@@ -793,7 +792,7 @@ __global__ __launch_bounds__(256) void row_kernel(RowArgs p) {
           } else if (q > 0.0f || q != q) {
             // log q + lse - z, the maximum's part first: it cancels where z is near the maximum
             const float up = mx_row - p.zt[i * p.k + j];
-            term = q * (lq + ((kB2 ? up * 0.6931471805599453f : up) + log_s));
+            term = q * (lq + (up * p.inv_t + log_s));
           }
         }
       }
@@ -822,6 +821,7 @@ struct DArgs {
   __bf16* d;            // fp32 inputs: D planes
   long long ld, plane;
   float* part;          // [row blocks][ld] bias gradient partials, or null
+  float unit;           // 1 / T, bf16 inputs: in log2 units
   int rw;               // rows per wave
   int label;            // targets are labels: q is all of D there
   int keep32;           // fp32 inputs: D also in fp32, in place of E
@@ -875,7 +875,7 @@ __global__ __launch_bounds__(256) void dscore_kernel(DArgs p) {
         // (a group that has only -inf, or nothing but the label: E is 0, and m = -inf makes f 0 too. With 0 for its m, f would be
         // e^-max, infinite for a row of low scores, and 0 f NaN)
         const float mg = m[b] - nr[b].x;
-        const float f = co * (kF32 ? exp_of<true>(mg) : __builtin_amdgcn_exp2f(mg - 15.0f));
+        const float f = co * (kF32 ? exp_of<true>(mg * p.unit) : __builtin_amdgcn_exp2f(fmaf(mg, p.unit, -15.0f)));
 #pragma unroll
         for (int j = 0; j < 8; ++j) d[b][j] *= f;
         // target classes: every entry of the list on that class is subtracted from p. bf16 lists take p from the fp32
@@ -890,7 +890,7 @@ __global__ __launch_bounds__(256) void dscore_kernel(DArgs p) {
             for (unsigned long long h = __ballot(at >= 0); h; h &= h - 1) {
               const int bit = __builtin_ctzll(h), vb = __builtin_amdgcn_readlane(at, bit);
               const long long e = i * p.k + j0 + bit;
-              const float x = pass != 0 ? p.q[e] : co * __builtin_amdgcn_exp2f(p.zt[e] - nr[b].x);
+              const float x = pass != 0 ? p.q[e] : co * __builtin_amdgcn_exp2f((p.zt[e] - nr[b].x) * p.unit);
 #pragma unroll
               for (int u = 0; u < 8; ++u)
                 if (vb == l * 8 + u) d[b][u] = pass == 0 ? x : d[b][u] - x;
@@ -1830,7 +1830,6 @@ extern "C" void ytk_head_loss(const uintptr_t* ptrs, const long long* lp, double
     t.idx = idx + r0 * h.k * (h.idx64 ? 8 : 4);
     t.idx64 = (int)h.idx64;
     t.k = (int)h.k, t.n = (int)rows, t.d = (int)h.d, t.V = (int)h.V, t.vec = dots_vec(h, x, w);
-    t.unit = h.f32 ? 1.0f / temp : 1.0f / temp * kLog2e;
     t.zt = (float*)(ws + p.o_zt);
     const void* label = h.mode == 0 ? t.idx : nullptr;
     if (p.few)
@@ -1850,7 +1849,7 @@ extern "C" void ytk_head_loss(const uintptr_t* ptrs, const long long* lp, double
     r.idx = t.idx, r.idx64 = t.idx64, r.ignore = h.ignore;
     r.tl = tl ? tl + r0 * h.k : nullptr, r.tlse = tlse ? tlse + r0 : nullptr;
     r.weight = weight ? weight + r0 : nullptr;
-    r.zt = t.zt, r.temp = temp;
+    r.zt = t.zt, r.temp = temp, r.inv_t = 1.0f / temp;
     r.lse = lse + r0, r.loss = loss + r0;
     r.coef = p.grads ? (float*)(ws + p.o_coef) : nullptr;
     r.q = p.grads ? (float*)(ws + p.o_q) : nullptr;
@@ -1864,6 +1863,7 @@ extern "C" void ytk_head_loss(const uintptr_t* ptrs, const long long* lp, double
     d.idx = t.idx, d.idx64 = t.idx64, d.n = (int)rows, d.V = (int)h.V, d.k = (int)h.k;
     d.e = ws + p.o_e, d.d = (__bf16*)(ws + p.o_d), d.ld = p.ld, d.plane = rows * p.ld;
     d.part = db ? (float*)(ws + p.o_part) : nullptr;
+    d.unit = h.f32 ? 1.0f / temp : 1.0f / temp * kLog2e;
     d.rw = p.rw;
     d.label = h.mode == 0;
     d.keep32 = p.few;
@@ -1955,6 +1955,7 @@ extern "C" void ytk_head_topk(const uintptr_t* ptrs, const long long* lp, double
     RowArgs r = {};
     r.stats = (const float2*)(ws + p.o_stats);
     r.groups = (int)p.groups, r.n = (int)rows, r.V = (int)h.V;
+    r.inv_t = 1.0f / (float)temp_;
     r.lse = (float*)ptrs[6] + r0;
     rows_pass(r, false, s);
     TopArgs t = {};
