@@ -39,11 +39,16 @@ struct Operand {
   int ext;          // extent of M (or N)
 };
 
+// m0 holds the LDS address. It is declared as written, although the compiler gives it to no value, so that a setting of its own
+// for an instruction that reads m0 is not carried across (the compiler warns of any such register on a list).
+#pragma clang diagnostic push
+#pragma clang diagnostic ignored "-Winline-asm"
 __device__ __forceinline__ void dma16(unsigned voff, i32x4 rsrc, unsigned soff, unsigned lds) {
   asm volatile("s_mov_b32 m0, %3\n\ts_nop 0\n\tbuffer_load_dwordx4 %0, %1, %2 offen lds" ::"v"(voff), "s"(rsrc), "s"(soff),
                "s"(lds)
-               : "memory");
+               : "memory", "m0");
 }
+#pragma clang diagnostic pop
 template <int N>
 __device__ __forceinline__ void wait_vm() {
   asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory");
