@@ -7,7 +7,7 @@
 //   top k:   the k largest z of each row and lse
 //
 // Rows are taken in pieces so that at most `piece_bytes` of exponentials live at a time. Per piece:
-//   1. scores_kernel   z by MFMA; per row and group of 64 classes the maximum m and sum s of e^(z - m); with
+//   1. scores_kernel   z by MFMA (top k: also the largest squared norm of w in each group); per row and group of 64 classes the maximum m and sum s of e^(z - m); with
 //                      gradients also E = e^(z - m) (bf16 inputs: as fp16 scaled by 2^15, 11 bits, so that
 //                      the one rounding that matters is D's own to bf16; fp32 inputs: fp32)
 //                      Maxima, and scores that are kept, are those before the division by T. A difference is taken before
@@ -124,6 +124,8 @@ struct ScoreArgs {
   const void* label;  // [n] or null: a row's label is left out of its group; its score (before the division) goes to zt
   int idx64;
   float* zt;
+  float* norms;       // scores that are kept: [parts][groups] largest squared norm of the group's classes, over each part of d
+  int parts;
 };
 
 __device__ __forceinline__ long long index_at(const void* p, int is64, long long i) {
@@ -186,11 +188,15 @@ enum { kStatsOnly = 0, kExpHalf = 1, kExpFloat = 2, kScores = 3, kStatsFloat = 4
 template <int kMode>
 constexpr bool kBase2 = kMode == kStatsOnly || kMode == kExpHalf;
 
+// parts of the squared norms of w: a quarter of the K step each, on two tiles of few rows, or the waves of one
+template <class C>
+constexpr int kNormParts = C::kWN == 1 ? 2 : C::kBK / 16;
+
 template <class C, int kMode>
 __global__ __launch_bounds__(C::kThreads) void scores_kernel(ScoreArgs p) {
   static_assert(C::kFM % 2 == 0, "a wave holds whole groups");
   const int wave = threadIdx.x >> 6, l = threadIdx.x & 63, hi = l >> 5;
-  gemm_tiles<C, kKC, kKC, kMode == kExpHalf || kMode == kExpFloat || kMode == kScores>(
+  gemm_tiles<C, kKC, kKC, kMode == kExpHalf || kMode == kExpFloat || kMode == kScores, kMode == kScores ? kNormParts<C> : 0>(
       p.w, p.x, p.kw, p.kx,
       [&](int j, int& m0, int& n0, int& kt0, int& nkt) {
         const int id = item_of(j, p.nm * p.nn);
@@ -200,7 +206,7 @@ __global__ __launch_bounds__(C::kThreads) void scores_kernel(ScoreArgs p) {
         m0 = tm * C::kBM, n0 = tn * C::kBN, kt0 = 0, nkt = (min(p.kw, p.kx) + C::kBK - 1) / C::kBK;
         return true;
       },
-      [&](int, int m0, int n0, f32x16(&acc)[C::kFM][C::kFN], const Turn& turn) {
+      [&](int, int m0, int n0, f32x16(&acc)[C::kFM][C::kFN], const Turn& turn, const float(&sq)[C::kFM]) {
         const int v0 = m0 + (wave / C::kWN) * C::kFM * 32, i0 = n0 + (wave % C::kWN) * C::kFN * 32;
         int label[C::kFN];
 #pragma unroll
@@ -212,6 +218,13 @@ __global__ __launch_bounds__(C::kThreads) void scores_kernel(ScoreArgs p) {
         for (int g = 0; g < C::kFM / 2; ++g) {
           const int vg = v0 + g * kGroup;
           if (vg >= p.V) break;
+          const int part = n0 / C::kBN * C::kWN + wave % C::kWN;
+          if (kMode == kScores && part < p.parts) {
+            float q = fmaxf(sq[2 * g] + __shfl_xor(sq[2 * g], 32, 64), sq[2 * g + 1] + __shfl_xor(sq[2 * g + 1], 32, 64));
+#pragma unroll
+            for (int o = 16; o; o >>= 1) q = fmaxf(q, __shfl_xor(q, o, 64));
+            if (l == 0) p.norms[(long long)part * ((p.V + kGroup - 1) / kGroup) + vg / kGroup] = q;
+          }
           if (p.bias) {  // (past the last class: the last one's bias, and -inf below)
             float b[2][16];
 #pragma unroll
@@ -329,7 +342,7 @@ struct FewArgs {
   long long ld;
   const void* label;
   int idx64;
-  float* zt;
+  float *zt, *norms;  // as in ScoreArgs, one part
 };
 
 // 4 floats from column c; zero past the end
@@ -370,8 +383,14 @@ __global__ __launch_bounds__(256, 2) void scores_few_kernel(FewArgs p) {
 #pragma unroll
   for (int t = 0; t < kNT; ++t) x[t] = p.x + (long long)min(i0 + t * 16 + r16, p.n - 1) * p.xrs;
   f32x4 acc[4][kNT] = {};
+  float sq[4] = {};  // this lane's part of the squared norms of four classes
   constexpr int kU = kNT > 2 ? 2 : 4;  // steps under way
   auto mma = [&](const f32x4 (&a)[4], const f32x4 (&b)[kNT]) {
+    if (kMode == kScores)
+#pragma unroll
+      for (int t = 0; t < 4; ++t)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) sq[t] = fmaf(a[t][j], a[t][j], sq[t]);
 #pragma unroll
     for (int j = 0; j < 4; ++j)
 #pragma unroll
@@ -400,8 +419,21 @@ __global__ __launch_bounds__(256, 2) void scores_few_kernel(FewArgs p) {
     for (int i = 0; i < kNT; ++i) b[i] = row4(x[i], c + g4 * 4, d1);
     mma(a, b);
   }
+  __shared__ float part[16][64];  // sums of squares of the 64 classes
+  if (kMode == kScores)
+#pragma unroll
+    for (int t = 0; t < 4; ++t) part[wave * 4 + g4][t * 16 + r16] = sq[t];
   f32x4 sum[4];
-  if (!few_sum<kNT>(acc, sum)) return;
+  const bool mine_too = few_sum<kNT>(acc, sum);
+  if (kMode == kScores && blockIdx.y == 0 && wave == 3) {  // (of up to 32 rows this wave has no scores)
+    float q = 0.0f;
+#pragma unroll
+    for (int u = 0; u < 16; ++u) q += part[u][l];
+#pragma unroll
+    for (int o = 32; o; o >>= 1) q = fmaxf(q, __shfl_xor(q, o, 64));
+    if (l == 0) p.norms[blockIdx.x] = q;
+  }
+  if (!mine_too) return;
   // lane: row l % 16 of the wave's tile, classes vg + 16 t + 4 (l / 16) + r
   const int row = i0 + wave * 16 + r16;
   const int label = kMode != kScores && p.label && row < p.n ? class_at(p.label, p.idx64, row, p.V) : -1;
@@ -674,6 +706,9 @@ struct RowArgs {
   float2* norm;         // [n] maximum (before the division by T) and 1 / sum: p = e^((z - max) / T) / sum, without the rounding of lse
   float* q;             // [n][k] g T q_j; of a label g (1 - p), all of its D
   int rb;               // rows per block (a power of two, <= 16)
+  float* norms;         // [parts][groups] or null: their sums go to the first, the largest sum is that of norm_max [4]
+  float* norm_max;
+  int parts;
 };
 
 // Scores and maxima are those before the division by T. kB2: bf16 inputs, whose exponentials are exp2 alone
@@ -684,6 +719,20 @@ __global__ __launch_bounds__(256) void row_kernel(RowArgs p) {
   auto ex = [&](float v) { return kB2 ? __builtin_amdgcn_exp2f(v * unit) : exp_of<true>(v * unit); };  // e^(v / T)
   const int t = threadIdx.x, rl = t & (p.rb - 1), strip = t / p.rb, strips = 256 / p.rb;
   const long long row = (long long)blockIdx.x * p.rb + rl;
+  if (p.norms && blockIdx.x == gridDim.x - 1) {  // a block of its own, behind those of the rows
+    float q = 0.0f;
+#pragma unroll 8
+    for (int g = t; g < p.groups; g += 256) {
+      float sum = p.norms[g];
+      for (int u = 1; u < p.parts; ++u) sum += p.norms[(long long)u * p.groups + g];
+      if (p.parts > 1) p.norms[g] = sum;
+      q = fmaxf(q, sum);
+    }
+#pragma unroll
+    for (int o = 32; o; o >>= 1) q = fmaxf(q, __shfl_xor(q, o, 64));
+    if ((t & 63) == 0) p.norm_max[t >> 6] = q;
+    return;
+  }
   // running maximum and sum over this thread's groups
   float m = -INFINITY, s = 0.0f;
   if (row < p.n) {
@@ -1012,7 +1061,7 @@ __global__ __launch_bounds__(C::kThreads) void grad_kernel(GradArgs p) {
         kt0 = k0 / C::kBK, nkt = (k1 - k0 + C::kBK - 1) / C::kBK;
         return true;
       },
-      [&](int j, int m0, int n0, f32x16(&acc)[C::kFM][C::kFN], const Turn&) {
+      [&](int j, int m0, int n0, f32x16(&acc)[C::kFM][C::kFN], const Turn&, const float(&)[C::kFM]) {
         int id, run;
         grad_item(p, j, id, run);
         const int mw = m0 + (wave / C::kWN) * C::kFM * 32, nw = n0 + (wave % C::kWN) * C::kFN * 32;
@@ -1137,12 +1186,18 @@ __global__ __launch_bounds__(256) void split_sum_kernel(const float* __restrict_
 //      (maximum, lower group) do: each of them holds a score that beats everything outside.
 //   2. the scores >= tau of those groups, as 64-bit keys (score order, then lower class)
 //   3. the kc largest keys
-//   4. their scores again as 64-bit sums, so that the order returned is that of the exact scores, and
-//      the k largest of them in order
+//   4. their scores again as 64-bit sums, and the k largest of them in order
+//   5. A class that is no candidate has an fp32 score of at most the candidates' least, `cut`. Where the k-th 64-bit score is
+//      above cut by more than fp32 scores are off, no such class belongs to the k best, and the row is done. Otherwise (scores that
+//      lie closer together than fp32 tells apart: a common offset, sums that cancel, equal classes) every class whose
+//      fp32 score reaches the k-th less that error is scored in 64 bits too, in turns of up to 768 that are merged with
+//      the k best so far. So the classes and their order are those of the 64-bit scores for every row.
+//      How far an fp32 score may be off: Slack.
 constexpr int kSpare = 8, kSlack = 24;
 constexpr int kTopMax = 256;       // k at most
 constexpr int kTopHold = 8;        // group maxima per thread
 constexpr int kTopList = 2048;     // keys held in LDS; where more reach tau (ties), they are read again from memory
+constexpr int kTurnList = 768, kTurnAdd = 512;  // classes scored in 64 bits per turn, and added per step at most
 
 struct TopArgs {
   const float2* stats;
@@ -1154,6 +1209,22 @@ struct TopArgs {
   double inv_t;
   float* values;
   long long* classes;
+  const float *norms, *norm_max;
+  double slack;         // Slack::c
+};
+
+// What a 32-bit score (before the division by T) of a row with squared norm xx may be off against classes of squared norm <= ww,
+// where only scores of magnitude <= z matter: c 2^-24 of sum |x||w| <= |x| |w|, and the rounding of the bias's sum.
+// The fp32 matrix product of 4 rounds after every product (c = d), the bf16 one of 16 after every four (against exact sums: at most
+// 5.3 units per instruction; c = d / 2 counts 8). Joined accumulators, cut planes and dropped plane pairs take less than 64 units.
+// ww is summed in fp32 (fp32 inputs: of the largest planes, at most 2^-8 off): 1.02 + d 2^-23 times it, and squares that underflow
+// are below 2^-125 each.
+struct Slack {
+  double xx, c;
+  int d;
+  __device__ __forceinline__ double operator()(float ww, double z) const {
+    return 0x1p-24 * (c * sqrt(xx * (ww * (1.02 + d * 0x1p-23) + d * 0x1p-125)) + 2.0 * z) + c * 0x1p-125;
+  }
 };
 
 __device__ __forceinline__ unsigned order_key(float v) {
@@ -1165,6 +1236,12 @@ __device__ __forceinline__ unsigned long long order_key(double v) {
   if (v != v) return ~0ull;
   const unsigned long long u = __builtin_bit_cast(unsigned long long, v);
   return u >> 63 ? ~u : u | 1ull << 63;
+}
+__device__ __forceinline__ float key_value(unsigned key) {
+  return __builtin_bit_cast(float, key >> 31 ? key & 0x7fffffffu : ~key);
+}
+__device__ __forceinline__ double key_value(unsigned long long key) {
+  return __builtin_bit_cast(double, key >> 63 ? key & ~(1ull << 63) : ~key);
 }
 
 // k-th largest (k >= 1) of `count` keys; on return `above` keys are larger than the result and `same` equal it. All
@@ -1223,8 +1300,9 @@ __global__ __launch_bounds__(1024) void topk_kernel(TopArgs p) {
   __shared__ unsigned long long keys[kTopList];
   __shared__ int hist[256], pick[3], cnt, wcnt[2][8][16];
   __shared__ int sel[kTopMax + kSpare + kSlack];
-  __shared__ double zs[kTopMax + kSpare];
   __shared__ int cls[kTopMax + kSpare];
+  __shared__ double xx;
+  __shared__ unsigned long long cut;  // the least candidate's key
   // 16 rows share a line of the stats: rows next to each other go to one XCD (4096 rows of 65536 classes 241 -> 234 us: threshold
   // 58, scores gathered and ranked 45, 64-bit scores of 72 candidates 131)
   const int row = (int)(blockIdx.x & 7) * (int)(gridDim.x >> 3) + (int)(blockIdx.x >> 3);
@@ -1233,9 +1311,10 @@ __global__ __launch_bounds__(1024) void topk_kernel(TopArgs p) {
   const float2* st = p.stats + row;
   const float* z = p.z + (long long)row * p.ld;
   auto gkey = [&](int g) { return order_key(st[(long long)g * p.n].x); };
+  const float4 ww4 = *(const float4*)p.norm_max;
   int nsel = p.groups;
   unsigned tau = 0;
-  if (t == 0) cnt = 0;
+  if (t == 0) cnt = 0, cut = 0;
   const int enough = p.kc + min(kSlack, p.kc >> 2);
   if (p.groups > p.kc) {
     if (p.groups <= nt * kTopHold) {
@@ -1356,6 +1435,7 @@ __global__ __launch_bounds__(1024) void topk_kernel(TopArgs p) {
 #pragma unroll 4
       for (int o = 0; o < total; ++o) rank += keys[o] > mine;
       if (rank < p.kc) cls[rank] = (int)~(unsigned)mine;
+      if (rank == p.kc - 1) cut = mine;
     }
   } else {
     const bool listed = total <= kTopList;
@@ -1367,32 +1447,44 @@ __global__ __launch_bounds__(1024) void topk_kernel(TopArgs p) {
       const unsigned long long key = lkey(i);
       if (key >= least) cls[atomicAdd(&cnt, 1)] = (int)~(unsigned)key;
     }
+    if (t == 0) cut = least;
   }
   __syncthreads();
-  // exact scores of the kc candidates, a few at a time per wave: two, further ahead, where the waves suffice
-  auto dots = [&](auto tag) {
+  // 64-bit scores (before the division by T) of `count` classes as keys, a few at a time per wave: two, further ahead, where
+  // the waves suffice. The last wave, which has the least to do, also takes the row's own squares.
+  auto dots = [&](auto tag, const int* c, int count, unsigned long long* key, bool squares) {
     constexpr int kW = decltype(tag)::kW;
     const T *x = (const T*)p.x + row * p.xrs, *bias = (const T*)p.bias;
-    for (int c = wave * kW; c < p.kc; c += waves * kW) {
+    for (int c0 = wave * kW; c0 < count; c0 += waves * kW) {
       const T* w[kW];
 #pragma unroll
-      for (int u = 0; u < kW; ++u) w[u] = (const T*)p.w + (long long)cls[min(c + u, p.kc - 1)] * p.wrs;
+      for (int u = 0; u < kW; ++u) w[u] = (const T*)p.w + (long long)c[min(c0 + u, count - 1)] * p.wrs;
       double s[kW];
       row_dots<T, double, kW, 8 / kW>(x, p.xcs, w, p.wcs, p.d, p.vec, s);
       if (l == 0)
 #pragma unroll
         for (int u = 0; u < kW; ++u)
-          if (c + u < p.kc) {
-            zs[c + u] = (s[u] + (bias ? (double)Elem<T>::get(bias, cls[c + u]) : 0.0)) * p.inv_t;
-            keys[c + u] = order_key(zs[c + u]);
-          }
+          if (c0 + u < count) key[c0 + u] = order_key(s[u] + (bias ? (double)Elem<T>::get(bias, c[c0 + u]) : 0.0));
+    }
+    if (squares && wave == waves - 1) {
+      const T* w[1] = {x};
+      double s[1];
+      row_dots<T, double, 1, 4>(x, p.xcs, w, p.xcs, p.d, p.vec, s);
+      if (l == 0) xx = s[0];
     }
   };
+  const bool all = p.kc == p.V;  // every class is a candidate
   if (p.kc <= 2 * waves)
-    dots(DotTag<2>());
+    dots(DotTag<2>(), cls, p.kc, keys, !all);
   else
-    dots(DotTag<4>());
+    dots(DotTag<4>(), cls, p.kc, keys, !all);
   __syncthreads();
+  // the k best so far (and room for the next), behind the candidates' keys and a turn's classes
+  unsigned long long *bkey = &keys[kTurnList + kTurnList / 2], *nkey = bkey + kTopMax + kTopMax / 2;
+  int *bcls = (int*)(bkey + kTopMax), *ncls = (int*)(nkey + kTopMax);
+  static_assert(kTurnList + kTurnList / 2 + 3 * kTopMax <= kTopList, "");
+  float* values = p.values + (long long)row * p.k;
+  long long* classes = p.classes + (long long)row * p.k;
   for (int c = t; c < p.kc; c += nt) {
     const unsigned long long mine = keys[c];
     const int v = cls[c];
@@ -1400,9 +1492,74 @@ __global__ __launch_bounds__(1024) void topk_kernel(TopArgs p) {
 #pragma unroll 4
     for (int o = 0; o < p.kc; ++o) rank += keys[o] > mine || (keys[o] == mine && cls[o] < v);
     if (rank < p.k) {
-      p.values[(long long)row * p.k + rank] = (float)zs[c];
-      p.classes[(long long)row * p.k + rank] = v;
+      values[rank] = (float)(key_value(mine) * p.inv_t);
+      classes[rank] = v;
+      bkey[rank] = mine, bcls[rank] = v;
     }
+  }
+  if (all) return;
+  __syncthreads();
+  double zk = key_value(bkey[p.k - 1]);
+  const double zc = key_value((unsigned)(cut >> 32));
+  const Slack slack = {xx, p.slack, p.d};
+  // (classes at -inf are switched off, in 64 bits too; comparisons with NaN are false: such a row has some classes)
+  const float ww = fmaxf(fmaxf(ww4.x, ww4.y), fmaxf(ww4.z, ww4.w));
+  if (!(zk <= zc + slack(ww, fmax(fabs(zk), fabs(zc)))) || zc == -INFINITY) return;
+
+  // classes of this turn and their keys
+  int* tcls = (int*)&keys[kTurnList];
+  unsigned long long* tkey = keys;
+  auto reach = [&](int g) { return zk - slack(p.norms[g], fabs(zk)); };  // what a score of group g has to reach
+  auto merge = [&]() {  // all threads, with the list written; cnt is 0 afterwards
+    const int listed = cnt, total = p.k + listed;
+    dots(DotTag<4>(), tcls, listed, tkey, false);
+    __syncthreads();
+    auto keyed = [&](int e) { return e < p.k ? bkey[e] : tkey[e - p.k]; };
+    auto classed = [&](int e) { return e < p.k ? bcls[e] : tcls[e - p.k]; };
+    for (int e = t; e < total; e += nt) {
+      const unsigned long long mine = keyed(e);
+      const int v = classed(e);
+      int rank = 0;
+      for (int o = 0; o < total; ++o) rank += keyed(o) > mine || (keyed(o) == mine && classed(o) < v);
+      if (rank < p.k) nkey[rank] = mine, ncls[rank] = v;
+    }
+    if (t == 0) cnt = 0;
+    __syncthreads();
+    unsigned long long* const k = bkey;
+    int* const c = bcls;
+    bkey = nkey, bcls = ncls, nkey = k, ncls = c;
+    zk = key_value(bkey[p.k - 1]);
+  };
+  __syncthreads();  // the candidates' keys have been read
+  if (t == 0) cnt = 0;
+  // groups in pieces of 256, those of a piece that reach far enough in `hist`; eight groups per step
+  for (int g0 = 0; g0 < p.groups; g0 += 256) {
+    if (t == 0) pick[0] = 0;
+    __syncthreads();
+    if (t < 256 && g0 + t < p.groups && (double)st[(long long)(g0 + t) * p.n].x >= reach(g0 + t)) hist[atomicAdd(&pick[0], 1)] = g0 + t;
+    __syncthreads();
+    const int listed = pick[0];
+    for (int s0 = 0; s0 < listed; s0 += kTurnAdd / kGroup) {
+      const int have = cnt;
+      __syncthreads();  // every wave has read it before one adds to it: all merge or none
+      if (have > kTurnList - kTurnAdd) merge();
+      for (int u = wave; u < kTurnAdd / kGroup && s0 + u < listed; u += waves) {
+        const int g = hist[s0 + u], v = g * kGroup + l;
+        const float zv = z[min(v, p.V - 1)];
+        const bool take = v < p.V && (double)zv >= reach(g) && ((unsigned long long)order_key(zv) << 32 | (unsigned)~v) < cut;
+        const unsigned long long m = __ballot(take);
+        int base = 0;
+        if (l == 0 && m) base = atomicAdd(&cnt, __popcll(m));
+        base = __builtin_amdgcn_readfirstlane(base) + __popcll(m & ((1ull << l) - 1));
+        if (take) tcls[base] = v;
+      }
+      __syncthreads();
+    }
+  }
+  merge();
+  for (int c = t; c < p.k; c += nt) {
+    values[c] = (float)(key_value(bkey[c]) * p.inv_t);
+    classes[c] = bcls[c];
   }
 }
 
@@ -1419,6 +1576,8 @@ typedef TileCfg<128, 128, 2, 2, 32, 4> CfgMid;   // 0.85 - 1.05 (bound by L2 rea
 typedef TileCfg<128, 128, 2, 2, 32, 10> CfgDeep; // the same tile where one round of blocks does: nine stages under way
 typedef TileCfg<128, 128, 2, 4, 32, 3, 3> CfgF32; // three planes
 typedef TileCfg<128, 32, 2, 1, 64, 4> CfgSlim;   // few rows: bound by reading w
+
+constexpr int kMostParts = 4;  // of kNormParts
 
 constexpr unsigned kLdsAll = 160 * 1024;
 
@@ -1468,10 +1627,12 @@ static long long run_bytes(const Layout& l, long long m, long long n) {
 // one round of Mid tiles: a block alone on its CU, so the latency of its K steps counts
 static bool use_deep(long long tiles) { return tiles <= 256; }
 
+// returns the parts of the squared norms
 template <class C>
-void scores_launch(ScoreArgs p, int mode, hipStream_t s) {
+int scores_launch(ScoreArgs p, int mode, hipStream_t s) {
   p.nm = ceil_div(p.V, C::kBM);
   p.nn = ceil_div(p.n, C::kBN);
+  p.parts = C::kWN * p.nn < kNormParts<C> ? 1 : kNormParts<C>;
   const int g = grid8((long long)p.nm * p.nn, kLdsAll / C::kLds);
 #define YTK_SC(M) scores_kernel<C, M><<<g, C::kThreads, C::kLds, s>>>(p)
   if constexpr (C::kPlanes == 3) {
@@ -1491,6 +1652,7 @@ void scores_launch(ScoreArgs p, int mode, hipStream_t s) {
   }
 #undef YTK_SC
   YTK_LAUNCH_CHECK();
+  return p.parts;
 }
 
 template <class C, int LA, int LB, typename T>
@@ -1533,7 +1695,7 @@ struct HeadPlan {
   bool pack_x, pack_w, grads, few, few_dw, planes_d;
   int rw, few_per, few_runs;
   bool many;  // more than one piece of rows
-  long long o_x, o_w, o_xg, o_e, o_d, o_stats, o_zt, o_q, o_coef, o_norm, o_part, o_dbacc, o_dwacc, o_split, bytes;
+  long long o_x, o_w, o_xg, o_e, o_d, o_stats, o_zt, o_q, o_coef, o_norm, o_part, o_dbacc, o_dwacc, o_split, o_wn, bytes;
 };
 
 static HeadPlan head_plan(const HeadIn& h, bool topk) {
@@ -1592,6 +1754,7 @@ static HeadPlan head_plan(const HeadIn& h, bool topk) {
   p.o_dbacc = take(db, h.V * 4);
   p.o_dwacc = take(h.want_dw && p.many, h.V * h.d * 4);
   p.o_split = take(part > 0, part);
+  p.o_wn = take(topk, (kMostParts * p.groups + 4) * 4);  // four, the largest of which is the largest squared norm of w; that of each group
   p.bytes = o;
   return p;
 }
@@ -1703,6 +1866,7 @@ static void scores_few(const HeadIn& h, const HeadPlan& p, const void* x, const 
   a.stats = (float2*)(ws + p.o_stats);
   a.e = (float*)(ws + p.o_e);
   a.ld = p.ld;
+  a.norms = (float*)(ws + p.o_wn) + 4;
   if (h.n <= 16)
     scores_few_n<1>(a, mode, s);
   else if (h.n <= 32)
@@ -1747,7 +1911,8 @@ static void dw_few(const HeadIn& h, const HeadPlan& p, const void* x, char* ws, 
   YTK_LAUNCH_CHECK();
 }
 
-static void scores(const HeadIn& h, const HeadPlan& p, const HeadOps& o, long long r0, long long rows, const void* bias, float temp,
+// returns the parts of the squared norms of w (scores that are kept)
+static int scores(const HeadIn& h, const HeadPlan& p, const HeadOps& o, long long r0, long long rows, const void* bias, float temp,
                    char* ws, int mode, const void* label, hipStream_t s) {
   ScoreArgs a = {};
   a.label = label, a.idx64 = (int)h.idx64, a.zt = (float*)(ws + p.o_zt);
@@ -1763,19 +1928,19 @@ static void scores(const HeadIn& h, const HeadPlan& p, const HeadOps& o, long lo
   a.e = ws + p.o_e;
   a.z = (float*)(ws + p.o_e);
   a.ld = p.ld;
+  a.norms = (float*)(ws + p.o_wn) + 4;
   const int tile = pick_layout(h.V, rows, p.kp, p.terms, false).cfg;
   if (h.f32)
-    scores_launch<CfgF32>(a, mode, s);
-  else if (rows <= 64)
-    scores_launch<CfgSlim>(a, mode, s);
-  else if (tile == kBig)
-    scores_launch<CfgBig>(a, mode, s);
-  else if (tile == kWide)
-    scores_launch<CfgWide>(a, mode, s);
-  else if (use_deep((long long)ceil_div(h.V, 128) * ceil_div(rows, 128)))
-    scores_launch<CfgDeep>(a, mode, s);
-  else
-    scores_launch<CfgMid>(a, mode, s);
+    return scores_launch<CfgF32>(a, mode, s);
+  if (rows <= 64)
+    return scores_launch<CfgSlim>(a, mode, s);
+  if (tile == kBig)
+    return scores_launch<CfgBig>(a, mode, s);
+  if (tile == kWide)
+    return scores_launch<CfgWide>(a, mode, s);
+  if (use_deep((long long)ceil_div(h.V, 128) * ceil_div(rows, 128)))
+    return scores_launch<CfgDeep>(a, mode, s);
+  return scores_launch<CfgMid>(a, mode, s);
 }
 
 // whole, aligned 16-byte pieces in the rows of x and w
@@ -1800,7 +1965,7 @@ static void rows_pass(RowArgs a, bool base2, hipStream_t s) {
   if (base2)
     row_kernel<true><<<ceil_div(a.n, a.rb), 256, 0, s>>>(a);
   else
-    row_kernel<false><<<ceil_div(a.n, a.rb), 256, 0, s>>>(a);
+    row_kernel<false><<<ceil_div(a.n, a.rb) + (a.norms ? 1 : 0), 256, 0, s>>>(a);
   YTK_LAUNCH_CHECK();
 }
 
@@ -1948,14 +2113,17 @@ extern "C" void ytk_head_topk(const uintptr_t* ptrs, const long long* lp, double
   const HeadOps o = head_operands(h, p, x, w, ws, s);
   for (long long r0 = 0; r0 < h.n; r0 += p.piece) {
     const long long rows = std::min(p.piece, h.n - r0);
+    int parts = 1;
     if (p.few)
       scores_few(h, p, x, w, bias, (float)temp_, ws, kScores, nullptr, s);
     else
-      scores(h, p, o, r0, rows, bias, (float)temp_, ws, kScores, nullptr, s);
+      parts = scores(h, p, o, r0, rows, bias, (float)temp_, ws, kScores, nullptr, s);
     RowArgs r = {};
+    r.parts = parts;
     r.stats = (const float2*)(ws + p.o_stats);
     r.groups = (int)p.groups, r.n = (int)rows, r.V = (int)h.V;
     r.inv_t = 1.0f / (float)temp_;
+    r.norm_max = (float*)(ws + p.o_wn), r.norms = r.norm_max + 4;
     r.lse = (float*)ptrs[6] + r0;
     rows_pass(r, false, s);
     TopArgs t = {};
@@ -1968,6 +2136,8 @@ extern "C" void ytk_head_topk(const uintptr_t* ptrs, const long long* lp, double
     t.x = x + r0 * h.xrs * el, t.w = w, t.bias = bias;
     t.xrs = h.xrs, t.xcs = h.xcs, t.wrs = h.wrs, t.wcs = h.wcs;
     t.inv_t = 1.0 / temp_;
+    t.norms = r.norms, t.norm_max = r.norm_max;
+    t.slack = (p.few ? 1.0 : 0.5) * h.d + 64.0;
     t.values = (float*)ptrs[4] + r0 * h.k;
     t.classes = (long long*)ptrs[5] + r0 * h.k;
     const int threads = rows < 256 ? 1024 : 256;  // fewer rows than CUs: more waves for each

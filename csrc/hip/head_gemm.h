@@ -198,17 +198,28 @@ struct Turn {
   }
 };
 
+// The squared norms of A's rows, as the products run: quarter q of a K step is taken by part q % kOf, and the waves that share A's
+// rows, in one tile or in tiles side by side, take a part each (kOf = 0: none). Taken whole by every wave they cost 78 us of
+// 650 (4096 x 65536, K = 1024); by one wave of the first tile, whose steps the others wait for, 13 there and 10 of 85 at
+// 300 x 32003, K = 2048; in parts 0 and 6.
+template <int kOf, int kIs>
+struct Part {
+  static constexpr bool takes(int q) { return kOf > 0 && q % (kOf > 0 ? kOf : 1) == kIs; }
+};
+
 // One block's tiles, one after the other: tile(j, m0, n0, kt0, nkt) tells its j-th (false: no more; nkt >= 1 steps
-// of kBK from step kt0), done(j, m0, n0, acc, turn) takes the accumulators, with a free stage to turn them in
-// where kTurn. The DMA runs S - 1 stages ahead across
+// of kBK from step kt0), done(j, m0, n0, acc, turn, sq) takes the accumulators, with a free stage to turn them in
+// where kTurn, and with kParts > 0 the lane's part of the squared norms of A's rows: of row l % 32 of fragment i, half of the elements
+// (lane l + 32 has the others) of its part, three planes by the largest. Wave wn of the t-th tile along n has part
+// t kWN + wn, if that is below `parts` (kParts, or 1 where there are fewer such waves than kParts). The DMA runs S - 1 stages ahead across
 // the border of two tiles, so only the epilogue's own instructions stand between their products. (Its stores share the
 // counter of the DMA, which counts down in the order of issue.)
 // ka, kb: extent of K in each operand's memory, a multiple of 8 for a KC operand; both reach every step:
 // (kt0 + nkt - 1) * kBK < min(ka, kb). Past it an operand counts as zero, whatever its memory holds there (a KC operand
 // whose K is no multiple of kBK: in the last step of every tile, so its tiles all run to the end of K).
-template <class C, int kLA, int kLB, bool kTurn, class FTile, class FDone>
+template <class C, int kLA, int kLB, bool kTurn, int kParts = 0, class FTile, class FDone>
 __device__ __forceinline__ void gemm_tiles(const Operand& A, const Operand& B, long long ka, long long kb, FTile tile,
-                                           FDone done) {
+                                           FDone done, int parts = kParts) {
   extern __shared__ __align__(1024) char head_smem[];
   typedef __attribute__((address_space(3))) char lc;
   const unsigned lds = (unsigned)(uintptr_t)(lc*)head_smem;
@@ -295,6 +306,8 @@ __device__ __forceinline__ void gemm_tiles(const Operand& A, const Operand& B, l
     // three planes: the five small pairs have sums of their own and the large one has two, so that these are rounded
     // less often and at a smaller size
     f32x16 acc[C::kFM][C::kFN] = {}, odd[C::kFM][C::kFN] = {}, low[C::kFM][C::kFN] = {};
+    float sq[C::kFM] = {};
+    auto steps = [&](auto part) {
     for (int left = nkt; left > 0; --left) {
       const unsigned after = so + C::kStageBytes == C::kLds ? 0u : so + C::kStageBytes;
 #pragma unroll
@@ -327,11 +340,37 @@ __device__ __forceinline__ void gemm_tiles(const Operand& A, const Operand& B, l
 #pragma unroll
             for (int u = slot * kLoads / kSlots; u < (slot + 1) * kLoads / kSlots; ++u) piece(u, fill);
           }
+          if (decltype(part)::takes(q)) {
+            typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+            const bf16x8 f = fa[q & 1][0][i];
+#pragma unroll
+            for (int u = 0; u < 8; u += 2) {
+              const bf16x2 v = {f[u], f[u + 1]};
+              sq[i] = __builtin_amdgcn_fdot2_f32_bf16(v, v, sq[i], false);
+            }
+          }
           __builtin_amdgcn_sched_barrier(0);
         }
       }
       so = after;
       fill = fill + C::kStageBytes == C::kLds ? 0u : fill + C::kStageBytes;
+    }
+    };
+    const int part = n0 / C::kBN * C::kWN + wn;
+    if constexpr (kParts == 0) {
+      steps(Part<0, 0>());
+    } else if (part >= parts) {
+      steps(Part<0, 0>());
+    } else if (C::kWN < kParts && parts == 1) {
+      steps(Part<C::kWN < kParts ? 1 : 0, 0>());
+    } else if (part == 0) {
+      steps(Part<kParts, 0>());
+    } else if (kParts == 2 || part == 1) {
+      steps(Part<kParts, 1>());
+    } else if (part == 2) {
+      steps(Part<kParts, kParts == 4 ? 2 : 0>());
+    } else {
+      steps(Part<kParts, kParts == 4 ? 3 : 0>());
     }
     if (P == 3)
 #pragma unroll
@@ -340,7 +379,7 @@ __device__ __forceinline__ void gemm_tiles(const Operand& A, const Operand& B, l
         for (int j = 0; j < C::kFN; ++j) acc[i][j] += odd[i][j] + low[i][j];
     // the stage to be filled next is free: every wave has read it (last barrier), and none fills it before the next one
     static_assert(C::kStageBytes >= 4096u * C::kNW, "");
-    done(j, m0, n0, acc, Turn{lds + fill + wave * 4096u});
+    done(j, m0, n0, acc, Turn{lds + fill + wave * 4096u}, sq);
     if (kTurn) {
       wait_lgkm();
       __builtin_amdgcn_s_barrier();

@@ -1,5 +1,5 @@
-"""Class head where the scores lie far from 0: common offsets, groups of 64 classes that hold nothing but
-switched-off classes or the label, and masks of large negative biases.
+"""Class head where the scores lie far from 0 or close together: common offsets, groups of 64 classes that hold nothing but
+switched-off classes or the label, masks of large negative biases, and scores nearer to each other than fp32 tells apart.
 
 Bounds as in test_head.py: they count |bias| in every score's rounding, so they grow with the offset.
 """
@@ -122,3 +122,57 @@ def test_label_at_the_lowest_bias(cuda, dtype, n):
     b[off] = -1e30
     for a, c in zip(r[2:], head.softmax_head_loss(x, w, y, bias=b)[2:]):
         assert bool(a.isfinite().all()) and torch.equal(a, c)
+
+
+def _close_scores(kind, n, d, V, dtype, dev):
+    """Scores that 64-bit sums tell apart and 32-bit ones do not."""
+    g = torch.Generator().manual_seed(V + n)
+    x, w = torch.randn(n, d, generator=g), torch.randn(V, d, generator=g)
+    b = None
+    if kind == "bias":  # a common bias of 64 and differences of 1e-6: below its rounding of 4e-6
+        w, b = w * 1e-7, torch.full((V,), 64.0)
+    elif kind == "column":  # a common product of 10^6 beside the others
+        x[:, d // 2], w[:, d // 2] = 1000.0, 1000.0
+    elif kind == "cancel":  # 3 is lost beside 10^9, which another column takes away again
+        w = w * (0.5 / d ** 0.5)
+        x[:, 0] = x[:, d // 2] = x[:, d - 1] = 1.0
+        w[:, 0], w[:, d - 1] = 1e9, -1e9
+        w[:, d // 2] = (torch.arange(V) * 7919 % V).float() / V
+    elif kind == "outlier":  # the same in one class alone, beside ordinary ones
+        w = w * (0.5 / d ** 0.5)
+        x[:, 0] = x[:, d // 2] = x[:, d - 1] = 1.0
+        w[V - 2] = 0.0
+        w[V - 2, 0], w[V - 2, d // 2], w[V - 2, d - 1] = 1e9, 12.0, -1e9
+    elif kind == "same":  # every class alike
+        w[:] = w[0]
+    elif kind == "zero":
+        w[:] = 0.0
+    return x.to(dtype).to(dev), w.to(dtype).to(dev), None if b is None else b.to(dtype).to(dev)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", BOTH)
+@pytest.mark.parametrize("kind", ["bias", "column", "cancel", "outlier", "same", "zero"])
+@pytest.mark.parametrize("n,d,V,k", [(1, 64, 3000, 5), (7, 130, 3000, 256), (70, 64, 700, 40), (300, 64, 3000, 1), (300, 72, 1009, 200),
+                                     (2, 40, 140001, 30)])
+def test_topk_of_scores_that_32_bits_mix_up(cuda, dtype, kind, n, d, V, k):
+    """The k best and their order are those of the 64-bit sums, whatever the 32-bit scores say."""
+    x, w, b = _close_scores(kind, n, d, V, dtype, cuda)
+    T = 2.0 if k % 2 == 0 else 1.0
+    v, c, _ = head.head_topk(x, w, k, bias=b, temperature=T)
+    z = x.double() @ w.double().t()
+    z = (z if b is None else z + b.double()) / T
+    # the two 64-bit sums add in other orders: each is off by d 2^-53 sum |x||w| at most
+    e = (d + 4) * 2.0 ** -53 * (x.double().abs() @ w.double().abs().t() + (0 if b is None else b.double().abs())) / T
+    rv, rc = z.sort(dim=1, descending=True, stable=True)
+    got = z.gather(1, c)
+    bound = e.amax(1, keepdim=True)
+    assert all(len(set(r)) == k for r in c.tolist())
+    assert bool(((got - rv[:, :k]).abs() <= 2 * bound).all())
+    apart = (rv[:, :k] - rv[:, 1:k + 1] > 4 * bound) & (torch.cat([rv.new_full((n, 1), float("inf")), rv[:, :k - 1]], 1) - rv[:, :k] > 4 * bound)
+    assert torch.equal(c[apart], rc[:, :k][apart])
+    if kind in ("same", "zero"):
+        assert c.tolist() == [list(range(k))] * n
+    else:
+        assert float(apart.double().mean()) > 0.5
+    near(v, rv[:, :k].cpu(), (1.01 * U * rv[:, :k].abs() + 2 * bound).cpu() + 1e-40, "values")

@@ -176,8 +176,9 @@ def distill_head_loss(x: torch.Tensor, w: torch.Tensor, top_idx: torch.Tensor, t
 def head_topk(x: torch.Tensor, w: torch.Tensor, k: int, bias: Optional[torch.Tensor] = None, temperature: float = 1.0):
     """(values [n, k] fp32 descending, classes [n, k] int64, lse [n] fp32) of the scores (x w^T + bias) / T.
 
-    The order is that of the scores summed in 64 bits, equal scores to the lower class (k + 8 candidates are found in
-    32 bits and scored again). 1 <= k <= min(V, 256). A row that holds NaN scores has some classes
+    Classes and order are those of the scores summed in 64 bits, equal scores to the lower class: k + 8 candidates are found
+    in 32 bits and scored again, and so is every other class that the 32-bit scores' error leaves possible (rows whose best
+    scores lie closer together than 32 bits tell apart take longer, up to a 64-bit score of every class). 1 <= k <= min(V, 256). A row that holds NaN scores has some classes
     in some order, and lse NaN."""
     _check(x, w, bias, temperature)
     n, V, dev = x.shape[0], w.shape[0], x.device
