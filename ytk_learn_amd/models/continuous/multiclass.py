@@ -28,9 +28,10 @@ from .base import ContinuousModelBase, jfloat
 
 
 def dense_rows(X) -> torch.Tensor:
-    """The rows of a SparseMatrix as a dense fp32 [n, ncols] matrix."""
+    """The rows of a SparseMatrix as a dense fp32 [n, ncols] matrix. A feature named more than once in a row adds up in an order
+    that does not change (index_put_ sorts the places; index_add_ would use atomics)."""
     out = torch.zeros(X.n * X.ncols, dtype=torch.float32, device=X.device)
-    out.index_add_(0, X.rows_of_nnz.long() * X.ncols + X.indices.long(), X.values)
+    out.index_put_((X.rows_of_nnz.long() * X.ncols + X.indices.long(),), X.values, accumulate=True)
     return out.view(X.n, X.ncols)
 
 
