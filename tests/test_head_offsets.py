@@ -176,3 +176,92 @@ def test_topk_of_scores_that_32_bits_mix_up(cuda, dtype, kind, n, d, V, k):
     else:
         assert float(apart.double().mean()) > 0.5
     near(v, rv[:, :k].cpu(), (1.01 * U * rv[:, :k].abs() + 2 * bound).cpu() + 1e-40, "values")
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", BOTH)
+@pytest.mark.parametrize("n", [3, 300])
+def test_topk_of_close_scores_in_pieces_strides_and_graphs(cuda, dtype, n, monkeypatch):
+    """Rows scored again in 64 bits, beside ordinary ones: the same answers from transposed weights, in pieces of rows, and from a
+    captured call replayed on other inputs."""
+    k, V, d = 40, 1500, 64
+    sets = []
+    for seed in range(3):
+        x, w, b = _close_scores("bias", n, d, V, dtype, cuda)
+        x = x.roll(seed, 0)
+        x[::2] *= 2.0 ** (20 + seed)  # scores that 32 bits do tell apart
+        sets.append((x, w.roll(seed, 0), b))
+    want = [head.head_topk(*s[:2], k, bias=s[2]) for s in sets]
+    for (x, w, b), (v, c, l) in zip(sets, want):
+        assert torch.equal(c, topk_ref(x, w, b, 1.0, k)[1])
+        got = head.head_topk(x, w.t().contiguous().t(), k, bias=b)
+        assert torch.equal(got[0], v) and torch.equal(got[1], c)
+    x, w, b = (t.clone() for t in sets[0])
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        head.head_topk(x, w, k, bias=b)
+    torch.cuda.current_stream().wait_stream(side)
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        out = head.head_topk(x, w, k, bias=b)
+    for i in (1, 2, 0, 1):
+        for t, s in zip((x, w, b), sets[i]):
+            t.copy_(s)
+        g.replay()
+        eager = head.head_topk(x, w, k, bias=b)
+        torch.cuda.synchronize()
+        for a, e, u in zip(out, eager, want[i]):
+            assert torch.equal(a, e) and torch.equal(a, u)
+    monkeypatch.setattr(head, "PIECE_BYTES", 1 << 10)
+    for s, u in zip(sets, want):
+        for a, e in zip(head.head_topk(*s[:2], k, bias=s[2]), u):
+            assert torch.equal(a, e)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", BOTH)
+@pytest.mark.parametrize("n,d,V", [(2, 1 << 21, 3), (140, 1 << 21, 3), (2, 3, 1 << 21), (140, 2, 1 << 21)])
+def test_most_features_and_classes(cuda, dtype, n, d, V):
+    """The documented limits: 2^21 features, 2^21 classes."""
+    g = torch.Generator(device=cuda).manual_seed(d + n)
+    x = torch.randn(n, d, generator=g, device=cuda).to(dtype)
+    w = (torch.randn(V, d, generator=g, device=cuda) * (2.0 / d ** 0.5)).to(dtype)
+    y = torch.randint(0, V, (n,), generator=g, device=cuda)
+    r = head.softmax_head_loss(x, w, y)
+    v, c, l = head.head_topk(x, w, min(V, 9))
+    z = x.double() @ w.double().t()
+    assert torch.equal(c, z.sort(dim=1, descending=True, stable=True).indices[:, :9])
+    lse = torch.logsumexp(z, 1)
+    # a score is a sum of d products: off by at most (d + 64) u sum |x||w|, and that is at most |x| |w|
+    ez = (d + 64) * U * (x.double().norm(dim=1) * w.double().norm(dim=1).max())
+    near(r.lse, lse.cpu(), (ez + (128 + V / 64) * U * (1 + lse.abs())).cpu(), "lse")
+    near(l, lse.cpu(), (ez + (128 + V / 64) * U * (1 + lse.abs())).cpu(), "lse of the best")
+    near(r.loss, (lse - z.gather(1, y[:, None])[:, 0]).cpu(), (2 * ez + (256 + V / 32) * U * (1 + lse.abs())).cpu(), "loss")
+    D = torch.softmax(z, 1)
+    D[torch.arange(n, device=cuda), y] -= 1
+    rel = torch.expm1((2 * ez).clamp(max=1.0))[:, None] + 2.0 ** -6
+    for got, D2, o in ((r.dx, D, w), (r.dw, D.t(), x)):
+        eD = (D.abs() * rel + 2.0 ** -38) if D2 is D else (D.abs() * rel + 2.0 ** -38).t()
+        want = D2 @ o.double()
+        bound = eD @ o.double().abs() + 2.0 ** -7 * want.abs() + 1e-30
+        bad = (got.double() - want).abs() > bound
+        assert not bool(bad.any()), float(((got.double() - want).abs() / bound).max())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", BOTH)
+@pytest.mark.parametrize("n", [5, 150])
+@pytest.mark.parametrize("T", [1e-6, 1e-3, 1e3, 1e6])
+def test_distill_at_extreme_temperatures(cuda, dtype, n, T):
+    """The documented limits of the temperature, with a group switched off."""
+    V = 200
+    x, w, _, _ = make(n, 64, V, dtype, cuda)
+    b = torch.zeros(V, dtype=dtype, device=cuda)
+    b[64:128] = float("-inf")
+    idx, tl = lists(n, 64, 6)
+    for tlse in (None, torch.logsumexp(tl.double() / T, 1).float()):
+        r = head.distill_head_loss(x, w, idx.to(cuda), tl.to(cuda), bias=b, temperature=T, top_lse=None if tlse is None else tlse.to(cuda))
+        assert all(bool(t.isfinite().all()) for t in r)
+        if tlse is None or T >= 1:  # (t / T - top_lse of 10^6 has a rounding of its own, which q shows)
+            Ref(x, w, idx, list_targets(idx, tl, T, tlse), bias=b, T=T).check(r, db=True)
