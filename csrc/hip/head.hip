@@ -6,10 +6,12 @@
 //            dx = D w, dw = D^T x, db = sum_i D
 //   top k:   the k largest z of each row and lse
 //
-// Rows are taken in pieces so that at most `piece_bytes` of exponentials live at a time. Per piece:
-//   1. scores_kernel   z by MFMA (top k: also the largest squared norm of w in each group); per row and group of 64 classes the maximum m and sum s of e^(z - m); with
+// Rows are taken in pieces so that at most `piece_bytes` of exponentials (256 rows of them at least) live at a time. Per piece:
+//   1. scores_kernel   z by MFMA; per row and group of 64 classes the maximum m and sum s of e^(z - m); with
 //                      gradients also E = e^(z - m) (bf16 inputs: as fp16 scaled by 2^15, 11 bits, so that
-//                      the one rounding that matters is D's own to bf16; fp32 inputs: fp32)
+//                      the one rounding that matters is D's own to bf16; a class more than 20 below its group's maximum
+//                      has fewer bits, and from 27 on its p, then below 2 10^-12 of that maximum's, counts as 0 in D, not in lse;
+//                      fp32 inputs: fp32); top k: also the largest squared norm of w in each group.
 //                      Maxima, and scores that are kept, are those before the division by T. A difference is taken before
 //                      it is scaled: the maximum's own exponent is exactly 0 and no other is above it, however large
 //                      the scores are (z / T - m / T in one fma keeps the rounding of m / T, 2^-24 of it: unbounded).
@@ -1303,8 +1305,7 @@ __global__ __launch_bounds__(1024) void topk_kernel(TopArgs p) {
   __shared__ int cls[kTopMax + kSpare];
   __shared__ double xx;
   __shared__ unsigned long long cut;  // the least candidate's key
-  // 16 rows share a line of the stats: rows next to each other go to one XCD (4096 rows of 65536 classes 241 -> 234 us: threshold
-  // 58, scores gathered and ranked 45, 64-bit scores of 72 candidates 131)
+  // 16 rows share a line of the stats: rows next to each other go to one XCD (4096 rows of 65536 classes 241 -> 234 us)
   const int row = (int)(blockIdx.x & 7) * (int)(gridDim.x >> 3) + (int)(blockIdx.x >> 3);
   if (row >= p.n) return;
   const int t = threadIdx.x, nt = blockDim.x, wave = t >> 6, waves = nt >> 6, l = t & 63;
@@ -1572,7 +1573,8 @@ inline int grid8(long long tiles, int per_cu) { return (int)std::min<long long>(
 // Tiles, with the rate of a long product (32768 x 8192 x 4096 and its two transposes, random data):
 typedef TileCfg<256, 256, 2, 4, 32, 5> CfgBig;   // 1.39 PFLOP/s; all 160 KB of LDS, one block per CU
 typedef TileCfg<128, 256, 2, 4, 64, 3> CfgWide;  // 1.25 - 1.35
-typedef TileCfg<128, 128, 2, 2, 32, 4> CfgMid;   // 0.85 - 1.05 (bound by L2 reads), two blocks per CU
+typedef TileCfg<128, 128, 2, 2, 32, 4> CfgMid;   // 0.85 - 1.05 (bound by L2 reads); two blocks per CU in the gradients (188
+                                                 // registers) and scores alone (244), one where E or z is kept (268)
 typedef TileCfg<128, 128, 2, 2, 32, 10> CfgDeep; // the same tile where one round of blocks does: nine stages under way
 typedef TileCfg<128, 128, 2, 4, 32, 3, 3> CfgF32; // three planes
 typedef TileCfg<128, 32, 2, 1, 64, 4> CfgSlim;   // few rows: bound by reading w

@@ -1,7 +1,8 @@
 """Softmax class head over many classes (``csrc/hip/head.hip``) + torch CPU path.
 
 Scores z = (x w^T + bias) / T of rows ``x`` [n, d] against classes ``w`` [V, d]. Rows are taken in pieces: at most
-``PIECE_BYTES`` of exponentials (or scores, head_topk) live at a time, however many rows and classes there are.
+``PIECE_BYTES`` of exponentials (or scores, head_topk) live at a time, or 256 rows of them where those are more
+(2, with gradients in float32 10, in head_topk 4 bytes per row and class).
 
 * :func:`softmax_head_loss`: per-row softmax cross entropy with the gradients of x, w and bias. With
   ``base_class`` one more class has score 0 and no weights (index V): the multiclass linear model's convention
@@ -13,7 +14,8 @@ Scores z = (x w^T + bias) / T of rows ``x`` [n, d] against classes ``w`` [V, d].
 
 float32 or bfloat16 (x, w and bias alike); any strides. float32 products run as six bf16 plane products
 (24-bit operands); all sums, softmax statistics and losses are 32 bits or more. On bf16 inputs the score
-gradient D = p - q is rounded to bf16 once before the two gradient products. Everything runs on the
+gradient D = p - q is rounded to bf16 once before the two gradient products, and a p below e^-27 of the largest in its group of 64
+classes counts as 0 there. Everything runs on the
 current stream of x's device without a host synchronisation, in a workspace of its own per call (torch's
 allocator), so calls on several streams and captured graphs do not share memory. Results are
 bitwise reproducible. Gradients are returned; nothing is recorded for autograd.
@@ -30,7 +32,7 @@ import torch
 
 from ._ext import hip, ptr, stream
 
-# bytes of exponentials (or scores, head_topk) that live at a time; rows beyond are taken in further pieces
+# bytes of exponentials (or scores, head_topk) that live at a time; rows beyond are taken in further pieces, of 256 rows at least
 PIECE_BYTES = 2 << 30
 FEW_ROWS = 128           # == kFewRows (head.hip)
 MAX_LIST = 256           # entries of a teacher's list, and k of head_topk
