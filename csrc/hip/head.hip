@@ -1212,7 +1212,7 @@ struct TopArgs {
   float* values;
   long long* classes;
   const float *norms, *norm_max;
-  double slack;         // Slack::c
+  float slack;          // Slack::c
 };
 
 // What a 32-bit score (before the division by T) of a row with squared norm xx may be off against classes of squared norm <= ww,
@@ -1220,12 +1220,14 @@ struct TopArgs {
 // The fp32 matrix product of 4 rounds after every product (c = d), the bf16 one of 16 after every four (against exact sums: at most
 // 5.3 units per instruction; c = d / 2 counts 8). Joined accumulators, cut planes and dropped plane pairs take less than 64 units.
 // ww is summed in fp32 (fp32 inputs: of the largest planes, at most 2^-8 off): 1.02 + d 2^-23 times it, and squares that underflow
-// are below 2^-125 each.
+// are below 2^-125 each. The roots are fp32's (a 64-bit root in the way of every row's answer costs 0.3 us), so xx is at least
+// 2^-120, and where it has no fp32 value the bound is infinite.
 struct Slack {
-  double xx, c;
-  int d;
+  float x, c, d;
+  __device__ __forceinline__ Slack(double xx, float c, int d) : x(__builtin_amdgcn_sqrtf(fmaxf((float)xx, 0x1p-120f))), c(c), d(d) {}
   __device__ __forceinline__ double operator()(float ww, double z) const {
-    return 0x1p-24 * (c * sqrt(xx * (ww * (1.02 + d * 0x1p-23) + d * 0x1p-125)) + 2.0 * z) + c * 0x1p-125;
+    const float w = __builtin_amdgcn_sqrtf(ww * (1.02f + d * 0x1p-23f) + d * 0x1p-125f);
+    return c * x * w * 0x1.001p-24f + (z * 0x1p-23 + c * 0x1p-125);
   }
 };
 
@@ -1298,7 +1300,7 @@ struct DotTag {
 };
 
 template <typename T>
-__global__ __launch_bounds__(1024) void topk_kernel(TopArgs p) {
+__global__ __launch_bounds__(1024, sizeof(T) == 4 ? 5 : 4) void topk_kernel(TopArgs p) {
   __shared__ unsigned long long keys[kTopList];
   __shared__ int hist[256], pick[3], cnt, wcnt[2][8][16];
   __shared__ int sel[kTopMax + kSpare + kSlack];
@@ -1484,28 +1486,28 @@ __global__ __launch_bounds__(1024) void topk_kernel(TopArgs p) {
   unsigned long long *bkey = &keys[kTurnList + kTurnList / 2], *nkey = bkey + kTopMax + kTopMax / 2;
   int *bcls = (int*)(bkey + kTopMax), *ncls = (int*)(nkey + kTopMax);
   static_assert(kTurnList + kTurnList / 2 + 3 * kTopMax <= kTopList, "");
-  float* values = p.values + (long long)row * p.k;
-  long long* classes = p.classes + (long long)row * p.k;
   for (int c = t; c < p.kc; c += nt) {
     const unsigned long long mine = keys[c];
     const int v = cls[c];
     int rank = 0;
 #pragma unroll 4
     for (int o = 0; o < p.kc; ++o) rank += keys[o] > mine || (keys[o] == mine && cls[o] < v);
-    if (rank < p.k) {
-      values[rank] = (float)(key_value(mine) * p.inv_t);
-      classes[rank] = v;
-      bkey[rank] = mine, bcls[rank] = v;
-    }
+    if (rank < p.k) bkey[rank] = mine, bcls[rank] = v;
   }
-  if (all) return;
   __syncthreads();
+  auto answer = [&]() {
+    for (int c = t; c < p.k; c += nt) {
+      p.values[(long long)row * p.k + c] = (float)(key_value(bkey[c]) * p.inv_t);
+      p.classes[(long long)row * p.k + c] = bcls[c];
+    }
+  };
+  if (all) return answer();
   double zk = key_value(bkey[p.k - 1]);
   const double zc = key_value((unsigned)(cut >> 32));
-  const Slack slack = {xx, p.slack, p.d};
+  const Slack slack(xx, p.slack, p.d);
   // (classes at -inf are switched off, in 64 bits too; comparisons with NaN are false: such a row has some classes)
   const float ww = fmaxf(fmaxf(ww4.x, ww4.y), fmaxf(ww4.z, ww4.w));
-  if (!(zk <= zc + slack(ww, fmax(fabs(zk), fabs(zc)))) || zc == -INFINITY) return;
+  if (!(zk <= zc + slack(ww, fmax(fabs(zk), fabs(zc)))) || zc == -INFINITY) return answer();
 
   // classes of this turn and their keys
   int* tcls = (int*)&keys[kTurnList];
@@ -1558,10 +1560,7 @@ __global__ __launch_bounds__(1024) void topk_kernel(TopArgs p) {
     }
   }
   merge();
-  for (int c = t; c < p.k; c += nt) {
-    values[c] = (float)(key_value(bkey[c]) * p.inv_t);
-    classes[c] = bcls[c];
-  }
+  answer();
 }
 
 // ------------------------------------------------------------------ host side
@@ -2139,7 +2138,7 @@ extern "C" void ytk_head_topk(const uintptr_t* ptrs, const long long* lp, double
     t.xrs = h.xrs, t.xcs = h.xcs, t.wrs = h.wrs, t.wcs = h.wcs;
     t.inv_t = 1.0 / temp_;
     t.norms = r.norms, t.norm_max = r.norm_max;
-    t.slack = (p.few ? 1.0 : 0.5) * h.d + 64.0;
+    t.slack = (p.few ? 1.0f : 0.5f) * (float)h.d + 64.0f;
     t.values = (float*)ptrs[4] + r0 * h.k;
     t.classes = (long long*)ptrs[5] + r0 * h.k;
     const int threads = rows < 256 ? 1024 : 256;  // fewer rows than CUs: more waves for each
