@@ -1222,9 +1222,15 @@ struct TopArgs {
 // ww is summed in fp32 (fp32 inputs: of the largest planes, at most 2^-8 off): 1.02 + d 2^-23 times it, and squares that underflow
 // are below 2^-125 each. The roots are fp32's (a 64-bit root in the way of every row's answer costs 0.3 us), so xx is at least
 // 2^-120, and where it has no fp32 value the bound is infinite.
+__device__ __forceinline__ float uniform(float v) {
+  return __builtin_bit_cast(float, __builtin_amdgcn_readfirstlane(__builtin_bit_cast(int, v)));
+}
+__device__ __forceinline__ unsigned long long uniform(unsigned long long v) {
+  return (unsigned long long)(unsigned)__builtin_amdgcn_readfirstlane((int)(v >> 32)) << 32 | (unsigned)__builtin_amdgcn_readfirstlane((int)v);
+}
 struct Slack {
   float x, c, d;
-  __device__ __forceinline__ Slack(double xx, float c, int d) : x(__builtin_amdgcn_sqrtf(fmaxf((float)xx, 0x1p-120f))), c(c), d(d) {}
+  __device__ __forceinline__ Slack(double xx, float c, int d) : x(uniform(__builtin_amdgcn_sqrtf(fmaxf((float)xx, 0x1p-120f)))), c(c), d(d) {}
   __device__ __forceinline__ double operator()(float ww, double z) const {
     const float w = __builtin_amdgcn_sqrtf(ww * (1.02f + d * 0x1p-23f) + d * 0x1p-125f);
     return c * x * w * 0x1.001p-24f + (z * 0x1p-23 + c * 0x1p-125);
@@ -1310,7 +1316,7 @@ __global__ __launch_bounds__(1024, sizeof(T) == 4 ? 5 : 4) void topk_kernel(TopA
   // 16 rows share a line of the stats: rows next to each other go to one XCD (4096 rows of 65536 classes 241 -> 234 us)
   const int row = (int)(blockIdx.x & 7) * (int)(gridDim.x >> 3) + (int)(blockIdx.x >> 3);
   if (row >= p.n) return;
-  const int t = threadIdx.x, nt = blockDim.x, wave = t >> 6, waves = nt >> 6, l = t & 63;
+  const int t = threadIdx.x, nt = blockDim.x, wave = __builtin_amdgcn_readfirstlane(t >> 6), waves = nt >> 6, l = t & 63;
   const float2* st = p.stats + row;
   const float* z = p.z + (long long)row * p.ld;
   auto gkey = [&](int g) { return order_key(st[(long long)g * p.n].x); };
@@ -1502,8 +1508,9 @@ __global__ __launch_bounds__(1024, sizeof(T) == 4 ? 5 : 4) void topk_kernel(TopA
     }
   };
   if (all) return answer();
-  double zk = key_value(bkey[p.k - 1]);
-  const double zc = key_value((unsigned)(cut >> 32));
+  double zk = key_value(uniform(bkey[p.k - 1]));
+  const unsigned long long last = uniform(cut);
+  const double zc = key_value((unsigned)(last >> 32));
   const Slack slack(xx, p.slack, p.d);
   // (classes at -inf are switched off, in 64 bits too; comparisons with NaN are false: such a row has some classes)
   const float ww = fmaxf(fmaxf(ww4.x, ww4.y), fmaxf(ww4.z, ww4.w));
@@ -1514,7 +1521,7 @@ __global__ __launch_bounds__(1024, sizeof(T) == 4 ? 5 : 4) void topk_kernel(TopA
   unsigned long long* tkey = keys;
   auto reach = [&](int g) { return zk - slack(p.norms[g], fabs(zk)); };  // what a score of group g has to reach
   auto merge = [&]() {  // all threads, with the list written; cnt is 0 afterwards
-    const int listed = cnt, total = p.k + listed;
+    const int listed = __builtin_amdgcn_readfirstlane(cnt), total = p.k + listed;
     dots(DotTag<4>(), tcls, listed, tkey, false);
     __syncthreads();
     auto keyed = [&](int e) { return e < p.k ? bkey[e] : tkey[e - p.k]; };
@@ -1531,7 +1538,7 @@ __global__ __launch_bounds__(1024, sizeof(T) == 4 ? 5 : 4) void topk_kernel(TopA
     unsigned long long* const k = bkey;
     int* const c = bcls;
     bkey = nkey, bcls = ncls, nkey = k, ncls = c;
-    zk = key_value(bkey[p.k - 1]);
+    zk = key_value(uniform(bkey[p.k - 1]));
   };
   __syncthreads();  // the candidates' keys have been read
   if (t == 0) cnt = 0;
@@ -1541,15 +1548,15 @@ __global__ __launch_bounds__(1024, sizeof(T) == 4 ? 5 : 4) void topk_kernel(TopA
     __syncthreads();
     if (t < 256 && g0 + t < p.groups && (double)st[(long long)(g0 + t) * p.n].x >= reach(g0 + t)) hist[atomicAdd(&pick[0], 1)] = g0 + t;
     __syncthreads();
-    const int listed = pick[0];
+    const int listed = __builtin_amdgcn_readfirstlane(pick[0]);
     for (int s0 = 0; s0 < listed; s0 += kTurnAdd / kGroup) {
-      const int have = cnt;
+      const int have = __builtin_amdgcn_readfirstlane(cnt);
       __syncthreads();  // every wave has read it before one adds to it: all merge or none
       if (have > kTurnList - kTurnAdd) merge();
       for (int u = wave; u < kTurnAdd / kGroup && s0 + u < listed; u += waves) {
         const int g = hist[s0 + u], v = g * kGroup + l;
         const float zv = z[min(v, p.V - 1)];
-        const bool take = v < p.V && (double)zv >= reach(g) && ((unsigned long long)order_key(zv) << 32 | (unsigned)~v) < cut;
+        const bool take = v < p.V && (double)zv >= reach(g) && ((unsigned long long)order_key(zv) << 32 | (unsigned)~v) < last;
         const unsigned long long m = __ballot(take);
         int base = 0;
         if (l == 0 && m) base = atomicAdd(&cnt, __popcll(m));
